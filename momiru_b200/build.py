@@ -13,9 +13,12 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB_DIR = os.path.join(HERE, "lib")
 LIB_PATH = os.path.join(LIB_DIR, "libmomiru_gemm.so")
-SOURCES = ["momiru_gemm.cu", "tc_strict_pair.cu", "tc_tf32_pair.cu", "tc_strict_1cta.cu", "tc_tf32_1cta.cu"]
+SOURCES = ["momiru_gemm.cu", "tc_strict_pair.cu", "tc_tf32_pair.cu", "tc_strict_1cta.cu", "tc_tf32_1cta.cu",
+           "ops.cu", "linear_strip.cu", "linear_pair_bf16.cu", "linear_pair_f16.cu"]
 HEADERS = ["ptx.cuh", "epilogue.cuh", "tc_gemm.cuh", "tc_gemm_2sm.cuh", "simt_gemm.cuh", "gemv.cuh", "gemv_tc.cuh", "fixup.cuh",
-           "tc_launch.h", "tc_launch.cuh", "launch.cuh"]
+           "tc_launch.h", "tc_launch.cuh", "launch.cuh", "linear_epi.cuh", "linear_strip.cuh", "linear_pair.cuh",
+           "linear_launch.h", "linear_pair_launch.cuh", "row_ops.cuh", "experts.cuh"]
+ABI_HEADERS = [os.path.join(HERE, "..", "include", f) for f in ("momiru_gemm.h", "momiru_ops.h")]
 OBJ_DIR = os.path.join(LIB_DIR, "obj")
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
@@ -37,7 +40,7 @@ def _stale() -> bool:
         return True
     t = os.path.getmtime(LIB_PATH)
     deps = [os.path.join(CSRC, f) for f in SOURCES + HEADERS]
-    deps.append(os.path.join(HERE, "..", "include", "momiru_gemm.h"))
+    deps += ABI_HEADERS
     return any(os.path.getmtime(d) > t for d in deps if os.path.exists(d))
 
 
@@ -45,7 +48,7 @@ def build(force: bool = False, verbose: bool = False, extra: list[str] | None = 
     if not force and not _stale():
         return LIB_PATH
     os.makedirs(OBJ_DIR, exist_ok=True)
-    headers = [os.path.join(CSRC, f) for f in HEADERS] + [os.path.join(HERE, "..", "include", "momiru_gemm.h")]
+    headers = [os.path.join(CSRC, f) for f in HEADERS] + ABI_HEADERS
     newest_header = max(os.path.getmtime(h) for h in headers if os.path.exists(h))
     objs, jobs = [], []
     for src in SOURCES:

@@ -43,6 +43,18 @@ int32_t fail(int32_t code, const char* fmt, ...) {
   return code;
 }
 
+}  // namespace
+
+namespace mmr {
+// The operators' unit reports its failures through the same per-thread message.
+int32_t set_last_error(int32_t code, const char* message) {
+  g_last_error = message;
+  return code;
+}
+}  // namespace mmr
+
+namespace {
+
 #define MMR_CUDA_TRY(expr)                                                                      \
   do {                                                                                          \
     cudaError_t e_ = (expr);                                                                    \

@@ -1,0 +1,1390 @@
+// ops.cu -- C ABI of the operators around the MatMul node (include/momiru_ops.h):
+// validation, kernel choice, TMA descriptors and workspaces at bind, and a run
+// that enqueues the steps bind laid down. Follows the bind / run / quiesce split
+// of momiru_gemm.cu, whose error message and f32 products it shares.
+#include <cuda.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <chrono>
+#include <cstdarg>
+#include <cstdint>
+#include <cstdio>
+#include <cstring>
+#include <functional>
+#include <initializer_list>
+#include <memory>
+#include <mutex>
+#include <new>
+#include <string>
+#include <thread>
+#include <vector>
+
+#include "../../include/momiru_ops.h"
+#include "experts.cuh"
+#include "launch.cuh"
+#include "linear_launch.h"
+#include "row_ops.cuh"
+
+namespace mmr {
+int32_t set_last_error(int32_t code, const char* message);  // momiru_gemm.cu
+}
+
+struct mmr_op_handle {
+  int device = 0;
+  int sms = 148;
+  cudaStream_t stream = nullptr, last_stream = nullptr;
+  struct Step {
+    std::string what;
+    std::function<int32_t(cudaStream_t)> launch;
+  };
+  std::vector<Step> steps;
+  std::string plan;
+  std::vector<void*> workspaces;
+  std::vector<mmr_gemm_handle*> products;  // f32 products of the MatMul node
+  int* d_err = nullptr;                    // device error word (256 bytes)
+  int* h_err = nullptr;                    // pinned copy
+  cudaEvent_t done = nullptr, err_ev = nullptr;
+  bool ran = false;      // `done` was recorded (a run outside stream capture)
+  bool launched = false;
+};
+
+namespace {
+
+using mmr::EpiMat;
+using Handle = mmr_op_handle;
+constexpr uint64_t kWaitNs = 2000000000ull;
+
+int32_t fail(int32_t code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof buf, fmt, ap);
+  va_end(ap);
+  return mmr::set_last_error(code, buf);
+}
+
+// Nothing throws across the C boundary.
+template <typename F>
+int32_t guarded(F&& f) {
+  try {
+    return f();
+  } catch (const std::bad_alloc&) {
+    return mmr::set_last_error(MMR_ERR_CUDA, "out of host memory");
+  } catch (...) {
+    return mmr::set_last_error(MMR_ERR_INVALID_ARGUMENT, "unexpected exception");
+  }
+}
+
+struct DeviceGuard {
+  int prev = -1;
+  bool ok = false;
+  explicit DeviceGuard(int dev) {
+    if (cudaGetDevice(&prev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) ok = true;
+  }
+  ~DeviceGuard() {
+    if (prev >= 0) cudaSetDevice(prev);
+  }
+};
+
+#define MMR_TRY(expr)                    \
+  do {                                   \
+    if (int32_t rc_ = (expr)) return rc_; \
+  } while (0)
+#define MMR_CUDA(expr)                                                                          \
+  do {                                                                                          \
+    cudaError_t e_ = (expr);                                                                    \
+    if (e_ != cudaSuccess) return fail(MMR_ERR_CUDA, "%s: %s", #expr, cudaGetErrorString(e_)); \
+  } while (0)
+
+// ---------------------------------------------------------------- tensors --
+bool present(const mmr_tensor& t) { return t.view.rank > 0; }
+
+int elem_size(int dtype) { return dtype == MMR_DTYPE_BF16 || dtype == MMR_DTYPE_F16 ? 2 : 4; }
+
+constexpr unsigned kF32 = 1u << MMR_DTYPE_F32, kBf16 = 1u << MMR_DTYPE_BF16, kF16 = 1u << MMR_DTYPE_F16,
+                   kI32 = 1u << MMR_DTYPE_I32;
+constexpr unsigned kHalf = kBf16 | kF16, kFloat = kHalf | kF32;
+
+const char* dtype_name(int d) {
+  switch (d) {
+    case MMR_DTYPE_F32: return "f32";
+    case MMR_DTYPE_BF16: return "bf16";
+    case MMR_DTYPE_F16: return "f16";
+    case MMR_DTYPE_I32: return "i32";
+    default: return "unknown";
+  }
+}
+
+// One checked operand: shape, bounds and the byte range it touches.
+struct Ref {
+  const char* name = "";
+  uint64_t base = 0;  // address of element [0, .., 0]
+  int rank = 0, es = 4, dtype = 0;
+  int64_t d[3] = {1, 1, 1}, s[3] = {0, 0, 0};
+  uint64_t lo = 0, hi = 0;  // [lo, hi) in bytes; empty when some extent is 0
+  uint64_t address = 0;
+  bool on = false;
+};
+
+// Reads `t` as a rank-`rank` operand of one of `dtypes`; axes are right-aligned
+// in Ref (a matrix is d[1] x d[2], a vector d[2]).
+int32_t read_tensor(const mmr_tensor& t, const char* name, int device, int rank, unsigned dtypes, Ref* r) {
+  const mmr_view& v = t.view;
+  r->name = name;
+  if (!present(t)) return fail(MMR_ERR_INVALID_ARGUMENT, "%s: missing", name);
+  if (t.dtype < 0 || t.dtype > MMR_DTYPE_I32 || !(dtypes >> t.dtype & 1u))
+    return fail(MMR_ERR_INVALID_ARGUMENT, "%s: element type %s is not taken here", name, dtype_name(t.dtype));
+  if (v.rank != rank) return fail(MMR_ERR_INVALID_SHAPE, "%s: rank %d, expected %d", name, v.rank, rank);
+  r->rank = rank;
+  r->dtype = t.dtype;
+  r->es = elem_size(t.dtype);
+  r->address = v.address;
+  r->on = true;
+  int64_t lo = 0, hi = 0;
+  bool empty = false;
+  for (int i = 0; i < rank; ++i) {
+    if (v.dims[i] < 0) return fail(MMR_ERR_INVALID_SHAPE, "%s: negative extent on axis %d", name, i);
+    if (v.dims[i] > (int64_t(1) << 31) - 1024)
+      return fail(MMR_ERR_INVALID_SHAPE, "%s: extent %lld on axis %d exceeds 2^31 - 1024", name, (long long)v.dims[i], i);
+    if (v.strides[i] > (int64_t(1) << 40) || v.strides[i] < -(int64_t(1) << 40))
+      return fail(MMR_ERR_UNSUPPORTED_LAYOUT, "%s: stride on axis %d beyond 2^40 elements", name, i);
+    r->d[3 - rank + i] = v.dims[i];
+    r->s[3 - rank + i] = v.strides[i];
+    if (v.dims[i] == 0) {
+      empty = true;
+      continue;
+    }
+    const int64_t reach = (v.dims[i] - 1) * v.strides[i];
+    (reach < 0 ? lo : hi) += reach;
+  }
+  if (v.base_offset_bytes % r->es || v.address % r->es)
+    return fail(MMR_ERR_UNSUPPORTED_LAYOUT, "%s: address or offset is not aligned to its %d-byte elements", name, r->es);
+  if (v.device_ordinal != device)
+    return fail(MMR_ERR_UNSUPPORTED_DEVICE, "%s: device ordinal %d differs from the operator's %d", name,
+                v.device_ordinal, device);
+  r->base = v.address + v.base_offset_bytes;
+  r->lo = r->hi = r->base;
+  if (!empty) {
+    if (v.address == 0) return fail(MMR_ERR_INVALID_ARGUMENT, "%s: null address", name);
+    if (int64_t(v.base_offset_bytes / r->es) + lo < 0)
+      return fail(MMR_ERR_OUT_OF_BOUNDS, "%s: a negative stride reaches before the buffer", name);
+    const uint64_t need = v.base_offset_bytes + uint64_t(hi + 1) * r->es;
+    if (need > v.bytes)
+      return fail(MMR_ERR_OUT_OF_BOUNDS, "%s: view needs %llu bytes but the buffer has %llu", name,
+                  (unsigned long long)need, (unsigned long long)v.bytes);
+    r->lo = r->base + uint64_t(lo * r->es);
+    r->hi = r->base + uint64_t((hi + 1) * r->es);
+  }
+  return MMR_OK;
+}
+
+int32_t want_dims(const Ref& r, std::initializer_list<int64_t> dims) {
+  int i = 3 - int(dims.size());
+  for (int64_t want : dims) {
+    if (r.d[i] != want)
+      return fail(MMR_ERR_INVALID_SHAPE, "%s: extent %lld on axis %d, expected %lld", r.name, (long long)r.d[i],
+                  i - (3 - r.rank), (long long)want);
+    ++i;
+  }
+  return MMR_OK;
+}
+
+int32_t same_dtype(const Ref& r, int dtype) {
+  if (r.dtype != dtype)
+    return fail(MMR_ERR_INVALID_ARGUMENT, "%s: element type %s where the other operands have %s", r.name,
+                dtype_name(r.dtype), dtype_name(dtype));
+  return MMR_OK;
+}
+
+// Whether two operands may share bytes. Two matrices that are column blocks of
+// one row pitch interleave without meeting, which their byte ranges cannot tell.
+bool overlap(const Ref& x, const Ref& y) {
+  if (x.lo == x.hi || y.lo == y.hi || x.lo >= y.hi || y.lo >= x.hi) return false;
+  if (x.rank == 2 && y.rank == 2 && x.es == y.es && x.s[2] == 1 && y.s[2] == 1 && x.s[1] == y.s[1] && x.s[1] > 0) {
+    const int64_t ld = x.s[1], gap = (int64_t(y.base) - int64_t(x.base)) / x.es;
+    const int64_t off = (gap % ld + ld) % ld;  // y's first column counted from x's
+    if (off >= x.d[2] && off + y.d[2] <= ld) return false;
+  }
+  return true;
+}
+bool same_view(const Ref& x, const Ref& y) {
+  return x.base == y.base && x.rank == y.rank && memcmp(x.d, y.d, sizeof x.d) == 0 && memcmp(x.s, y.s, sizeof x.s) == 0;
+}
+
+// An output's elements must be distinct: sorted by stride, each axis steps past
+// the whole extent of the finer ones.
+int32_t check_output(const Ref& o) {
+  if (o.lo == o.hi) return MMR_OK;
+  std::vector<std::pair<int64_t, int64_t>> ax;
+  for (int i = 0; i < 3; ++i)
+    if (o.d[i] > 1) ax.emplace_back(o.s[i] < 0 ? -o.s[i] : o.s[i], o.d[i]);
+  std::sort(ax.begin(), ax.end());
+  int64_t span = 1;
+  for (const auto& [stride, extent] : ax) {
+    if (stride < span) return fail(MMR_ERR_UNSAFE_ALIASING, "%s: the output's own elements overlap", o.name);
+    span += stride * (extent - 1);
+  }
+  return MMR_OK;
+}
+
+int32_t check_aliasing(std::initializer_list<const Ref*> outs, std::initializer_list<const Ref*> ins,
+                       const Ref* in_place = nullptr) {
+  for (const Ref* o : outs) {
+    if (!o->on) continue;
+    MMR_TRY(check_output(*o));
+    for (const Ref* i : ins)
+      if (i->on && overlap(*o, *i) && !(i == in_place && o == *outs.begin() && same_view(*o, *i)))
+        return fail(MMR_ERR_UNSAFE_ALIASING, "%s overlaps %s", o->name, i->name);
+    for (const Ref* q : outs)
+      if (q != o && q->on && overlap(*o, *q)) return fail(MMR_ERR_UNSAFE_ALIASING, "%s overlaps %s", o->name, q->name);
+  }
+  return MMR_OK;
+}
+
+// ----------------------------------------------------------------- device --
+int32_t check_device(int device, std::initializer_list<const Ref*> refs, int* sms) {
+  int ndev = 0;
+  if (cudaGetDeviceCount(&ndev) != cudaSuccess || ndev == 0) {
+    cudaGetLastError();
+    return fail(MMR_ERR_UNSUPPORTED_DEVICE, "no CUDA device is visible");
+  }
+  if (device < 0 || device >= ndev)
+    return fail(MMR_ERR_UNSUPPORTED_DEVICE, "device ordinal %d outside 0..%d", device, ndev - 1);
+  int major = 0, minor = 0;
+  MMR_CUDA(cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, device));
+  MMR_CUDA(cudaDeviceGetAttribute(&minor, cudaDevAttrComputeCapabilityMinor, device));
+  MMR_CUDA(cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, device));
+  if (major != 10 || minor != 0)
+    return fail(MMR_ERR_UNSUPPORTED_DEVICE, "device %d is sm_%d%d; this library is built for sm_100a", device, major,
+                minor);
+  for (const Ref* r : refs) {
+    if (!r->on || r->lo == r->hi) continue;
+    cudaPointerAttributes pa;
+    if (cudaPointerGetAttributes(&pa, reinterpret_cast<void*>(r->address)) != cudaSuccess) {
+      cudaGetLastError();
+      return fail(MMR_ERR_UNSUPPORTED_DEVICE, "%s: its address is not known to CUDA", r->name);
+    }
+    if ((pa.type != cudaMemoryTypeDevice && pa.type != cudaMemoryTypeManaged) || pa.device != device)
+      return fail(MMR_ERR_UNSUPPORTED_DEVICE, "%s: not memory of device %d", r->name, device);
+  }
+  return MMR_OK;
+}
+
+struct Destroy {
+  void operator()(Handle* h) const { mmr_op_destroy(h); }
+};
+using Owned = std::unique_ptr<Handle, Destroy>;
+
+int32_t new_handle(int device, int sms, void* stream, Owned* out) {
+  Owned h(new Handle());
+  h->device = device;
+  h->sms = sms;
+  h->stream = reinterpret_cast<cudaStream_t>(stream);
+  MMR_CUDA(cudaMalloc(&h->d_err, 256));
+  MMR_CUDA(cudaMemset(h->d_err, 0, 256));
+  MMR_CUDA(cudaHostAlloc(&h->h_err, sizeof(int), cudaHostAllocDefault));
+  *h->h_err = 0;
+  MMR_CUDA(cudaEventCreateWithFlags(&h->done, cudaEventDisableTiming));
+  MMR_CUDA(cudaEventCreateWithFlags(&h->err_ev, cudaEventDisableTiming));
+  *out = std::move(h);
+  return MMR_OK;
+}
+
+int32_t workspace(Handle* h, size_t bytes, void** out) {
+  void* p = nullptr;
+  const cudaError_t e = cudaMalloc(&p, std::max<size_t>(bytes, 256));
+  if (e != cudaSuccess) {
+    cudaGetLastError();
+    return fail(MMR_ERR_CUDA, "allocating a workspace of %zu bytes: %s", bytes, cudaGetErrorString(e));
+  }
+  h->workspaces.push_back(p);
+  *out = p;
+  return MMR_OK;
+}
+
+// Records a launch; `fn` returns the cudaError_t of the enqueue.
+template <typename F>
+void add_step(Handle* h, const char* fmt, F fn, long long a = 0, long long b = 0, long long c = 0) {
+  char buf[192];
+  snprintf(buf, sizeof buf, fmt, a, b, c);
+  std::string what = buf;
+  h->plan += what + "\n";
+  h->steps.push_back({what, [fn, what](cudaStream_t s) -> int32_t {
+                        const cudaError_t e = fn(s);
+                        return e == cudaSuccess ? MMR_OK : fail(MMR_ERR_CUDA, "%s: %s", what.c_str(), cudaGetErrorString(e));
+                      }});
+}
+
+// ------------------------------------------------------------ tensor maps --
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapEncodeTiled", &ptr, 12000, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<EncodeTiledFn>(ptr);
+  });
+  return fn;
+}
+
+// A 16-bit product operand as TMA reads it: `mn` rows or columns by `k`.
+struct Operand {
+  uint64_t base = 0;
+  int64_t mn = 0, k = 0, batch = 1;
+  int64_t s_mn = 0, s_k = 0, s_b = 0;
+  bool mn_major = false;
+};
+
+// 128-byte swizzled boxes: K-major 64 k x `rows` of mn, MN-major 64 mn x 64 k.
+int32_t encode16(CUtensorMap* tm, const Operand& o, int dtype, int rows, const char* name) {
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return fail(MMR_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const uint64_t inner = o.mn_major ? o.mn : o.k, outer = o.mn_major ? o.k : o.mn;
+  uint64_t pitch = uint64_t(o.mn_major ? o.s_k : o.s_mn) * 2;
+  if (outer <= 1) pitch = (inner * 2 + 15) & ~uint64_t(15);
+  uint64_t bpitch = uint64_t(o.s_b) * 2;
+  if (o.batch <= 1) bpitch = pitch * outer;
+  cuuint64_t dims[3] = {inner, outer, uint64_t(o.batch)};
+  cuuint64_t strides[2] = {pitch, bpitch};
+  cuuint32_t box[3] = {64, cuuint32_t(o.mn_major ? 64 : rows), 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r =
+      fn(tm, dtype == MMR_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
+         reinterpret_cast<void*>(o.base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS)
+    return fail(MMR_ERR_UNSUPPORTED_LAYOUT, "%s: cuTensorMapEncodeTiled failed (%d): dims {%llu,%llu,%llu}", name, int(r),
+                (unsigned long long)inner, (unsigned long long)outer, (unsigned long long)o.batch);
+  return MMR_OK;
+}
+
+bool tma_pitch(uint64_t base, int64_t pitch, int64_t extent, int64_t s_b, int64_t batch, int64_t inner) {
+  if (base % 16) return false;
+  if (extent > 1 && (pitch <= 0 || pitch % 8 || pitch < inner || pitch >= (int64_t(1) << 38))) return false;
+  return batch <= 1 || (s_b > 0 && s_b % 8 == 0 && s_b < (int64_t(1) << 38));
+}
+
+// Makes `o` readable by TMA: as it lies where it can, else packed by a step of
+// each run into rows of a 16-byte pitch. `major`: 0 any, 1 K-major only, 2
+// MN-major only.
+int32_t admit(Handle* h, Operand* o, int major, const char* name) {
+  if (o->mn == 0 || o->k == 0 || o->batch == 0) return MMR_OK;  // nothing is loaded
+  if (major != 2 && (o->s_k == 1 || o->k == 1) && tma_pitch(o->base, o->s_mn, o->mn, o->s_b, o->batch, o->k)) {
+    o->mn_major = false;
+    return MMR_OK;
+  }
+  if (major != 1 && (o->s_mn == 1 || o->mn == 1) && tma_pitch(o->base, o->s_k, o->k, o->s_b, o->batch, o->mn)) {
+    o->mn_major = true;
+    return MMR_OK;
+  }
+  const int64_t as_mn = std::abs(o->s_mn), as_k = std::abs(o->s_k);
+  const bool mn_major = major == 2 || (major == 0 && as_mn < as_k);
+  mmr::PackParams q;
+  q.src = reinterpret_cast<const void*>(o->base);
+  q.s_b = o->s_b;
+  q.rows = int(mn_major ? o->k : o->mn);
+  q.cols = int(mn_major ? o->mn : o->k);
+  q.s_r = mn_major ? o->s_k : o->s_mn;
+  q.s_c = mn_major ? o->s_mn : o->s_k;
+  q.pitch = (q.cols + 7) / 8 * 8;
+  if (o->batch > 65535) return fail(MMR_ERR_UNSUPPORTED_LAYOUT, "%s: more than 65535 matrices to pack", name);
+  const int64_t per = int64_t(q.rows) * q.pitch;
+  MMR_TRY(workspace(h, size_t(per) * o->batch * 2, &q.dst));
+  const int64_t tiles = int64_t((q.rows + 31) / 32) * ((q.pitch + 31) / 32);
+  const dim3 grid(unsigned(std::min<int64_t>(tiles, 8 * h->sms)), 1, unsigned(o->batch));
+  add_step(h, "mmr_pack_kernel grid %lld x %lld", [q, grid](cudaStream_t s) {
+    return mmr::launch_kernel(mmr::mmr_pack_kernel, grid, dim3(256), 0, s, dim3(1, 1, 1), q);
+  }, grid.x, grid.z);
+  o->base = reinterpret_cast<uint64_t>(q.dst);
+  o->mn_major = mn_major;
+  (mn_major ? o->s_k : o->s_mn) = q.pitch;
+  (mn_major ? o->s_mn : o->s_k) = 1;
+  o->s_b = per;
+  return MMR_OK;
+}
+
+// Never read by TMA: a valid descriptor for a product without any k-blocks.
+void no_operand(Handle* h, Operand* o) {
+  o->base = reinterpret_cast<uint64_t>(h->d_err);
+  o->mn = o->batch = 1;
+  o->k = o->s_mn = 64;
+  o->s_k = 1;
+  o->mn_major = false;
+}
+
+EpiMat epi_mat(const Ref& r) {
+  EpiMat m;
+  if (!r.on) return m;
+  m.p = reinterpret_cast<void*>(r.base);
+  m.bs = r.s[0];
+  m.ld = r.s[1];
+  m.cs = r.s[2];
+  const int per = 16 / r.es;
+  m.vec = (r.s[2] == 1 || r.d[2] == 1) && r.base % 16 == 0 && (r.s[1] % per == 0 || r.d[1] == 1) &&
+          (r.s[0] % per == 0 || r.d[0] == 1);
+  if (r.d[2] == 1) m.vec = 0;
+  return m;
+}
+
+// --------------------------------------------------------------- products --
+struct Groups {  // ragged rows or contraction
+  int experts = 0;
+  const int *offsets = nullptr, *counts = nullptr;
+  int64_t rows = 0, assignments = 0;
+};
+
+// Up to this many rows the weights' stream bounds the product and the strip
+// kernel takes it; above, the CTA pairs.
+constexpr int64_t kStripRows = 256;
+constexpr int64_t kStripRowsPerExpert = 96;
+
+int round16(int64_t v) { return int((v + 15) / 16 * 16); }
+
+// out[m, n] = epilogue(A[m, k] B[k, n]) in 16-bit operands; a.mn = m, b.mn = n.
+// With `g`, the experts' products over ragged rows (b batched).
+int32_t add_product(Handle* h, int dtype, Operand a, Operand b, mmr::EpiParams epi, const Groups* g) {
+  const bool bf16 = dtype == MMR_DTYPE_BF16;
+  const int64_t m = a.mn, n = b.mn, k = a.k;
+  epi.n = int(n);
+  if (m == 0 || n == 0) return MMR_OK;
+  const int k_blocks = int((k + 63) / 64);
+  const int64_t per_expert = g ? (g->assignments + g->experts - 1) / g->experts : 0;
+  const bool strip = g ? per_expert <= kStripRowsPerExpert : m <= kStripRows;
+  MMR_TRY(admit(h, &a, strip || g ? 1 : 0, "lhs"));
+  MMR_TRY(admit(h, &b, 0, "rhs"));
+  if (k == 0) {
+    no_operand(h, &a);
+    no_operand(h, &b);
+  }
+  CUtensorMap ta, tb;
+  if (strip) {
+    mmr::StripParams p;
+    p.m = int(m);
+    p.n = int(n);
+    p.k_blocks = k_blocks;
+    p.mt = 16;
+    const int64_t cover = g ? 2 * per_expert : m;
+    while (p.mt < 256 && p.mt < cover) p.mt *= 2;
+    if (!g) p.mt = std::min(p.mt, round16(m));
+    p.strips = int((n + mmr::LS_COLS - 1) / mmr::LS_COLS);
+    p.m_units = g ? int(std::min<int64_t>(g->experts, g->assignments) + g->assignments / p.mt)
+                  : int((m + p.mt - 1) / p.mt);
+    if (g) {
+      p.experts = g->experts;
+      p.offsets = g->offsets;
+      p.counts = g->counts;
+      p.rows = g->rows;
+    }
+    // Two CTAs of about 100 KB of stages share an SM.
+    const int64_t units = int64_t(p.strips) * (g ? std::min<int64_t>(g->experts, g->assignments) : p.m_units);
+    while (p.split < mmr::LS_MAX_SPLIT && units * p.split < 2 * h->sms && k_blocks >= 8 * p.split) p.split *= 2;
+    p.stages = p.mt > 128 ? 4 : std::min(mmr::LS_MAX_STAGES, 102400 / (mmr::LS_W_BYTES + p.mt * 128));
+    p.tmem_cols = 32;
+    while (p.tmem_cols < uint32_t(p.mt)) p.tmem_cols *= 2;
+    p.epi = epi;
+    p.err = h->d_err;
+    p.timeout_ns = kWaitNs;
+    MMR_TRY(encode16(&tb, b, dtype, mmr::LS_COLS, "rhs"));
+    MMR_TRY(encode16(&ta, a, dtype, p.mt, "lhs"));
+    const int64_t grid = int64_t(p.strips) * p.m_units * p.split;
+    if (grid > (int64_t(1) << 31) - 1) return fail(MMR_ERR_INVALID_SHAPE, "more than 2^31 units of work");
+    const int smem = mmr::strip_smem_bytes(p.mt, p.stages);
+    const bool w_mn = b.mn_major;
+    MMR_CUDA(mmr::strip_prepare(bf16, w_mn, smem));
+    add_step(h, "mmr_linear_strip_kernel grid %lld, split %lld, rows %lld", [=](cudaStream_t s) {
+      return mmr::strip_launch(bf16, w_mn, int(grid), smem, s, tb, ta, p);
+    }, grid, p.split, p.mt);
+    return MMR_OK;
+  }
+  mmr::PairParams p;
+  p.m = int(m);
+  p.n = int(n);
+  p.tiles_m = int((m + 255) / 256);
+  p.tiles_n = int((n + mmr::LP_BN - 1) / mmr::LP_BN);
+  p.k_blocks = k_blocks;
+  int64_t tiles = int64_t(p.tiles_m) * p.tiles_n;
+  if (g) {
+    p.experts = g->experts;
+    p.offsets = g->offsets;
+    p.counts = g->counts;
+    p.rows = g->rows;
+    tiles = (std::min<int64_t>(g->experts, g->assignments) + g->assignments / 256) * p.tiles_n;
+  }
+  if (tiles > (int64_t(1) << 31) - 1024) return fail(MMR_ERR_INVALID_SHAPE, "more than 2^31 output tiles");
+  p.tiles_total = int(tiles);
+  p.epi = epi;
+  p.err = h->d_err;
+  p.timeout_ns = kWaitNs;
+  MMR_TRY(encode16(&ta, a, dtype, 128, "lhs"));
+  MMR_TRY(encode16(&tb, b, dtype, 128, "rhs"));
+  const int rag = g ? 1 : 0;
+  const bool a_mn = a.mn_major, b_mn = b.mn_major;
+  const int grid = 2 * int(std::min<int64_t>(h->sms / 2, std::max<int64_t>(tiles, 1)));
+  MMR_CUDA(bf16 ? mmr::pair_prepare_bf16(a_mn, b_mn, rag) : mmr::pair_prepare_f16(a_mn, b_mn, rag));
+  add_step(h, "mmr_linear_pair_kernel grid %lld, tiles %lld, k-blocks %lld", [=](cudaStream_t s) {
+    return bf16 ? mmr::pair_launch_bf16(a_mn, b_mn, rag, grid, s, ta, tb, p)
+                : mmr::pair_launch_f16(a_mn, b_mn, rag, grid, s, ta, tb, p);
+  }, grid, tiles, k_blocks);
+  return MMR_OK;
+}
+
+// out[e] (m x n) = A_e^T B_e over the rows of each expert's segment.
+int32_t add_segment_product(Handle* h, int dtype, Operand a, Operand b, const EpiMat& out, const Groups& g) {
+  const bool bf16 = dtype == MMR_DTYPE_BF16;
+  mmr::PairParams p;
+  p.m = int(a.mn);
+  p.n = int(b.mn);
+  if (p.m == 0 || p.n == 0 || g.experts == 0) return MMR_OK;
+  MMR_TRY(admit(h, &a, 2, "rows"));
+  MMR_TRY(admit(h, &b, 2, "d_out"));
+  if (g.rows == 0) {
+    no_operand(h, &a);
+    no_operand(h, &b);
+  }
+  p.tiles_m = (p.m + 255) / 256;
+  p.tiles_n = (p.n + mmr::LP_BN - 1) / mmr::LP_BN;
+  const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n * g.experts;
+  if (tiles > (int64_t(1) << 31) - 1024) return fail(MMR_ERR_INVALID_SHAPE, "more than 2^31 output tiles");
+  p.tiles_total = int(tiles);
+  p.experts = g.experts;
+  p.offsets = g.offsets;
+  p.counts = g.counts;
+  p.rows = g.rows;
+  p.epi.out = out;
+  p.epi.n = p.n;
+  p.err = h->d_err;
+  p.timeout_ns = kWaitNs;
+  CUtensorMap ta, tb;
+  MMR_TRY(encode16(&ta, a, dtype, 128, "rows"));
+  MMR_TRY(encode16(&tb, b, dtype, 128, "d_out"));
+  const int grid = 2 * int(std::min<int64_t>(h->sms / 2, tiles));
+  MMR_CUDA(bf16 ? mmr::pair_prepare_bf16(true, true, 2) : mmr::pair_prepare_f16(true, true, 2));
+  add_step(h, "mmr_linear_pair_kernel (segments) grid %lld, tiles %lld", [=](cudaStream_t s) {
+    return bf16 ? mmr::pair_launch_bf16(true, true, 2, grid, s, ta, tb, p)
+                : mmr::pair_launch_f16(true, true, 2, grid, s, ta, tb, p);
+  }, grid, tiles);
+  return MMR_OK;
+}
+
+// d_pre (and d_bias) from d_out and pre. Fills `d_pre` with the view that the
+// products read: d_out itself without an activation, else a workspace.
+int32_t add_act_grad(Handle* h, int act, const Ref& d_out, const Ref& pre, const Ref& d_bias, Ref* d_pre,
+                     const Groups* g, const int* sources) {
+  const int64_t rows = d_out.d[1], n = d_out.d[2];
+  *d_pre = d_out;
+  const bool through = act != MMR_ACT_NONE;
+  if (n == 0 || (!through && !d_bias.on)) return MMR_OK;
+  mmr::ActGradParams p;
+  p.d_out = epi_mat(d_out);
+  p.rows = rows;
+  p.n = int(n);
+  p.act = act;
+  p.sources = sources;
+  const int64_t chunks = (rows + mmr::AG_ROWS - 1) / mmr::AG_ROWS;
+  if (through) {
+    p.pre = epi_mat(pre);
+    d_pre->s[2] = 1;
+    d_pre->s[1] = (n + 7) / 8 * 8;
+    void* w = nullptr;
+    MMR_TRY(workspace(h, size_t(rows) * d_pre->s[1] * d_out.es, &w));
+    d_pre->base = reinterpret_cast<uint64_t>(w);
+    d_pre->name = "d_pre";
+    p.d_pre = epi_mat(*d_pre);
+  }
+  if (d_bias.on) {
+    void* w = nullptr;
+    MMR_TRY(workspace(h, size_t(chunks) * n * sizeof(float), &w));
+    p.partial = static_cast<float*>(w);
+  }
+  const int dt = d_out.dtype;
+  const dim3 grid(unsigned((n + mmr::AG_COLS - 1) / mmr::AG_COLS), unsigned(std::min<int64_t>(std::max<int64_t>(chunks, 1), 65535)));
+  if (rows > 0)
+    add_step(h, "mmr_act_grad_kernel grid %lld x %lld", [=](cudaStream_t s) {
+      auto k = dt == MMR_DTYPE_F32    ? mmr::mmr_act_grad_kernel<float>
+               : dt == MMR_DTYPE_BF16 ? mmr::mmr_act_grad_kernel<__nv_bfloat16>
+                                      : mmr::mmr_act_grad_kernel<__half>;
+      return mmr::launch_kernel(k, grid, dim3(256), 0, s, dim3(1, 1, 1), p);
+    }, grid.x, grid.y);
+  if (d_bias.on) {
+    mmr::ColSumParams c;
+    c.partial = p.partial;
+    c.out = reinterpret_cast<void*>(d_bias.base);
+    c.out_bs = d_bias.s[1];
+    c.out_s = d_bias.s[2];
+    c.n = int(n);
+    c.chunks = int(chunks);
+    c.offsets = g ? g->offsets : nullptr;
+    const dim3 cg(unsigned((n + 31) / 32), unsigned(g ? g->experts : 1));
+    add_step(h, "mmr_col_sum_kernel grid %lld x %lld", [=](cudaStream_t s) {
+      auto k = dt == MMR_DTYPE_F32    ? mmr::mmr_col_sum_kernel<float>
+               : dt == MMR_DTYPE_BF16 ? mmr::mmr_col_sum_kernel<__nv_bfloat16>
+                                      : mmr::mmr_col_sum_kernel<__half>;
+      return mmr::launch_kernel(k, cg, dim3(256), 0, s, dim3(1, 1, 1), c);
+    }, cg.x, cg.y);
+  }
+  return MMR_OK;
+}
+
+// ------------------------------------------------- f32 through the MatMul node --
+mmr_view f32_view(uint64_t base, int64_t rows, int64_t cols, int64_t s_r, int64_t s_c, int device, uint64_t lo,
+                  uint64_t hi) {
+  mmr_view v{};
+  v.address = lo;  // the view's own bytes: bounds were checked against its buffer
+  v.bytes = hi - lo;
+  v.base_offset_bytes = base - lo;
+  v.rank = 2;
+  v.device_ordinal = device;
+  v.dims[0] = rows;
+  v.dims[1] = cols;
+  v.strides[0] = s_r;
+  v.strides[1] = s_c;
+  return v;
+}
+mmr_view f32_view(const Ref& r, int device) {
+  return f32_view(r.base, r.d[1], r.d[2], r.s[1], r.s[2], device, r.lo, r.hi);
+}
+// A dense workspace matrix.
+mmr_view f32_view(const void* p, int64_t rows, int64_t cols, int64_t ld, int device) {
+  const uint64_t b = reinterpret_cast<uint64_t>(p);
+  return f32_view(b, rows, cols, ld, 1, device, b, b + 4 * uint64_t(rows) * ld);
+}
+mmr_view transposed(mmr_view v) {
+  std::swap(v.dims[0], v.dims[1]);
+  std::swap(v.strides[0], v.strides[1]);
+  return v;
+}
+
+int32_t add_f32_product(Handle* h, int math, const mmr_view& lhs, const mmr_view& rhs, const mmr_view& out,
+                        const Ref* bias, int epilogue) {
+  mmr_matmul_desc d{};
+  d.lhs = lhs;
+  d.rhs = rhs;
+  d.out = out;
+  if (bias && bias->on) {
+    d.bias.address = bias->lo;
+    d.bias.bytes = bias->hi - bias->lo;
+    d.bias.base_offset_bytes = bias->base - bias->lo;
+    d.bias.rank = 1;
+    d.bias.device_ordinal = h->device;
+    d.bias.dims[0] = bias->d[2];
+    d.bias.strides[0] = bias->s[2];
+  }
+  d.math_mode = math;
+  d.epilogue = epilogue;
+  d.family = MMR_FAMILY_AUTO;
+  d.device_ordinal = h->device;
+  d.stream = h->stream;
+  mmr_gemm_handle* g = nullptr;
+  MMR_TRY(mmr_gemm_bind(&d, &g));
+  h->products.push_back(g);
+  h->plan += "matmul node (f32)\n";
+  h->steps.push_back({"matmul node (f32)", [g](cudaStream_t s) { return mmr_gemm_run_on(g, s); }});
+  return MMR_OK;
+}
+
+int f32_epilogue(int act, bool bias) {
+  switch (act) {
+    case MMR_ACT_RELU: return bias ? MMR_EPI_BIAS_RELU : MMR_EPI_RELU;
+    case MMR_ACT_RELU6: return bias ? MMR_EPI_BIAS_RELU6 : MMR_EPI_RELU6;
+    case MMR_ACT_GELU_ERF: return bias ? MMR_EPI_BIAS_GELU_ERF : MMR_EPI_GELU_ERF;
+    case MMR_ACT_GELU_TANH: return bias ? MMR_EPI_BIAS_GELU_TANH : MMR_EPI_GELU_TANH;
+    case MMR_ACT_SILU: return bias ? MMR_EPI_BIAS_SILU : MMR_EPI_SILU;
+    default: return bias ? MMR_EPI_BIAS : MMR_EPI_NONE;
+  }
+}
+
+int32_t check_math(int dtype, int math) {
+  if (math < MMR_MATH_STRICT_FP32 || math > MMR_MATH_EXACT) return fail(MMR_ERR_INVALID_ARGUMENT, "unknown math mode %d", math);
+  if (dtype != MMR_DTYPE_F32 && math != MMR_MATH_STRICT_FP32)
+    return fail(MMR_ERR_UNSUPPORTED_MATH, "%s operands are multiplied exactly with f32 sums: the math mode is StrictFp32",
+                dtype_name(dtype));
+  return MMR_OK;
+}
+
+int32_t check_act(int act) {
+  if (act < MMR_ACT_NONE || act > MMR_ACT_SILU) return fail(MMR_ERR_INVALID_ARGUMENT, "unknown activation %d", act);
+  return MMR_OK;
+}
+
+// The logical matrix of a view given transposed.
+void untranspose(Ref* r) {
+  std::swap(r->d[1], r->d[2]);
+  std::swap(r->s[1], r->s[2]);
+}
+
+Operand operand(const Ref& r, bool rows_are_mn) {
+  Operand o;
+  o.base = r.base;
+  o.mn = rows_are_mn ? r.d[1] : r.d[2];
+  o.k = rows_are_mn ? r.d[2] : r.d[1];
+  o.s_mn = rows_are_mn ? r.s[1] : r.s[2];
+  o.s_k = rows_are_mn ? r.s[2] : r.s[1];
+  return o;
+}
+
+// out = A B with no bias, activation or residual; written along out's unit
+// stride (out^T = B^T A^T where that is the row axis).
+int32_t add_plain_product(Handle* h, int dtype, Operand a, Operand b, Ref out) {
+  if (out.s[2] != 1 && out.s[1] == 1) {
+    std::swap(a, b);
+    untranspose(&out);
+  }
+  mmr::EpiParams epi;
+  epi.out = epi_mat(out);
+  return add_product(h, dtype, a, b, epi, nullptr);
+}
+
+// ----------------------------------------------------------------- linear --
+int32_t linear_bind(const mmr_linear_desc* d, Handle** out) {
+  if (!out) return fail(MMR_ERR_INVALID_ARGUMENT, "null output handle pointer");
+  *out = nullptr;
+  if (!d) return fail(MMR_ERR_INVALID_ARGUMENT, "null descriptor");
+  const int dev = d->device_ordinal;
+  Ref lhs, rhs, o, bias, res, pre;
+  MMR_TRY(check_act(d->activation));
+  MMR_TRY(read_tensor(d->lhs, "lhs", dev, 2, kFloat, &lhs));
+  MMR_TRY(check_math(lhs.dtype, d->math_mode));
+  MMR_TRY(read_tensor(d->rhs, "rhs", dev, 2, kFloat, &rhs));
+  MMR_TRY(read_tensor(d->out, "out", dev, 2, kFloat, &o));
+  if (present(d->bias)) MMR_TRY(read_tensor(d->bias, "bias", dev, 1, kFloat, &bias));
+  if (present(d->residual)) MMR_TRY(read_tensor(d->residual, "residual", dev, 2, kFloat, &res));
+  if (present(d->pre)) MMR_TRY(read_tensor(d->pre, "pre", dev, 2, kFloat, &pre));
+  for (const Ref* r : {&rhs, &o, &bias, &res, &pre})
+    if (r->on) MMR_TRY(same_dtype(*r, lhs.dtype));
+  if (d->transpose_lhs) untranspose(&lhs);
+  if (d->transpose_rhs) untranspose(&rhs);
+  const int64_t m = lhs.d[1], k = lhs.d[2], n = rhs.d[2];
+  MMR_TRY(want_dims(rhs, {k, n}));
+  MMR_TRY(want_dims(o, {m, n}));
+  if (bias.on) MMR_TRY(want_dims(bias, {n}));
+  if (res.on) MMR_TRY(want_dims(res, {m, n}));
+  if (pre.on) MMR_TRY(want_dims(pre, {m, n}));
+  MMR_TRY(check_aliasing({&o, &pre}, {&lhs, &rhs, &bias, &res}, &res));
+  int sms = 0;
+  MMR_TRY(check_device(dev, {&lhs, &rhs, &o, &bias, &res, &pre}, &sms));
+  DeviceGuard guard(dev);
+  if (!guard.ok) return fail(MMR_ERR_CUDA, "cudaSetDevice(%d) failed", dev);
+  Owned h;
+  MMR_TRY(new_handle(dev, sms, d->stream, &h));
+  if (m == 0 || n == 0) {
+    *out = h.release();
+    return MMR_OK;
+  }
+  if (lhs.dtype == MMR_DTYPE_F32) {
+    if (!res.on && !pre.on) {
+      MMR_TRY(add_f32_product(h.get(), d->math_mode, f32_view(lhs, dev), f32_view(rhs, dev), f32_view(o, dev), &bias,
+                              f32_epilogue(d->activation, bias.on)));
+    } else {
+      // The node leaves pre in its own buffer (or a workspace), and one pass
+      // applies the activation and adds the residual.
+      mmr::ActResParams q;
+      mmr_view to;
+      if (pre.on) {
+        to = f32_view(pre, dev);
+        q.pre = reinterpret_cast<const float*>(pre.base);
+        q.pre_ld = pre.s[1];
+        q.pre_cs = pre.s[2];
+      } else {
+        void* w = nullptr;
+        const int64_t ld = (n + 3) / 4 * 4;
+        MMR_TRY(workspace(h.get(), size_t(m) * ld * 4, &w));
+        to = f32_view(w, m, n, ld, dev);
+        q.pre = static_cast<const float*>(w);
+        q.pre_ld = ld;
+        q.pre_cs = 1;
+      }
+      MMR_TRY(add_f32_product(h.get(), d->math_mode, f32_view(lhs, dev), f32_view(rhs, dev), to, &bias,
+                              f32_epilogue(MMR_ACT_NONE, bias.on)));
+      q.residual = reinterpret_cast<const float*>(res.on ? res.base : 0);
+      q.res_ld = res.s[1];
+      q.res_cs = res.s[2];
+      q.out = reinterpret_cast<float*>(o.base);
+      q.out_ld = o.s[1];
+      q.out_cs = o.s[2];
+      q.m = int(m);
+      q.n = int(n);
+      q.act = d->activation;
+      const int grid = int(std::min<int64_t>((m * n + 255) / 256, 16 * sms));
+      add_step(h.get(), "mmr_act_res_kernel grid %lld", [=](cudaStream_t s) {
+        return mmr::launch_kernel(mmr::mmr_act_res_kernel, dim3(grid), dim3(256), 0, s, dim3(1, 1, 1), q);
+      }, grid);
+    }
+  } else {
+    mmr::EpiParams epi;
+    epi.out = epi_mat(o);
+    epi.pre = epi_mat(pre);
+    epi.residual = epi_mat(res);
+    epi.bias = reinterpret_cast<const void*>(bias.on ? bias.base : 0);
+    epi.bias_s = bias.s[2];
+    epi.act = d->activation;
+    MMR_TRY(add_product(h.get(), lhs.dtype, operand(lhs, true), operand(rhs, false), epi, nullptr));
+  }
+  *out = h.release();
+  return MMR_OK;
+}
+
+int32_t linear_grad_bind(const mmr_linear_grad_desc* d, Handle** out) {
+  if (!out) return fail(MMR_ERR_INVALID_ARGUMENT, "null output handle pointer");
+  *out = nullptr;
+  if (!d) return fail(MMR_ERR_INVALID_ARGUMENT, "null descriptor");
+  const int dev = d->device_ordinal;
+  Ref dy, lhs, rhs, pre, dl, dr, db;
+  MMR_TRY(check_act(d->activation));
+  MMR_TRY(read_tensor(d->d_out, "d_out", dev, 2, kFloat, &dy));
+  MMR_TRY(check_math(dy.dtype, d->math_mode));
+  MMR_TRY(read_tensor(d->lhs, "lhs", dev, 2, kFloat, &lhs));
+  MMR_TRY(read_tensor(d->rhs, "rhs", dev, 2, kFloat, &rhs));
+  if (d->activation != MMR_ACT_NONE) MMR_TRY(read_tensor(d->pre, "pre", dev, 2, kFloat, &pre));
+  if (present(d->d_lhs)) MMR_TRY(read_tensor(d->d_lhs, "d_lhs", dev, 2, kFloat, &dl));
+  if (present(d->d_rhs)) MMR_TRY(read_tensor(d->d_rhs, "d_rhs", dev, 2, kFloat, &dr));
+  if (present(d->d_bias)) MMR_TRY(read_tensor(d->d_bias, "d_bias", dev, 1, kFloat, &db));
+  if (!dl.on && !dr.on && !db.on) return fail(MMR_ERR_INVALID_ARGUMENT, "no gradient is asked for");
+  for (const Ref* r : {&lhs, &rhs, &pre, &dl, &dr, &db})
+    if (r->on) MMR_TRY(same_dtype(*r, dy.dtype));
+  if (d->transpose_lhs) {
+    untranspose(&lhs);
+    untranspose(&dl);
+  }
+  if (d->transpose_rhs) {
+    untranspose(&rhs);
+    untranspose(&dr);
+  }
+  const int64_t m = lhs.d[1], k = lhs.d[2], n = rhs.d[2];
+  MMR_TRY(want_dims(rhs, {k, n}));
+  MMR_TRY(want_dims(dy, {m, n}));
+  if (pre.on) MMR_TRY(want_dims(pre, {m, n}));
+  if (dl.on) MMR_TRY(want_dims(dl, {m, k}));
+  if (dr.on) MMR_TRY(want_dims(dr, {k, n}));
+  if (db.on) MMR_TRY(want_dims(db, {n}));
+  MMR_TRY(check_aliasing({&dl, &dr, &db}, {&dy, &lhs, &rhs, &pre}));
+  int sms = 0;
+  MMR_TRY(check_device(dev, {&dy, &lhs, &rhs, &pre, &dl, &dr, &db}, &sms));
+  DeviceGuard guard(dev);
+  if (!guard.ok) return fail(MMR_ERR_CUDA, "cudaSetDevice(%d) failed", dev);
+  Owned h;
+  MMR_TRY(new_handle(dev, sms, d->stream, &h));
+  Ref dp;
+  MMR_TRY(add_act_grad(h.get(), d->activation, dy, pre, db, &dp, nullptr, nullptr));
+  if (dy.dtype == MMR_DTYPE_F32) {
+    mmr_view dpv = d->activation == MMR_ACT_NONE ? f32_view(dy, dev)
+                                                 : f32_view(reinterpret_cast<const void*>(dp.base), m, n, dp.s[1], dev);
+    // out^T = B^T A^T where the gradient's unit stride is its row axis
+    auto product = [&](mmr_view a, mmr_view b, const Ref& o) -> int32_t {
+      if (o.lo == o.hi) return MMR_OK;
+      mmr_view v = f32_view(o, dev);
+      if (o.s[2] != 1 && o.s[1] == 1) {
+        std::swap(a, b);
+        a = transposed(a);
+        b = transposed(b);
+        v = transposed(v);
+      }
+      return add_f32_product(h.get(), d->math_mode, a, b, v, nullptr, MMR_EPI_NONE);
+    };
+    if (dl.on) MMR_TRY(product(dpv, transposed(f32_view(rhs, dev)), dl));
+    if (dr.on) MMR_TRY(product(transposed(f32_view(lhs, dev)), dpv, dr));
+  } else {
+    if (dl.on) MMR_TRY(add_plain_product(h.get(), dy.dtype, operand(dp, true), operand(rhs, true), dl));
+    if (dr.on) MMR_TRY(add_plain_product(h.get(), dy.dtype, operand(lhs, false), operand(dp, false), dr));
+  }
+  *out = h.release();
+  return MMR_OK;
+}
+
+// ---------------------------------------------------------------- experts --
+int32_t expert_rows(int64_t tokens, int64_t top_k, int64_t experts, int64_t align, int64_t* rows) {
+  if (tokens < 0 || top_k < 1 || top_k > 1024 || experts < 1 || experts > mmr::ES_MAX_EXPERTS)
+    return fail(MMR_ERR_INVALID_SHAPE, "expert layout of %lld tokens, %lld choices, %lld experts: 1..1024 choices and 1..%d experts",
+                (long long)tokens, (long long)top_k, (long long)experts, mmr::ES_MAX_EXPERTS);
+  if (align < 1 || align > 128 || (align & (align - 1)))
+    return fail(MMR_ERR_INVALID_ARGUMENT, "row_align %lld is not a power of two up to 128", (long long)align);
+  if (tokens > ((int64_t(1) << 31) - (1 << 18)) / top_k)
+    return fail(MMR_ERR_INVALID_SHAPE, "more than 2^31 assignments");
+  const int64_t n = tokens * top_k;
+  *rows = (n + std::min(experts, n) * (align - 1)) / align * align;
+  return MMR_OK;
+}
+
+struct Layout {
+  Ref slots, sources, offsets, counts;
+  int64_t tokens = 0, top_k = 0, experts = 0, align = 1, rows = 0;
+  int* p(const Ref& r) const { return reinterpret_cast<int*>(r.base); }
+  Groups groups() const {
+    Groups g;
+    g.experts = int(experts);
+    g.offsets = p(offsets);
+    g.counts = p(counts);
+    g.rows = rows;
+    g.assignments = tokens * top_k;
+    return g;
+  }
+};
+
+int32_t read_layout(const mmr_expert_layout& l, int dev, Layout* o) {
+  MMR_TRY(expert_rows(l.tokens, l.top_k, l.experts, l.row_align, &o->rows));
+  o->tokens = l.tokens;
+  o->top_k = l.top_k;
+  o->experts = l.experts;
+  o->align = l.row_align;
+  MMR_TRY(read_tensor(l.slots, "slots", dev, 2, kI32, &o->slots));
+  MMR_TRY(read_tensor(l.sources, "sources", dev, 1, kI32, &o->sources));
+  MMR_TRY(read_tensor(l.offsets, "offsets", dev, 1, kI32, &o->offsets));
+  MMR_TRY(read_tensor(l.counts, "counts", dev, 1, kI32, &o->counts));
+  MMR_TRY(want_dims(o->slots, {o->tokens, o->top_k}));
+  MMR_TRY(want_dims(o->sources, {o->rows}));
+  MMR_TRY(want_dims(o->offsets, {o->experts + 1}));
+  MMR_TRY(want_dims(o->counts, {o->experts}));
+  for (const Ref* r : {&o->slots, &o->sources, &o->offsets, &o->counts})
+    if ((r->d[2] > 1 && r->s[2] != 1) || (r->rank == 2 && r->d[1] > 1 && r->s[1] != r->d[2]))
+      return fail(MMR_ERR_UNSUPPORTED_LAYOUT, "%s: the layout's arrays are contiguous", r->name);
+  return MMR_OK;
+}
+
+// The row length in vectors of the widest kind that every row allows, and that
+// kind's bytes: 16, 8, 4 or (16-bit types) 2.
+int32_t row_vector(std::initializer_list<const Ref*> refs, int64_t width, int* vb) {
+  *vb = 16;
+  for (const Ref* r : refs) {
+    if (!r->on) continue;
+    if (r->d[2] > 1 && r->s[2] != 1)
+      return fail(MMR_ERR_UNSUPPORTED_LAYOUT, "%s: rows must have unit column stride", r->name);
+    while (r->base % *vb || (r->d[1] > 1 && (r->s[1] * r->es) % *vb) || (width * r->es) % *vb) *vb /= 2;
+  }
+  return MMR_OK;
+}
+
+mmr::RowMat row_mat(const Ref& r) {
+  mmr::RowMat m;
+  if (!r.on) return m;
+  m.p = reinterpret_cast<void*>(r.base);
+  m.ld = r.s[1] * r.es;
+  return m;
+}
+
+int32_t dispatch_bind(const mmr_dispatch_desc* d, Handle** out) {
+  if (!out) return fail(MMR_ERR_INVALID_ARGUMENT, "null output handle pointer");
+  *out = nullptr;
+  if (!d) return fail(MMR_ERR_INVALID_ARGUMENT, "null descriptor");
+  const int dev = d->device_ordinal;
+  Layout l;
+  Ref ids, x, rows;
+  MMR_TRY(read_layout(d->layout, dev, &l));
+  MMR_TRY(read_tensor(d->ids, "ids", dev, 2, kI32, &ids));
+  MMR_TRY(read_tensor(d->x, "x", dev, 2, kFloat, &x));
+  MMR_TRY(read_tensor(d->rows, "rows", dev, 2, kFloat, &rows));
+  MMR_TRY(same_dtype(rows, x.dtype));
+  const int64_t width = x.d[2];
+  MMR_TRY(want_dims(ids, {l.tokens, l.top_k}));
+  MMR_TRY(want_dims(x, {l.tokens, width}));
+  MMR_TRY(want_dims(rows, {l.rows, width}));
+  MMR_TRY(check_aliasing({&rows, &l.slots, &l.sources, &l.offsets, &l.counts}, {&ids, &x}));
+  int vb = 16;
+  MMR_TRY(row_vector({&x, &rows}, width, &vb));
+  int sms = 0;
+  MMR_TRY(check_device(dev, {&ids, &x, &rows, &l.slots, &l.sources, &l.offsets, &l.counts}, &sms));
+  DeviceGuard guard(dev);
+  if (!guard.ok) return fail(MMR_ERR_CUDA, "cudaSetDevice(%d) failed", dev);
+  Owned h;
+  MMR_TRY(new_handle(dev, sms, d->stream, &h));
+  mmr::DispatchParams p;
+  p.ids = reinterpret_cast<const int*>(ids.base);
+  p.ids_t = ids.s[1];
+  p.ids_j = ids.s[2];
+  p.tokens = int(l.tokens);
+  p.top_k = int(l.top_k);
+  p.experts = int(l.experts);
+  p.align = int(l.align);
+  p.rows = l.rows;
+  p.slots = l.p(l.slots);
+  p.sources = l.p(l.sources);
+  p.offsets = l.p(l.offsets);
+  p.counts = l.p(l.counts);
+  p.x = row_mat(x);
+  p.out = row_mat(rows);
+  p.row_vecs = int(width * x.es / vb);
+  // Enough CTAs to fill the GPU twice over, a whole number of tokens each.
+  p.run = int(std::max<int64_t>(1, (l.tokens + 2 * sms - 1) / (2 * sms)));
+  const int64_t need = (l.tokens + p.run - 1) / p.run;
+  const int grid = int(std::max<int64_t>(need, std::min<int64_t>(2 * sms, 1 + l.rows / mmr::ES_WARPS)));
+  if (l.tokens * l.top_k > mmr::ES_DIRECT) {
+    void* w = nullptr;
+    MMR_TRY(workspace(h.get(), size_t(grid) * l.experts * 4, &w));
+    p.hist = static_cast<int*>(w);
+    add_step(h.get(), "mmr_expert_hist_kernel grid %lld", [=](cudaStream_t s) {
+      return mmr::launch_kernel(mmr::mmr_expert_hist_kernel, dim3(grid), dim3(mmr::ES_THREADS), p.experts * 4, s,
+                                dim3(1, 1, 1), p);
+    }, grid);
+  }
+  const int smem = mmr::dispatch_smem_bytes(p.experts);
+  auto kernel = vb == 16 ? mmr::mmr_dispatch_kernel<16> : vb == 8 ? mmr::mmr_dispatch_kernel<8>
+                : vb == 4 ? mmr::mmr_dispatch_kernel<4> : mmr::mmr_dispatch_kernel<2>;
+  if (smem > 48 * 1024)
+    MMR_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  add_step(h.get(), "mmr_dispatch_kernel grid %lld, %lld-byte vectors", [=](cudaStream_t s) {
+    return mmr::launch_kernel(kernel, dim3(grid), dim3(mmr::ES_THREADS), smem, s, dim3(1, 1, 1), p);
+  }, grid, vb);
+  *out = h.release();
+  return MMR_OK;
+}
+
+// Picks the kernel for an element type and vector width.
+#define MMR_PICK(KERNEL, dt, vb)                                                                              \
+  ((dt) == MMR_DTYPE_F32                                                                                      \
+       ? ((vb) == 16 ? KERNEL<float, 16> : (vb) == 8 ? KERNEL<float, 8> : KERNEL<float, 4>)                   \
+   : (dt) == MMR_DTYPE_BF16                                                                                   \
+       ? ((vb) == 16 ? KERNEL<__nv_bfloat16, 16> : (vb) == 8 ? KERNEL<__nv_bfloat16, 8>                       \
+          : (vb) == 4 ? KERNEL<__nv_bfloat16, 4> : KERNEL<__nv_bfloat16, 2>)                                  \
+       : ((vb) == 16 ? KERNEL<__half, 16> : (vb) == 8 ? KERNEL<__half, 8> : (vb) == 4 ? KERNEL<__half, 4>     \
+                                                                                       : KERNEL<__half, 2>))
+
+int32_t combine_bind(const mmr_combine_desc* d, Handle** out) {
+  if (!out) return fail(MMR_ERR_INVALID_ARGUMENT, "null output handle pointer");
+  *out = nullptr;
+  if (!d) return fail(MMR_ERR_INVALID_ARGUMENT, "null descriptor");
+  const int dev = d->device_ordinal;
+  Layout l;
+  Ref rows, w, res, o;
+  MMR_TRY(read_layout(d->layout, dev, &l));
+  MMR_TRY(read_tensor(d->rows, "rows", dev, 2, kFloat, &rows));
+  if (present(d->weights)) MMR_TRY(read_tensor(d->weights, "weights", dev, 2, kF32, &w));
+  if (present(d->residual)) MMR_TRY(read_tensor(d->residual, "residual", dev, 2, kFloat, &res));
+  MMR_TRY(read_tensor(d->out, "out", dev, 2, kFloat, &o));
+  MMR_TRY(same_dtype(o, rows.dtype));
+  if (res.on) MMR_TRY(same_dtype(res, rows.dtype));
+  const int64_t width = rows.d[2];
+  MMR_TRY(want_dims(rows, {l.rows, width}));
+  MMR_TRY(want_dims(o, {l.tokens, width}));
+  if (w.on) MMR_TRY(want_dims(w, {l.tokens, l.top_k}));
+  if (res.on) MMR_TRY(want_dims(res, {l.tokens, width}));
+  MMR_TRY(check_aliasing({&o}, {&rows, &w, &res, &l.slots}, &res));
+  int vb = 16;
+  MMR_TRY(row_vector({&rows, &res, &o}, width, &vb));
+  int sms = 0;
+  MMR_TRY(check_device(dev, {&rows, &w, &res, &o, &l.slots, &l.sources, &l.offsets, &l.counts}, &sms));
+  DeviceGuard guard(dev);
+  if (!guard.ok) return fail(MMR_ERR_CUDA, "cudaSetDevice(%d) failed", dev);
+  Owned h;
+  MMR_TRY(new_handle(dev, sms, d->stream, &h));
+  if (l.tokens > 0 && width > 0) {
+    mmr::CombineParams p;
+    p.slots = l.p(l.slots);
+    p.tokens = int(l.tokens);
+    p.top_k = int(l.top_k);
+    p.weights = reinterpret_cast<const float*>(w.on ? w.base : 0);
+    p.w_t = w.s[1];
+    p.w_j = w.s[2];
+    p.rows = row_mat(rows);
+    p.residual = row_mat(res);
+    p.out = row_mat(o);
+    p.row_vecs = int(width * rows.es / vb);
+    const int64_t units = l.tokens * ((p.row_vecs + 127) / 128);
+    const int grid = int(std::min<int64_t>(units, int64_t(1) << 30));
+    auto kernel = MMR_PICK(mmr::mmr_combine_kernel, rows.dtype, vb);
+    add_step(h.get(), "mmr_combine_kernel grid %lld, %lld-byte vectors", [=](cudaStream_t s) {
+      return mmr::launch_kernel(kernel, dim3(grid), dim3(128), 0, s, dim3(1, 1, 1), p);
+    }, grid, vb);
+  }
+  *out = h.release();
+  return MMR_OK;
+}
+
+int32_t combine_grad_bind(const mmr_combine_grad_desc* d, Handle** out) {
+  if (!out) return fail(MMR_ERR_INVALID_ARGUMENT, "null output handle pointer");
+  *out = nullptr;
+  if (!d) return fail(MMR_ERR_INVALID_ARGUMENT, "null descriptor");
+  const int dev = d->device_ordinal;
+  Layout l;
+  Ref dy, rows, w, dr, dw;
+  MMR_TRY(read_layout(d->layout, dev, &l));
+  MMR_TRY(read_tensor(d->d_out, "d_out", dev, 2, kFloat, &dy));
+  if (present(d->weights)) MMR_TRY(read_tensor(d->weights, "weights", dev, 2, kF32, &w));
+  if (present(d->d_rows)) MMR_TRY(read_tensor(d->d_rows, "d_rows", dev, 2, kFloat, &dr));
+  if (present(d->d_weights)) {
+    MMR_TRY(read_tensor(d->d_weights, "d_weights", dev, 2, kF32, &dw));
+    MMR_TRY(read_tensor(d->rows, "rows", dev, 2, kFloat, &rows));
+  }
+  if (!dr.on && !dw.on) return fail(MMR_ERR_INVALID_ARGUMENT, "no gradient is asked for");
+  const int64_t width = dy.d[2];
+  MMR_TRY(want_dims(dy, {l.tokens, width}));
+  for (const Ref* r : {&rows, &dr})
+    if (r->on) {
+      MMR_TRY(same_dtype(*r, dy.dtype));
+      MMR_TRY(want_dims(*r, {l.rows, width}));
+    }
+  for (const Ref* r : {&w, &dw})
+    if (r->on) MMR_TRY(want_dims(*r, {l.tokens, l.top_k}));
+  MMR_TRY(check_aliasing({&dr, &dw}, {&dy, &rows, &w, &l.slots, &l.sources}));
+  int vb = 16;
+  MMR_TRY(row_vector({&dy, &rows, &dr}, width, &vb));
+  int sms = 0;
+  MMR_TRY(check_device(dev, {&dy, &rows, &w, &dr, &dw, &l.slots, &l.sources, &l.offsets, &l.counts}, &sms));
+  DeviceGuard guard(dev);
+  if (!guard.ok) return fail(MMR_ERR_CUDA, "cudaSetDevice(%d) failed", dev);
+  Owned h;
+  MMR_TRY(new_handle(dev, sms, d->stream, &h));
+  mmr::CombineGradParams p;
+  p.slots = l.p(l.slots);
+  p.sources = l.p(l.sources);
+  p.tokens = int(l.tokens);
+  p.top_k = int(l.top_k);
+  p.n_rows = l.rows;
+  p.weights = reinterpret_cast<const float*>(w.on ? w.base : 0);
+  p.w_t = w.s[1];
+  p.w_j = w.s[2];
+  p.d_out = row_mat(dy);
+  p.rows = row_mat(rows);
+  p.d_rows = row_mat(dr);
+  p.d_weights = reinterpret_cast<float*>(dw.on ? dw.base : 0);
+  p.dw_t = dw.s[1];
+  p.dw_j = dw.s[2];
+  p.row_vecs = int(width * dy.es / vb);
+  p.zero_blocks = dr.on && width > 0 ? int(std::min<int64_t>((l.rows + 31) / 32, 4 * sms)) : 0;
+  const int grid = int(l.tokens) + p.zero_blocks;
+  auto kernel = MMR_PICK(mmr::mmr_combine_grad_kernel, dy.dtype, vb);
+  if (grid > 0)
+    add_step(h.get(), "mmr_combine_grad_kernel grid %lld, %lld-byte vectors", [=](cudaStream_t s) {
+      return mmr::launch_kernel(kernel, dim3(grid), dim3(256), 0, s, dim3(1, 1, 1), p);
+    }, grid, vb);
+  *out = h.release();
+  return MMR_OK;
+}
+
+// The experts' weights as a product's B: batch e, mn = columns of the product.
+Operand weights_operand(const Ref& w, bool axis1_is_mn) {
+  Operand o = operand(w, axis1_is_mn);
+  o.batch = w.d[0];
+  o.s_b = w.s[0];
+  return o;
+}
+
+int32_t expert_linear_bind(const mmr_expert_linear_desc* d, Handle** out) {
+  if (!out) return fail(MMR_ERR_INVALID_ARGUMENT, "null output handle pointer");
+  *out = nullptr;
+  if (!d) return fail(MMR_ERR_INVALID_ARGUMENT, "null descriptor");
+  const int dev = d->device_ordinal;
+  Layout l;
+  Ref rows, w, bias, o, pre;
+  MMR_TRY(check_act(d->activation));
+  MMR_TRY(read_layout(d->layout, dev, &l));
+  MMR_TRY(read_tensor(d->rows, "rows", dev, 2, kHalf, &rows));
+  MMR_TRY(read_tensor(d->weights, "weights", dev, 3, kHalf, &w));
+  MMR_TRY(read_tensor(d->out, "out", dev, 2, kHalf, &o));
+  if (present(d->bias)) MMR_TRY(read_tensor(d->bias, "bias", dev, 2, kHalf, &bias));
+  if (present(d->pre)) MMR_TRY(read_tensor(d->pre, "pre", dev, 2, kHalf, &pre));
+  for (const Ref* r : {&w, &o, &bias, &pre})
+    if (r->on) MMR_TRY(same_dtype(*r, rows.dtype));
+  if (d->transpose_rhs) untranspose(&w);
+  const int64_t k = rows.d[2], n = w.d[2];
+  MMR_TRY(want_dims(rows, {l.rows, k}));
+  MMR_TRY(want_dims(w, {l.experts, k, n}));
+  MMR_TRY(want_dims(o, {l.rows, n}));
+  if (pre.on) MMR_TRY(want_dims(pre, {l.rows, n}));
+  if (bias.on) MMR_TRY(want_dims(bias, {l.experts, n}));
+  MMR_TRY(check_aliasing({&o, &pre}, {&rows, &w, &bias, &l.offsets, &l.counts}));
+  int sms = 0;
+  MMR_TRY(check_device(dev, {&rows, &w, &o, &bias, &pre, &l.slots, &l.sources, &l.offsets, &l.counts}, &sms));
+  DeviceGuard guard(dev);
+  if (!guard.ok) return fail(MMR_ERR_CUDA, "cudaSetDevice(%d) failed", dev);
+  Owned h;
+  MMR_TRY(new_handle(dev, sms, d->stream, &h));
+  mmr::EpiParams epi;
+  epi.out = epi_mat(o);
+  epi.pre = epi_mat(pre);
+  epi.bias = reinterpret_cast<const void*>(bias.on ? bias.base : 0);
+  epi.bias_bs = bias.s[1];
+  epi.bias_s = bias.s[2];
+  epi.act = d->activation;
+  const Groups g = l.groups();
+  MMR_TRY(add_product(h.get(), rows.dtype, operand(rows, true), weights_operand(w, false), epi, &g));
+  *out = h.release();
+  return MMR_OK;
+}
+
+int32_t expert_linear_grad_bind(const mmr_expert_linear_grad_desc* d, Handle** out) {
+  if (!out) return fail(MMR_ERR_INVALID_ARGUMENT, "null output handle pointer");
+  *out = nullptr;
+  if (!d) return fail(MMR_ERR_INVALID_ARGUMENT, "null descriptor");
+  const int dev = d->device_ordinal;
+  Layout l;
+  Ref dy, rows, w, pre, dr, dw, db;
+  MMR_TRY(check_act(d->activation));
+  MMR_TRY(read_layout(d->layout, dev, &l));
+  MMR_TRY(read_tensor(d->d_out, "d_out", dev, 2, kHalf, &dy));
+  MMR_TRY(read_tensor(d->rows, "rows", dev, 2, kHalf, &rows));
+  MMR_TRY(read_tensor(d->weights, "weights", dev, 3, kHalf, &w));
+  if (d->activation != MMR_ACT_NONE) MMR_TRY(read_tensor(d->pre, "pre", dev, 2, kHalf, &pre));
+  if (present(d->d_rows)) MMR_TRY(read_tensor(d->d_rows, "d_rows", dev, 2, kHalf, &dr));
+  if (present(d->d_weights)) MMR_TRY(read_tensor(d->d_weights, "d_weights", dev, 3, kHalf, &dw));
+  if (present(d->d_bias)) MMR_TRY(read_tensor(d->d_bias, "d_bias", dev, 2, kHalf, &db));
+  if (!dr.on && !dw.on && !db.on) return fail(MMR_ERR_INVALID_ARGUMENT, "no gradient is asked for");
+  for (const Ref* r : {&rows, &w, &pre, &dr, &dw, &db})
+    if (r->on) MMR_TRY(same_dtype(*r, dy.dtype));
+  if (d->transpose_rhs) {
+    untranspose(&w);
+    untranspose(&dw);
+  }
+  const int64_t k = rows.d[2], n = dy.d[2];
+  MMR_TRY(want_dims(dy, {l.rows, n}));
+  MMR_TRY(want_dims(rows, {l.rows, k}));
+  MMR_TRY(want_dims(w, {l.experts, k, n}));
+  if (pre.on) MMR_TRY(want_dims(pre, {l.rows, n}));
+  if (dr.on) MMR_TRY(want_dims(dr, {l.rows, k}));
+  if (dw.on) MMR_TRY(want_dims(dw, {l.experts, k, n}));
+  if (db.on) MMR_TRY(want_dims(db, {l.experts, n}));
+  if ((dw.on || db.on) && l.align % mmr::AG_ROWS)
+    return fail(MMR_ERR_UNSUPPORTED_LAYOUT, "d_weights and d_bias need a row_align of 64 or 128, not %lld", (long long)l.align);
+  MMR_TRY(check_aliasing({&dr, &dw, &db}, {&dy, &rows, &w, &pre, &l.offsets, &l.counts, &l.sources}));
+  int sms = 0;
+  MMR_TRY(check_device(dev, {&dy, &rows, &w, &pre, &dr, &dw, &db, &l.slots, &l.sources, &l.offsets, &l.counts}, &sms));
+  DeviceGuard guard(dev);
+  if (!guard.ok) return fail(MMR_ERR_CUDA, "cudaSetDevice(%d) failed", dev);
+  Owned h;
+  MMR_TRY(new_handle(dev, sms, d->stream, &h));
+  const Groups g = l.groups();
+  Ref dp;
+  MMR_TRY(add_act_grad(h.get(), d->activation, dy, pre, db, &dp, &g, l.p(l.sources)));
+  if (dr.on) {
+    mmr::EpiParams epi;
+    epi.out = epi_mat(dr);
+    MMR_TRY(add_product(h.get(), dy.dtype, operand(dp, true), weights_operand(w, true), epi, &g));
+  }
+  if (dw.on) {
+    // d_weights[e] = rows_e^T d_pre_e, written along its unit stride
+    Operand a = operand(rows, false), b = operand(dp, false);
+    if (dw.s[2] != 1 && dw.s[1] == 1) {
+      std::swap(a, b);
+      untranspose(&dw);
+    }
+    MMR_TRY(add_segment_product(h.get(), dy.dtype, a, b, epi_mat(dw), g));
+  }
+  *out = h.release();
+  return MMR_OK;
+}
+
+int32_t poll_event(cudaEvent_t ev, uint64_t timeout_ns) {
+  const auto t0 = std::chrono::steady_clock::now();
+  for (;;) {
+    const cudaError_t e = cudaEventQuery(ev);
+    if (e == cudaSuccess) return MMR_OK;
+    if (e != cudaErrorNotReady) return fail(MMR_ERR_CUDA, "cudaEventQuery: %s", cudaGetErrorString(e));
+    const auto el = std::chrono::duration_cast<std::chrono::nanoseconds>(std::chrono::steady_clock::now() - t0).count();
+    if (uint64_t(el) > timeout_ns)
+      return fail(MMR_ERR_TIMEOUT, "work did not complete within %llu ns", (unsigned long long)timeout_ns);
+    std::this_thread::sleep_for(std::chrono::microseconds(50));
+  }
+}
+
+int32_t run_on(Handle* h, cudaStream_t s) {
+  DeviceGuard guard(h->device);
+  if (!guard.ok) return fail(MMR_ERR_CUDA, "cudaSetDevice(%d) failed", h->device);
+  cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
+  MMR_CUDA(cudaStreamIsCapturing(s, &cap));
+  const bool capturing = cap != cudaStreamCaptureStatusNone;
+  // The workspaces are the handle's own: a run on another stream follows the last.
+  if (!capturing && h->ran && s != h->last_stream) MMR_CUDA(cudaStreamWaitEvent(s, h->done, 0));
+  for (const auto& step : h->steps) MMR_TRY(step.launch(s));
+  h->launched = true;
+  if (!capturing) {
+    MMR_CUDA(cudaEventRecord(h->done, s));
+    h->ran = true;
+    h->last_stream = s;
+  }
+  return MMR_OK;
+}
+
+int32_t quiesce(Handle* h, uint64_t timeout_ns) {
+  if (!h->launched) return MMR_OK;
+  DeviceGuard guard(h->device);
+  if (h->ran) MMR_TRY(poll_event(h->done, timeout_ns));
+  for (mmr_gemm_handle* g : h->products) MMR_TRY(mmr_gemm_quiesce(g, timeout_ns));
+  MMR_CUDA(cudaMemcpyAsync(h->h_err, h->d_err, sizeof(int), cudaMemcpyDeviceToHost, h->stream));
+  MMR_CUDA(cudaEventRecord(h->err_ev, h->stream));
+  MMR_TRY(poll_event(h->err_ev, timeout_ns));
+  if (const int code = *h->h_err) {
+    *h->h_err = 0;
+    cudaMemsetAsync(h->d_err, 0, sizeof(int), h->stream);
+    return fail(MMR_ERR_TIMEOUT, "kernel reported device error word %d (a bounded wait expired)", code);
+  }
+  return MMR_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t mmr_expert_rows(int64_t tokens, int64_t top_k, int64_t experts, int64_t row_align, int64_t* rows) {
+  return guarded([&] {
+    if (!rows) return fail(MMR_ERR_INVALID_ARGUMENT, "null output pointer");
+    return expert_rows(tokens, top_k, experts, row_align, rows);
+  });
+}
+
+int32_t mmr_linear_bind(const mmr_linear_desc* d, mmr_op_handle** out) {
+  return guarded([&] { return linear_bind(d, out); });
+}
+int32_t mmr_linear_grad_bind(const mmr_linear_grad_desc* d, mmr_op_handle** out) {
+  return guarded([&] { return linear_grad_bind(d, out); });
+}
+int32_t mmr_dispatch_bind(const mmr_dispatch_desc* d, mmr_op_handle** out) {
+  return guarded([&] { return dispatch_bind(d, out); });
+}
+int32_t mmr_combine_bind(const mmr_combine_desc* d, mmr_op_handle** out) {
+  return guarded([&] { return combine_bind(d, out); });
+}
+int32_t mmr_combine_grad_bind(const mmr_combine_grad_desc* d, mmr_op_handle** out) {
+  return guarded([&] { return combine_grad_bind(d, out); });
+}
+int32_t mmr_expert_linear_bind(const mmr_expert_linear_desc* d, mmr_op_handle** out) {
+  return guarded([&] { return expert_linear_bind(d, out); });
+}
+int32_t mmr_expert_linear_grad_bind(const mmr_expert_linear_grad_desc* d, mmr_op_handle** out) {
+  return guarded([&] { return expert_linear_grad_bind(d, out); });
+}
+
+int32_t mmr_op_run_on(mmr_op_handle* h, void* stream) {
+  return guarded([&] {
+    if (!h) return fail(MMR_ERR_INVALID_ARGUMENT, "null handle");
+    return run_on(h, reinterpret_cast<cudaStream_t>(stream));
+  });
+}
+int32_t mmr_op_run(mmr_op_handle* h) {
+  return guarded([&] {
+    if (!h) return fail(MMR_ERR_INVALID_ARGUMENT, "null handle");
+    return run_on(h, h->stream);
+  });
+}
+int32_t mmr_op_quiesce(mmr_op_handle* h, uint64_t timeout_ns) {
+  return guarded([&] {
+    if (!h) return fail(MMR_ERR_INVALID_ARGUMENT, "null handle");
+    return quiesce(h, timeout_ns);
+  });
+}
+int32_t mmr_op_destroy(mmr_op_handle* h) {
+  return guarded([&] {
+    if (!h) return int32_t(MMR_OK);
+    int32_t rc = MMR_OK;
+    {
+      DeviceGuard guard(h->device);
+      if (h->ran && h->done) rc = poll_event(h->done, 10000000000ull);
+      for (mmr_gemm_handle* g : h->products) {
+        const int32_t r = mmr_gemm_destroy(g);
+        if (rc == MMR_OK) rc = r;
+      }
+      for (void* p : h->workspaces) cudaFree(p);
+      if (h->done) cudaEventDestroy(h->done);
+      if (h->err_ev) cudaEventDestroy(h->err_ev);
+      if (h->d_err) cudaFree(h->d_err);
+      if (h->h_err) cudaFreeHost(h->h_err);
+    }
+    delete h;
+    return rc;
+  });
+}
+const char* mmr_op_plan(const mmr_op_handle* h) { return h ? h->plan.c_str() : ""; }
+
+}  // extern "C"

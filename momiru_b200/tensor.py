@@ -13,8 +13,9 @@ through torch.
 """
 from __future__ import annotations
 
+import enum
 import itertools
-from dataclasses import dataclass, field
+from dataclasses import dataclass, field, replace
 
 import numpy as np
 
@@ -25,6 +26,35 @@ _alloc_ids = itertools.count(1)
 
 class ViewError(ValueError):
     pass
+
+
+class DType(enum.Enum):
+    """Element types of a view: f32 everywhere, the others where an operator takes them."""
+    F32 = (0, 4, "float32")
+    BF16 = (1, 2, "bfloat16")
+    F16 = (2, 2, "float16")
+    I32 = (3, 4, "int32")
+
+    @property
+    def code(self) -> int:
+        """The ABI's MMR_DTYPE_* value."""
+        return self.value[0]
+
+    @property
+    def itemsize(self) -> int:
+        return self.value[1]
+
+    @property
+    def torch(self):
+        import torch
+        return getattr(torch, self.value[2])
+
+    @staticmethod
+    def of_torch(dtype) -> "DType":
+        for d in DType:
+            if str(dtype) == f"torch.{d.value[2]}":
+                return d
+        raise ViewError(f"element type {dtype} is not one of {', '.join(d.name for d in DType)}")
 
 
 @dataclass
@@ -56,21 +86,28 @@ class DeviceView:
     dims: tuple
     strides: tuple          # element strides (>= 0)
     offset: int = 0         # element offset of [0, .., 0]
+    dtype: DType = DType.F32
 
     # ---------------------------------------------------------------- create
     @staticmethod
-    def contiguous(buffer: DeviceBuffer, dims, offset: int = 0) -> "DeviceView":
+    def contiguous(buffer: DeviceBuffer, dims, offset: int = 0, dtype: DType = DType.F32) -> "DeviceView":
         dims = tuple(int(d) for d in dims)
         strides, acc = [], 1
         for d in reversed(dims):
             strides.append(acc)
             acc *= max(d, 1)
-        return DeviceView(buffer, dims, tuple(reversed(strides)), offset)
+        return DeviceView(buffer, dims, tuple(reversed(strides)), offset, dtype)
 
     @staticmethod
-    def empty(dims, device_ordinal: int = 0) -> "DeviceView":
+    def empty(dims, device_ordinal: int = 0, dtype: DType = DType.F32) -> "DeviceView":
         n = int(np.prod(dims)) if len(dims) else 1
-        return DeviceView.contiguous(DeviceBuffer.allocate(4 * n, device_ordinal), dims)
+        return DeviceView.contiguous(DeviceBuffer.allocate(dtype.itemsize * n, device_ordinal), dims, dtype=dtype)
+
+    @staticmethod
+    def from_torch(t) -> "DeviceView":
+        """The CUDA tensor's own elements as a view (no copy); it keeps the tensor alive."""
+        return DeviceView(DeviceBuffer.from_torch(t), tuple(t.shape), tuple(t.stride()), t.storage_offset(),
+                          DType.of_torch(t.dtype))
 
     @staticmethod
     def from_host(arr: np.ndarray, device_ordinal: int = 0) -> "DeviceView":
@@ -89,7 +126,7 @@ class DeviceView:
         return int(np.prod(self.dims)) if self.dims else 1
 
     def is_row_major_contiguous(self) -> bool:
-        return self == DeviceView.contiguous(self.buffer, self.dims, self.offset)
+        return self == DeviceView.contiguous(self.buffer, self.dims, self.offset, self.dtype)
 
     # ------------------------------------------------------------ view ops
     def transpose(self, a: int = -2, b: int = -1) -> "DeviceView":
@@ -98,7 +135,7 @@ class DeviceView:
         d, s = list(self.dims), list(self.strides)
         d[a], d[b] = d[b], d[a]
         s[a], s[b] = s[b], s[a]
-        return DeviceView(self.buffer, tuple(d), tuple(s), self.offset)
+        return replace(self, dims=tuple(d), strides=tuple(s))
 
     def narrow(self, axis: int, start: int, length: int) -> "DeviceView":
         axis %= self.rank
@@ -106,7 +143,7 @@ class DeviceView:
             raise ViewError(f"narrow({axis}, {start}, {length}) outside extent {self.dims[axis]}")
         d = list(self.dims)
         d[axis] = length
-        return DeviceView(self.buffer, tuple(d), self.strides, self.offset + start * self.strides[axis])
+        return replace(self, dims=tuple(d), offset=self.offset + start * self.strides[axis])
 
     def slice(self, specs) -> "DeviceView":
         """specs: one (start, stop, step>0) tuple or None (full axis) per axis."""
@@ -120,29 +157,36 @@ class DeviceView:
             off += start * s[ax]
             d[ax] = (stop - start + step - 1) // step
             s[ax] *= step
-        return DeviceView(self.buffer, tuple(d), tuple(s), off)
+        return replace(self, dims=tuple(d), strides=tuple(s), offset=off)
 
     def as_strided_view(self, dims, strides, offset: int | None = None) -> "DeviceView":
-        return DeviceView(self.buffer, tuple(dims), tuple(strides), self.offset if offset is None else offset)
+        return replace(self, dims=tuple(dims), strides=tuple(strides), offset=self.offset if offset is None else offset)
 
     def unsqueeze(self, axis: int) -> "DeviceView":
         d, s = list(self.dims), list(self.strides)
         d.insert(axis, 1)
         s.insert(axis, 0)
-        return DeviceView(self.buffer, tuple(d), tuple(s), self.offset)
+        return replace(self, dims=tuple(d), strides=tuple(s))
 
     # ----------------------------------------------------------- host copies
     def torch_view(self):
         """A torch view over the same memory (for copies in and out)."""
         import torch
         base = self.buffer.owner
-        if base is None or not isinstance(base, torch.Tensor) or base.dtype != torch.float32:
-            raise ViewError("buffer not allocated through torch as f32")
+        if base is None or not isinstance(base, torch.Tensor):
+            raise ViewError("buffer not allocated through torch")
+        if base.dtype != self.dtype.torch:
+            if self.dtype == DType.F32:
+                raise ViewError("buffer not allocated through torch as f32")
+            # DeviceBuffer.allocate counts f32 words: the same bytes as this type
+            flat = torch.as_strided(base, (base.untyped_storage().nbytes() // base.element_size(),), (1,), 0)
+            base = flat.view(self.dtype.torch)
         # as_strided offsets are absolute within the storage, as ours are.
         return torch.as_strided(base, self.dims, self.strides, self.offset)
 
     def to_host(self) -> np.ndarray:
-        return self.torch_view().cpu().numpy()
+        t = self.torch_view().cpu()
+        return (t.float() if self.dtype == DType.BF16 else t).numpy()
 
     def copy_from_host(self, arr: np.ndarray) -> None:
         import torch
@@ -150,12 +194,18 @@ class DeviceView:
 
     # ------------------------------------------------------------------ ABI
     def to_abi(self) -> _abi.MmrView:
+        """The view as the f32 MatMul node takes it."""
+        if self.dtype != DType.F32:
+            raise ViewError(f"a view of {self.dtype.name} where the MatMul node takes F32")
+        return self._abi_view()
+
+    def _abi_view(self) -> _abi.MmrView:
         if self.rank > _abi.MAX_RANK:
             raise ViewError(f"rank {self.rank} above {_abi.MAX_RANK}")
         v = _abi.MmrView()
         v.address = self.buffer.address
         v.bytes = self.buffer.bytes
-        v.base_offset_bytes = 4 * self.offset
+        v.base_offset_bytes = self.dtype.itemsize * self.offset
         v.rank = self.rank
         v.device_ordinal = self.buffer.device_ordinal
         for i, (d, s) in enumerate(zip(self.dims, self.strides)):
@@ -163,3 +213,8 @@ class DeviceView:
             v.strides[i] = s
         v.allocation_id = self.buffer.allocation_id
         return v
+
+    def to_abi_tensor(self):
+        """The view with its element type (MmrTensor of include/momiru_ops.h)."""
+        from . import _ops_abi
+        return _ops_abi.MmrTensor(self._abi_view(), self.dtype.code, 0)
