@@ -189,29 +189,55 @@ __global__ void __launch_bounds__(ES_THREADS) mmr_dispatch_kernel(const Dispatch
   }
   __syncthreads();  // the run's slots (written above by this CTA) are read back below
 
-  // rows that hold no token: the pads of the segments and what follows the last
-  const int gw = static_cast<int>(blockIdx.x) * ES_WARPS + warp, gn = static_cast<int>(gridDim.x) * ES_WARPS;
+  // Rows that hold no token, every warp-count-th row a warp's, so that the long
+  // run of them after the last segment is spread over all warps; 32 at a time,
+  // finding a row's segment by bisection.
+  const long long warps = static_cast<long long>(gridDim.x) * ES_WARPS;
   Vec zero;
   memset(&zero, 0, sizeof zero);
-  for (int e = 0; e <= E; ++e) {
-    const long long from = e < E ? static_cast<long long>(start[e]) + total[e] : start[E];
-    const long long to = e < E ? start[e + 1] : p.rows;
-    for (long long r = from + (gw + e * 37) % gn; r < to; r += gn) {
-      Vec* dst = reinterpret_cast<Vec*>(static_cast<char*>(p.out.p) + r * p.out.ld);
+  for (long long rb = static_cast<long long>(blockIdx.x) * ES_WARPS + warp; rb < p.rows; rb += 32 * warps) {
+    const long long r = rb + lane * warps;
+    bool none = false;
+    if (r < p.rows) {
+      int lo = 0, hi = E;  // the last segment that starts at or before r
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (start[mid] <= r) lo = mid;
+        else hi = mid - 1;
+      }
+      none = lo == E || r - start[lo] >= total[lo];
+      if (none) p.sources[r] = -1;
+    }
+    for (unsigned left = __ballot_sync(0xffffffffu, none); left; left &= left - 1) {
+      Vec* dst = reinterpret_cast<Vec*>(static_cast<char*>(p.out.p) + (rb + (__ffs(left) - 1) * warps) * p.out.ld);
       for (int c = lane; c < p.row_vecs; c += 32) dst[c] = zero;
-      if (lane == 0) p.sources[r] = -1;
     }
   }
-  // the rows of this run's tokens
+  // The rows of this run's tokens, in pieces of 32 vectors: four pieces' loads in
+  // flight in a warp where there are enough of them.
   const int t0 = static_cast<int>(blockIdx.x) * p.run, t1 = min(t0 + p.run, p.tokens);
-  const int cols = (p.row_vecs + 31) / 32;  // 32-vector pieces of a row
-  for (int u = warp; u < (t1 - t0) * cols; u += ES_WARPS) {
-    const int t = t0 + u / cols, c = (u % cols) * 32 + lane;
-    if (c >= p.row_vecs) continue;
-    const Vec v = reinterpret_cast<const Vec*>(static_cast<const char*>(p.x.p) + t * p.x.ld)[c];
-    for (int j = 0; j < p.top_k; ++j) {
-      const int slot = p.slots[t * p.top_k + j];
-      if (slot >= 0) reinterpret_cast<Vec*>(static_cast<char*>(p.out.p) + slot * p.out.ld)[c] = v;
+  const int pieces = (p.row_vecs + 31) / 32;
+  const bool many = (t1 - t0) * pieces >= 4 * ES_WARPS;
+  const int group = many ? 4 : 1, groups = (pieces + group - 1) / group;
+  for (int u = warp; u < (t1 - t0) * groups; u += ES_WARPS) {
+    const int t = t0 + u / groups, c = (u % groups) * group * 32 + lane;
+    const Vec* src = reinterpret_cast<const Vec*>(static_cast<const char*>(p.x.p) + t * p.x.ld);
+    Vec v[4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+      if (q < group && c + 32 * q < p.row_vecs) v[q] = __ldg(src + c + 32 * q);
+    for (int j0 = 0; j0 < p.top_k; j0 += 4) {
+      int slot[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) slot[j] = j0 + j < p.top_k ? p.slots[t * p.top_k + j0 + j] : -1;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (slot[j] < 0) continue;
+        Vec* dst = reinterpret_cast<Vec*>(static_cast<char*>(p.out.p) + slot[j] * p.out.ld);
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (q < group && c + 32 * q < p.row_vecs) dst[c + 32 * q] = v[q];
+      }
     }
   }
 }
@@ -245,44 +271,55 @@ __device__ __forceinline__ typename VecOf<VB>::type vec_from_f32(const float (&v
 
 // out[t] = sum_j weights[t, j] rows[slots[t, j]] (+ residual[t]): f32 sums in
 // increasing j, one rounding. A thread takes one vector of a token's row, so a
-// warp reads 512 contiguous bytes of every row it adds; the reads of four
+// warp reads 512 contiguous bytes of every row it adds; the reads of kChoices
 // choices are in flight together.
-template <typename T, int VB>
+template <typename T, int VB, int kChoices>
 __global__ void __launch_bounds__(128) mmr_combine_kernel(const CombineParams p) {
   using Vec = typename VecOf<VB>::type;
   constexpr int V = VB / sizeof(T);
   griddep_wait();
   griddep_release();
+  const int lane = static_cast<int>(threadIdx.x) & 31;
   const int pieces = (p.row_vecs + 127) / 128;
   const long long units = static_cast<long long>(p.tokens) * pieces;
   for (long long u = blockIdx.x; u < units; u += gridDim.x) {
     const int t = static_cast<int>(u / pieces), c = static_cast<int>(u % pieces) * 128 + static_cast<int>(threadIdx.x);
-    if (c >= p.row_vecs) continue;
     float acc[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[i] = 0.0f;
-    for (int j0 = 0; j0 < p.top_k; j0 += 4) {
-      Vec w[4];
-      float scale[4];
-      int slot[4];
+    // a lane per choice reads its slot and weight; the rows' addresses then
+    // depend on nothing else
+    for (int jb = 0; jb < p.top_k; jb += 32) {
+      const int many = min(p.top_k - jb, 32);
+      int my_slot = -1;
+      float my_scale = 1.0f;
+      if (lane < many) {
+        my_slot = __ldg(p.slots + static_cast<long long>(t) * p.top_k + jb + lane);
+        if (p.weights && my_slot >= 0) my_scale = __ldg(p.weights + t * p.w_t + (jb + lane) * p.w_j);
+      }
+      for (int j0 = 0; j0 < many; j0 += kChoices) {
+        Vec w[kChoices];
+        float scale[kChoices];
+        int slot[kChoices];
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        slot[q] = j0 + q < p.top_k ? p.slots[static_cast<long long>(t) * p.top_k + j0 + q] : -1;
-        scale[q] = 1.0f;
-        if (slot[q] >= 0) {
-          w[q] = __ldg(reinterpret_cast<const Vec*>(static_cast<const char*>(p.rows.p) + slot[q] * p.rows.ld) + c);
-          if (p.weights) scale[q] = p.weights[t * p.w_t + (j0 + q) * p.w_j];
+        for (int q = 0; q < kChoices; ++q) {
+          slot[q] = __shfl_sync(0xffffffffu, my_slot, (j0 + q) & 31);
+          scale[q] = __shfl_sync(0xffffffffu, my_scale, (j0 + q) & 31);
+          if (j0 + q >= many || c >= p.row_vecs) slot[q] = -1;
+          if (slot[q] >= 0)
+            w[q] = __ldg(reinterpret_cast<const Vec*>(static_cast<const char*>(p.rows.p) + slot[q] * p.rows.ld) + c);
+        }
+#pragma unroll
+        for (int q = 0; q < kChoices; ++q) {
+          if (slot[q] < 0) continue;
+          float v[V];
+          vec_to_f32<T, VB>(w[q], v);
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[i] = fmaf(scale[q], v[i], acc[i]);
         }
       }
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (slot[q] < 0) continue;
-        float v[V];
-        vec_to_f32<T, VB>(w[q], v);
-#pragma unroll
-        for (int i = 0; i < V; ++i) acc[i] = fmaf(scale[q], v[i], acc[i]);
-      }
     }
+    if (c >= p.row_vecs) continue;
     if (p.residual.p) {
       float v[V];
       vec_to_f32<T, VB>(reinterpret_cast<const Vec*>(static_cast<const char*>(p.residual.p) + t * p.residual.ld)[c], v);
@@ -307,29 +344,37 @@ struct CombineGradParams {
   int zero_blocks = 0;  // trailing blocks that zero the rows without a token
 };
 
-// One block per token: d_rows[slot] = w d_out[t] and d_w = <d_out[t],
-// rows[slot]> in one pass, four choices at a time so that d_out's row is read
-// from memory once. The dot products are joined in a fixed order.
-template <typename T, int VB>
+// d_rows[slot] = w d_out[t] and d_w = <d_out[t], rows[slot]> in one pass, four
+// choices at a time. W warps take a token: one where the tokens alone fill the
+// GPU (no block-wide joins), else the block's eight. The dot products are
+// joined in a fixed order.
+template <typename T, int VB, int W>
 __global__ void __launch_bounds__(256) mmr_combine_grad_kernel(const CombineGradParams p) {
   using Vec = typename VecOf<VB>::type;
   constexpr int V = VB / sizeof(T);
+  constexpr int U = VB == 16 ? 1 : 2;  // vectors of a row that a thread has in flight
   __shared__ float part[8][4];
   griddep_wait();
   griddep_release();
   const int tid = static_cast<int>(threadIdx.x), warp = tid >> 5, lane = tid & 31;
-  if (static_cast<int>(blockIdx.x) >= p.tokens) {
+  const int token_blocks = (p.tokens * W + 7) / 8;
+  if (static_cast<int>(blockIdx.x) >= token_blocks) {
     Vec zero;
     memset(&zero, 0, sizeof zero);
-    const long long b = static_cast<int>(blockIdx.x) - p.tokens;
-    for (long long r = b * 8 + warp; r < p.n_rows; r += p.zero_blocks * 8ll) {
-      if (p.sources[r] >= 0) continue;
-      Vec* dst = reinterpret_cast<Vec*>(static_cast<char*>(p.d_rows.p) + r * p.d_rows.ld);
-      for (int c = lane; c < p.row_vecs; c += 32) dst[c] = zero;
+    // rows strided over the warps: those without a token come in runs
+    const long long warps = p.zero_blocks * 8ll;
+    for (long long rb = (static_cast<int>(blockIdx.x) - token_blocks) * 8 + warp; rb < p.n_rows; rb += 32 * warps) {
+      const bool none = rb + lane * warps < p.n_rows && p.sources[rb + lane * warps] < 0;
+      for (unsigned left = __ballot_sync(0xffffffffu, none); left; left &= left - 1) {
+        Vec* dst = reinterpret_cast<Vec*>(static_cast<char*>(p.d_rows.p) + (rb + (__ffs(left) - 1) * warps) * p.d_rows.ld);
+        for (int c = lane; c < p.row_vecs; c += 32) dst[c] = zero;
+      }
     }
     return;
   }
-  const int t = static_cast<int>(blockIdx.x);
+  const int t = W == 8 ? static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x) * 8 + warp;
+  const int me = W == 8 ? tid : lane;
+  if (t >= p.tokens) return;  // whole warps, and only where warps are on their own
   const Vec* d_out = reinterpret_cast<const Vec*>(static_cast<const char*>(p.d_out.p) + t * p.d_out.ld);
   for (int j0 = 0; j0 < p.top_k; j0 += 4) {
     int slot[4];
@@ -340,27 +385,38 @@ __global__ void __launch_bounds__(256) mmr_combine_grad_kernel(const CombineGrad
       scale[q] = slot[q] >= 0 ? (p.weights ? p.weights[t * p.w_t + (j0 + q) * p.w_j] : 1.0f) : 0.0f;
       dot[q] = 0.0f;
     }
-    for (int c = tid; c < p.row_vecs; c += 256) {
-      float d[V];
-      vec_to_f32<T, VB>(__ldg(d_out + c), d);
-      Vec w[4];
+    for (int c0 = me; c0 < p.row_vecs; c0 += 32 * W * U) {
+      Vec dv[U], w[U][4];
 #pragma unroll
-      for (int q = 0; q < 4; ++q)
-        if (slot[q] >= 0 && p.d_weights)
-          w[q] = __ldg(reinterpret_cast<const Vec*>(static_cast<const char*>(p.rows.p) + slot[q] * p.rows.ld) + c);
+      for (int x = 0; x < U; ++x) {
+        const int c = c0 + x * 32 * W;
+        if (c >= p.row_vecs) continue;
+        dv[x] = __ldg(d_out + c);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if (slot[q] < 0) continue;
-        float v[V];
-        if (p.d_weights) {
-          vec_to_f32<T, VB>(w[q], v);
+        for (int q = 0; q < 4; ++q)
+          if (slot[q] >= 0 && p.d_weights)
+            w[x][q] = __ldg(reinterpret_cast<const Vec*>(static_cast<const char*>(p.rows.p) + slot[q] * p.rows.ld) + c);
+      }
 #pragma unroll
-          for (int i = 0; i < V; ++i) dot[q] = fmaf(d[i], v[i], dot[q]);
-        }
-        if (p.d_rows.p) {
+      for (int x = 0; x < U; ++x) {
+        const int c = c0 + x * 32 * W;
+        if (c >= p.row_vecs) continue;
+        float d[V];
+        vec_to_f32<T, VB>(dv[x], d);
 #pragma unroll
-          for (int i = 0; i < V; ++i) v[i] = scale[q] * d[i];
-          reinterpret_cast<Vec*>(static_cast<char*>(p.d_rows.p) + slot[q] * p.d_rows.ld)[c] = vec_from_f32<T, VB>(v);
+        for (int q = 0; q < 4; ++q) {
+          if (slot[q] < 0) continue;
+          float v[V];
+          if (p.d_weights) {
+            vec_to_f32<T, VB>(w[x][q], v);
+#pragma unroll
+            for (int i = 0; i < V; ++i) dot[q] = fmaf(d[i], v[i], dot[q]);
+          }
+          if (p.d_rows.p) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[i] = scale[q] * d[i];
+            reinterpret_cast<Vec*>(static_cast<char*>(p.d_rows.p) + slot[q] * p.d_rows.ld)[c] = vec_from_f32<T, VB>(v);
+          }
         }
       }
     }
@@ -369,16 +425,26 @@ __global__ void __launch_bounds__(256) mmr_combine_grad_kernel(const CombineGrad
     for (int q = 0; q < 4; ++q) {
 #pragma unroll
       for (int d = 16; d; d >>= 1) dot[q] += __shfl_xor_sync(0xffffffffu, dot[q], d);
-      if (lane == 0) part[warp][q] = dot[q];
     }
-    __syncthreads();
-    if (tid < 4 && j0 + tid < p.top_k) {
-      float s = 0.0f;
+    if (W == 1) {
+      float s = dot[0];
 #pragma unroll
-      for (int w = 0; w < 8; ++w) s += part[w][tid];
-      p.d_weights[t * p.dw_t + (j0 + tid) * p.dw_j] = s;
+      for (int q = 1; q < 4; ++q) s = lane == q ? dot[q] : s;
+      if (lane < 4 && j0 + lane < p.top_k) p.d_weights[t * p.dw_t + (j0 + lane) * p.dw_j] = s;
+    } else {
+      if (lane == 0) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) part[warp][q] = dot[q];
+      }
+      __syncthreads();
+      if (tid < 4 && j0 + tid < p.top_k) {
+        float s = 0.0f;
+#pragma unroll
+        for (int w = 0; w < 8; ++w) s += part[w][tid];
+        p.d_weights[t * p.dw_t + (j0 + tid) * p.dw_j] = s;
+      }
+      __syncthreads();
     }
-    __syncthreads();
   }
 }
 

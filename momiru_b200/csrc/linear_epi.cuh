@@ -36,39 +36,52 @@ __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float x) { retu
 template <>
 __device__ __forceinline__ __half from_f32<__half>(float x) { return __float2half_rn(x); }
 
-// Activations for 16-bit results. Each is written so that one exponential and
-// one division carry it: their approximate forms are good to about 2^-21,
-// against the 2^-12 of an f16 rounding.
+// 2^x and 1 / x by the special function unit: about 2 and 1 units in the last
+// place, subnormals flushed.
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float fast_rcp(float x) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Activations for 16-bit results, each of one exponential and one reciprocal
+// (good to about 2^-20, against the 2^-12 of an f16 rounding).
 //   silu       x / (1 + e^-x)
 //   gelu_tanh  x (1 + tanh u) / 2 = x / (1 + e^-2u), u = sqrt(2/pi)(x + 0.044715 x^3):
 //              no 1 + tanh, which cancels for x < 0
 //   gelu_erf   x Phi(x) with erfc by Abramowitz & Stegun 7.1.26 (absolute
 //              error below 1.5e-7)
-// As in the f32 epilogue, -inf gives -0 (not inf / inf) and NaN stays NaN.
-__device__ __forceinline__ float lact_silu(float x) {
-  return x == -__int_as_float(0x7f800000) ? -0.0f : __fdividef(x, 1.0f + __expf(-x));
+// As in the f32 epilogue, -inf gives -0 (not inf times 0) and NaN stays NaN.
+constexpr float kLog2e = 1.4426950408890f;
+__device__ __forceinline__ float no_inf(float x, float y) { return x == -__int_as_float(0x7f800000) ? -0.0f : y; }
+__device__ __forceinline__ float fast_sigmoid(float x) { return fast_rcp(1.0f + fast_exp2(-kLog2e * x)); }
+// sigmoid(2u): the coefficients 2 sqrt(2/pi) (0.044715, 1)
+__device__ __forceinline__ float gelu_gate(float x) {
+  return fast_rcp(1.0f + fast_exp2(x * fmaf(-0.0713548162726f * kLog2e, x * x, -1.5957691216057f * kLog2e)));
 }
-__device__ __forceinline__ float lact_gelu_tanh(float x) {
-  const float u2 = x * fmaf(0.0713548162726f, x * x, 1.5957691216057f);  // 2 sqrt(2/pi) (0.044715, 1)
-  return x == -__int_as_float(0x7f800000) ? -0.0f : __fdividef(x, 1.0f + __expf(-u2));
-}
+__device__ __forceinline__ float lact_silu(float x) { return no_inf(x, x * fast_sigmoid(x)); }
+__device__ __forceinline__ float lact_gelu_tanh(float x) { return no_inf(x, x * gelu_gate(x)); }
 // Phi(x) and e^(-x^2/2).
 __device__ __forceinline__ float normal_cdf(float x, float* gauss) {
-  const float z = fabsf(x) * 0.70710678118655f;
-  const float t = __fdividef(1.0f, fmaf(0.3275911f, z, 1.0f));
-  const float g = __expf(-z * z);
-  float p = fmaf(1.061405429f, t, -1.453152027f);
-  p = fmaf(p, t, 1.421413741f);
-  p = fmaf(p, t, -0.284496736f);
-  p = fmaf(p, t, 0.254829592f);
-  const float half_erfc = 0.5f * p * t * g;
+  const float t = fast_rcp(fmaf(0.3275911f * 0.70710678118655f, fabsf(x), 1.0f));
+  const float g = fast_exp2(-0.5f * kLog2e * x * x);
+  float p = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
+  p = fmaf(p, t, 0.5f * 1.421413741f);
+  p = fmaf(p, t, 0.5f * -0.284496736f);
+  p = fmaf(p, t, 0.5f * 0.254829592f);
+  const float half_erfc = p * t * g;
   *gauss = g;
   return x < 0.0f ? half_erfc : 1.0f - half_erfc;
 }
 __device__ __forceinline__ float lact_gelu_erf(float x) {
   float g;
   const float c = normal_cdf(x, &g);
-  return x == -__int_as_float(0x7f800000) ? -0.0f : x * c;
+  return no_inf(x, x * c);
 }
 
 template <int N>
@@ -115,20 +128,38 @@ struct EpiParams {
   int n = 0;
 };
 
-union Pack8 {
-  uint4 u;
-  unsigned short h[8];
-};
+// Eight f32 to eight 16-bit values, two a conversion, and back.
+__device__ __forceinline__ uint32_t pack2(__nv_bfloat16, float a, float b) {
+  const __nv_bfloat162 p = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+__device__ __forceinline__ uint32_t pack2(__half, float a, float b) {
+  const __half2 p = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+__device__ __forceinline__ float2 unpack2(__nv_bfloat16, uint32_t w) {
+  return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
+}
+__device__ __forceinline__ float2 unpack2(__half, uint32_t w) {
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+  return make_uint4(pack2(T(), v[0], v[1]), pack2(T(), v[2], v[3]), pack2(T(), v[4], v[5]), pack2(T(), v[6], v[7]));
+}
+template <typename T>
+__device__ __forceinline__ void add8(float (&v)[8], const uint4& w) {
+  const float2 a = unpack2(T(), w.x), b = unpack2(T(), w.y), c = unpack2(T(), w.z), d = unpack2(T(), w.w);
+  v[0] += a.x; v[1] += a.y; v[2] += b.x; v[3] += b.y;
+  v[4] += c.x; v[5] += c.y; v[6] += d.x; v[7] += d.y;
+}
 
 template <typename T>
 __device__ __forceinline__ void store8(const EpiMat& m, long long b, long long row, int col, int n,
                                        const float (&v)[8]) {
   T* q = static_cast<T*>(m.p) + b * m.bs + row * m.ld + col * m.cs;
   if (m.vec && col + 8 <= n) {
-    Pack8 w;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) *reinterpret_cast<T*>(&w.h[i]) = from_f32<T>(v[i]);
-    *reinterpret_cast<uint4*>(q) = w.u;
+    *reinterpret_cast<uint4*>(q) = pack8<T>(v);
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)
@@ -140,10 +171,16 @@ __device__ __forceinline__ void store8(const EpiMat& m, long long b, long long r
 template <typename T>
 __device__ __forceinline__ void load_bias8(const EpiParams& e, int batch, int col, float (&b)[8]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    b[i] = e.bias && col + i < e.n
-               ? to_f32<T>(static_cast<const T*>(e.bias)[batch * e.bias_bs + (col + i) * e.bias_s])
-               : 0.0f;
+  for (int i = 0; i < 8; ++i) b[i] = 0.0f;
+  if (!e.bias) return;
+  const T* q = static_cast<const T*>(e.bias) + batch * e.bias_bs + col * e.bias_s;
+  if (e.bias_s == 1 && col + 8 <= e.n && (reinterpret_cast<uintptr_t>(q) & 15) == 0) {
+    add8<T>(b, __ldg(reinterpret_cast<const uint4*>(q)));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (col + i < e.n) b[i] = to_f32<T>(q[i * e.bias_s]);
+  }
 }
 
 // The epilogue of (row, col .. col + 7): v holds the accumulators. The residual
@@ -159,10 +196,7 @@ __device__ __forceinline__ void epi_store8(const EpiParams& e, long long batch, 
   if (e.residual.p) {
     const T* q = static_cast<const T*>(e.residual.p) + row * e.residual.ld + col * e.residual.cs;
     if (e.residual.vec && col + 8 <= e.n) {
-      Pack8 w;
-      w.u = *reinterpret_cast<const uint4*>(q);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] += to_f32<T>(*reinterpret_cast<T*>(&w.h[i]));
+      add8<T>(v, *reinterpret_cast<const uint4*>(q));
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i)
@@ -170,6 +204,20 @@ __device__ __forceinline__ void epi_store8(const EpiParams& e, long long batch, 
     }
   }
   store8<T>(e.out, batch, row, col, e.n, v);
+}
+
+// The same for one element: what views without 16-byte vectors take, with
+// neighbouring lanes on neighbouring columns. `residual` is read by the caller.
+template <typename T>
+__device__ __forceinline__ void epi_store1(const EpiParams& e, long long batch, long long row, int col, float v,
+                                           float bias, float residual) {
+  float x[1] = {v + bias};
+  if (e.pre.p) static_cast<T*>(e.pre.p)[batch * e.pre.bs + row * e.pre.ld + col * e.pre.cs] = from_f32<T>(x[0]);
+  lact_apply(e.act, x);
+  static_cast<T*>(e.out.p)[batch * e.out.bs + row * e.out.ld + col * e.out.cs] = from_f32<T>(x[0] + residual);
+}
+__device__ __forceinline__ bool epi_vec(const EpiParams& e) {
+  return e.out.vec && (!e.pre.p || e.pre.vec) && (!e.residual.p || e.residual.vec);
 }
 
 template <typename T>

@@ -2,10 +2,10 @@
 //   out = epilogue(A B), A m x k, B k x n, both bf16 or both f16, f32 sums.
 //
 // A pair computes a 256 x 256 tile with one 256 x 256 x 16 instruction per
-// k-step: each CTA stages its 128 rows of A and its 128 columns of B in
+// k-step: each CTA stages its 128 rows of A and its half of B's columns in
 // 64-wide k-blocks (128-byte swizzled rows, 32 KiB a stage), and keeps two
-// 128 x 256 f32 accumulators in tensor memory, so that the epilogue of one
-// tile runs under the MMAs of the next.
+// 128 x 256 f32 accumulators in tensor memory, so that the epilogue of one tile
+// runs under the MMAs of the next.
 //
 // RAG 0: one product; tiles walk in groups of LP_GROUP row tiles so that the
 //        pairs running together share panels in L2.
@@ -19,8 +19,17 @@
 //        rows are zero, so a k-block never meets another expert's rows; an
 //        expert without tokens gets zeros.
 //
-// Bound: the tensor pipe. 128 cycles per instruction; the issuing thread only
-// adds fixed offsets to precomputed descriptors.
+// Work split: whole rounds of tiles, one a pair. Where the tiles of the last
+// round fill at most half the pairs they are cut into two 256 x 128 halves
+// (64 columns a CTA), one a pair, so the round ends after half the MMAs and a
+// product of few tiles reaches twice the SMs: 512 x 4096 x 4096 23 us against
+// 29 uncut, 4096^3 (3.46 rounds) 96 us before. Dividing those tiles along K
+// instead, with parts parked in memory and joined by the last to finish, cost
+// more than it saved (104 and 36 us): a part's 256 KB go out and come back.
+//
+// Bound: the tensor pipe. A tile of 4096 k takes 33.3 thousand cycles against
+// 32.8 of MMAs; the clock under that load is the power cap's (1.63 GHz where it
+// was traced), 1.53 PFLOP/s at 4096 x 11008 x 4096.
 //
 // Warps: 0-7 epilogue (TMEM lane quarter x column half), 8 TMA producer, 9 MMA
 // issuer (even CTA), 10-11 idle.
@@ -33,13 +42,13 @@
 namespace mmr {
 
 constexpr int LP_THREADS = 384;
-constexpr int LP_BN = 256;
 constexpr int LP_BK = 64;
 constexpr int LP_A_BYTES = 128 * LP_BK * 2;
-constexpr int LP_STAGE_BYTES = 2 * LP_A_BYTES;
 constexpr int LP_CSTAGE_BYTES = 4096;  // per epilogue warp: 32 rows x 32 f32
 constexpr int LP_GROUP = 8;
 constexpr int LP_MAX_EXPERTS = 1024;
+
+constexpr int LP_STAGE_BYTES = 2 * LP_A_BYTES;
 
 constexpr int lp_stages(int rag) { return rag ? 5 : 6; }
 // ragged: every expert's first tile and first row (and the ends), and its token count
@@ -62,11 +71,12 @@ struct PairParams {
   unsigned long long timeout_ns = 0;
 };
 
-// One tile of work, found from its index.
+// One piece of work, found from its index.
 struct LpTile {
   int row0, row_end, zero_end;  // output rows: [row0, row_end) computed, up to zero_end zeroed
   int a_row;                    // row coordinate of A's tile
   int col0;
+  bool half;                    // 128 columns instead of 256
   int batch;                    // expert
   int kb, k_row;                // k-blocks, and the row where the contraction starts (RAG 2)
 };
@@ -75,33 +85,43 @@ template <int RAG>
 struct LpWalk {
   const PairParams& p;
   const int *first, *off, *cnt;  // shared-memory tables (RAG 1, 2)
-  int t, step, total, e;
-  __device__ __forceinline__ LpWalk(const PairParams& p_, const int* table, int t0, int step_)
-      : p(p_), first(table), off(table + LP_MAX_EXPERTS + 1), cnt(table + 2 * LP_MAX_EXPERTS + 2), t(t0), step(step_),
-        total(RAG == 1 ? table[p_.experts] : p_.tiles_total), e(0) {}
+  int t, step, e;
+  int whole, end;                // pieces before `whole` are tiles, up to `end` half tiles
+  __device__ __forceinline__ LpWalk(const PairParams& p_, const int* table, int pair, int npairs)
+      : p(p_), first(table), off(table + LP_MAX_EXPERTS + 1), cnt(table + 2 * LP_MAX_EXPERTS + 2), t(pair), step(npairs), e(0) {
+    const int total = RAG == 1 ? table[p_.experts] : p_.tiles_total;
+    const int rem = total % npairs;
+    whole = 2 * rem <= npairs ? total - rem : total;
+    end = total + (total - whole);
+  }
   __device__ __forceinline__ bool next(LpTile& w) {
-    if (t >= total) return false;
+    if (t >= end) return false;
+    int tile = t, right = 0;
+    w.half = t >= whole;
+    if (w.half) {
+      tile = whole + ((t - whole) >> 1);
+      right = (t - whole) & 1;
+    }
+    t += step;
     int mt, nt;
+    w.batch = 0;
+    w.kb = p.k_blocks;
+    w.k_row = 0;
     if (RAG == 1) {
-      while (first[e + 1] <= t) ++e;
-      const int local = t - first[e], tm = (cnt[e] + 255) >> 8;
+      while (first[e + 1] <= tile) ++e;
+      const int local = tile - first[e], tm = (cnt[e] + 255) >> 8;
       mt = local % tm;
       nt = local / tm;
       w.row0 = w.a_row = off[e] + mt * 256;
       w.row_end = off[e] + cnt[e];
       w.zero_end = off[e + 1];
       w.batch = e;
-      w.kb = p.k_blocks;
-      w.k_row = 0;
     } else {
-      int r = t;
-      w.batch = 0;
-      w.kb = p.k_blocks;
-      w.k_row = 0;
+      int r = tile;
       if (RAG == 2) {
         const int per = p.tiles_m * p.tiles_n;
-        w.batch = t / per;
-        r = t - w.batch * per;
+        w.batch = tile / per;
+        r = tile - w.batch * per;
         w.kb = (cnt[w.batch] + LP_BK - 1) / LP_BK;
         w.k_row = off[w.batch];
       }
@@ -113,8 +133,7 @@ struct LpWalk {
       w.row_end = p.m;
       w.zero_end = 0;
     }
-    w.col0 = nt * LP_BN;
-    t += step;
+    w.col0 = nt * 256 + right * 128;
     return true;
   }
 };
@@ -205,52 +224,138 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
     uint32_t acc_phase = 0;
     LpWalk<RAG> walk(p, table, pair, npairs);
     LpTile w;
+    const bool vec = epi_vec(p.epi);
+    // The residual of one 32 x 32 box, in the layout it is added in: vector `it`
+    // of lane l is row 8 it + l / 4, columns 8 (l % 4) of the box.
+    auto load_residual = [&](const LpTile& w, int row0, int col0, uint4 (&res)[4]) {
+      const int row = row0 + (lane >> 2), col = col0 + (lane & 3) * 8;
+      const T* q = static_cast<const T*>(p.epi.residual.p) + row * p.epi.residual.ld + col;
+#pragma unroll
+      for (int it = 0; it < 4; ++it)
+        if (row + 8 * it < w.row_end && col + 8 <= p.n)
+          res[it] = *reinterpret_cast<const uint4*>(q + 8 * it * p.epi.residual.ld);
+    };
+    // Stores one staged 32 x 32 box (row r: 16-byte chunk q at q ^ (r & 7)). All
+    // 32 of a lane's values go through each step together: with two warps a
+    // scheduler, their independence is what hides the latencies.
+    auto store_box = [&](const LpTile& w, int row0, int col0, const uint4 (&res)[4]) {
+      const long long batch = RAG == 2 ? w.batch : 0;
+      if (vec) {
+        const int c2 = (lane & 3) * 2, col = col0 + (lane & 3) * 8, r0 = lane >> 2;
+        if (col >= p.n) return;
+        float bias[8];
+        load_bias8<T>(p.epi, w.batch, col, bias);
+        if (col + 8 <= p.n && row0 + 32 <= w.row_end) {
+          float v[32];
+#pragma unroll
+          for (int it = 0; it < 4; ++it) {
+            const uint8_t* src = buf + (it * 8 + r0) * 128;  // row & 7 == r0
+            *reinterpret_cast<float4*>(v + 8 * it) = *reinterpret_cast<const float4*>(src + ((c2 ^ r0) << 4));
+            *reinterpret_cast<float4*>(v + 8 * it + 4) = *reinterpret_cast<const float4*>(src + (((c2 + 1) ^ r0) << 4));
+          }
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] += bias[i & 7];
+          auto put = [&](const EpiMat& m) {
+            T* q = static_cast<T*>(m.p) + batch * m.bs + (row0 + r0) * m.ld + col;
+#pragma unroll
+            for (int it = 0; it < 4; ++it)
+              *reinterpret_cast<uint4*>(q + 8 * it * m.ld) = pack8<T>(*reinterpret_cast<const float(*)[8]>(v + 8 * it));
+          };
+          if (p.epi.pre.p) put(p.epi.pre);
+          lact_apply(p.epi.act, v);
+          if (p.epi.residual.p) {
+#pragma unroll
+            for (int it = 0; it < 4; ++it) add8<T>(*reinterpret_cast<float(*)[8]>(v + 8 * it), res[it]);
+          }
+          put(p.epi.out);
+          return;
+        }
+#pragma unroll 1
+        for (int it = 0; it < 4; ++it) {
+          const int rr = it * 8 + r0, row = row0 + rr;
+          const float4 x = *reinterpret_cast<const float4*>(buf + rr * 128 + ((c2 ^ r0) << 4));
+          const float4 y = *reinterpret_cast<const float4*>(buf + rr * 128 + (((c2 + 1) ^ r0) << 4));
+          float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+          if (row < w.row_end) epi_store8<T>(p.epi, batch, row, col, v, bias);
+          else if (RAG == 1 && row < w.zero_end) epi_zero8<T>(p.epi, row, col);
+        }
+      } else {
+        // a lane a column, so that any pitch is stored in whole segments
+        const int col = col0 + lane;
+        if (col >= p.n) return;
+        const float bias =
+            p.epi.bias ? to_f32<T>(static_cast<const T*>(p.epi.bias)[w.batch * p.epi.bias_bs + col * p.epi.bias_s]) : 0.0f;
+        const T* res = p.epi.residual.p ? static_cast<const T*>(p.epi.residual.p) + col * p.epi.residual.cs : nullptr;
+        const int rows = min(max(w.row_end, w.zero_end) - row0, 32);
+        for (int r0 = 0; r0 < rows; r0 += 8) {
+          float add[8];
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            add[q] = res && row0 + r0 + q < w.row_end ? to_f32<T>(res[(row0 + r0 + q) * p.epi.residual.ld]) : 0.0f;
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            const int rr = r0 + q, row = row0 + rr;
+            const float v = *reinterpret_cast<const float*>(buf + rr * 128 + ((((lane >> 2) ^ (rr & 7)) << 4) | ((lane & 3) << 2)));
+            if (row < w.row_end) {
+              epi_store1<T>(p.epi, batch, row, col, v, bias, add[q]);
+            } else if (RAG == 1 && row < w.zero_end) {
+              if (p.epi.pre.p) static_cast<T*>(p.epi.pre.p)[row * p.epi.pre.ld + col * p.epi.pre.cs] = from_f32<T>(0.0f);
+              static_cast<T*>(p.epi.out.p)[row * p.epi.out.ld + col * p.epi.out.cs] = from_f32<T>(0.0f);
+            }
+          }
+        }
+      }
+    };
     while (walk.next(w)) {
-      if (w.kb > 0) {
+      const bool sums = w.kb > 0;
+      const int row0 = w.row0 + static_cast<int>(rank) * 128 + quarter * 32;
+      const int boxes = w.half ? 2 : 4;  // of 32 columns, in this warp's half of the tile
+      const int cbase = w.col0 + half * boxes * 32;
+      const bool adds = vec && p.epi.residual.p && cbase < p.n && row0 < w.row_end;
+      uint4 res[2][4];
+      if (adds) {
+        // under the MMAs: the tile's residual to L2, its first box to registers
+        if (row0 + lane < w.row_end) {
+          const T* q = static_cast<const T*>(p.epi.residual.p) + (row0 + lane) * p.epi.residual.ld + cbase;
+          for (int c = 0; c < boxes * 32 && cbase + c < p.n; c += 64) prefetch_l2(q + c);
+        }
+        load_residual(w, row0, cbase, res[0]);
+      }
+      if (sums) {
         if (!mbar_wait_cluster(&acc_full[acc], acc_phase, ctl, kDevTimeoutAcc)) break;
         tc_fence_after();
       }
-      const int row0 = w.row0 + static_cast<int>(rank) * 128 + quarter * 32;
-      const uint32_t tb = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + acc * LP_BN + half * 128;
+      const uint32_t tb = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + acc * 256 + half * boxes * 32;
 #pragma unroll 1
-      for (int j = 0; j < 4; ++j) {
-        const int col0 = w.col0 + half * 128 + j * 32;
-        uint32_t r[32];
-        if (w.kb > 0) {
-          tmem_ld_32x32b_x32(tb + j * 32, r);
-          tmem_ld_wait();
-          if (j == 3) {
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive_cluster(acc_empty_leader + 8u * acc);
+      for (int j2 = 0; j2 < boxes; j2 += 2) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const int j = j2 + b, col0 = cbase + j * 32;
+          if (adds && j + 1 < boxes) load_residual(w, row0, col0 + 32, res[b ^ 1]);
+          uint32_t r[32];
+          if (sums) {
+            tmem_ld_32x32b_x32(tb + j * 32, r);
+            tmem_ld_wait();
+            if (j == boxes - 1) {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_cluster(acc_empty_leader + 8u * acc);
+            }
+          } else {
+#pragma unroll
+            for (int i = 0; i < 32; ++i) r[i] = 0u;
           }
-        } else {
+          if (col0 >= p.n || row0 >= max(w.row_end, w.zero_end)) continue;
+          __syncwarp();  // the box before has been read
 #pragma unroll
-          for (int i = 0; i < 32; ++i) r[i] = 0u;
+          for (int q = 0; q < 8; ++q)
+            *reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) << 4)) =
+                make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
+          __syncwarp();
+          store_box(w, row0, col0, res[b]);
         }
-        if (col0 >= p.n || row0 >= max(w.row_end, w.zero_end)) continue;
-        // row `lane`: 16-byte chunk q at q ^ (lane & 7)
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-          *reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) << 4)) =
-              make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
-        __syncwarp();
-        const int c2 = (lane & 3) * 2, col = col0 + (lane & 3) * 8;
-        float bias[8];
-        load_bias8<T>(p.epi, w.batch, col, bias);
-#pragma unroll
-        for (int it = 0; it < 4; ++it) {
-          const int rr = it * 8 + (lane >> 2), row = row0 + rr;
-          const float4 x = *reinterpret_cast<const float4*>(buf + rr * 128 + ((c2 ^ (rr & 7)) << 4));
-          const float4 y = *reinterpret_cast<const float4*>(buf + rr * 128 + (((c2 + 1) ^ (rr & 7)) << 4));
-          float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
-          if (col >= p.n) continue;
-          if (row < w.row_end) epi_store8<T>(p.epi, RAG == 2 ? w.batch : 0, row, col, v, bias);
-          else if (RAG == 1 && row < w.zero_end) epi_zero8<T>(p.epi, row, col);
-        }
-        __syncwarp();
       }
-      if (w.kb > 0 && ++acc == 2) { acc = 0; acc_phase ^= 1u; }
+      if (sums && ++acc == 2) { acc = 0; acc_phase ^= 1u; }
     }
     if (RAG == 1) {
       const int g = static_cast<int>(blockIdx.x) * 8 + warp, gn = static_cast<int>(gridDim.x) * 8;
@@ -270,25 +375,27 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
       LpWalk<RAG> walk(p, table, pair, npairs);
       LpTile w;
       while (ok && walk.next(w)) {
-        const int m0 = w.a_row + static_cast<int>(rank) * 128, n0 = w.col0 + static_cast<int>(rank) * 128;
+        const int m0 = w.a_row + static_cast<int>(rank) * 128, n0 = w.col0 + static_cast<int>(rank) * (w.half ? 64 : 128);
         for (int kb = 0; kb < w.kb; ++kb) {
           if (!mbar_wait_cluster(&empty[stage], phase ^ 1u, ctl, kDevTimeoutEmpty)) { ok = false; break; }
           uint8_t* sa = ops + stage * LP_STAGE_BYTES;
           uint8_t* sb = sa + LP_A_BYTES;
           const uint32_t bar = full_leader + 8u * stage;
           const int k0 = w.k_row + kb * LP_BK, bb = RAG == 1 ? w.batch : 0;
-          if (rank == 0) mbar_arrive_expect_tx(&full[stage], 2 * LP_STAGE_BYTES);
+          if (rank == 0) mbar_arrive_expect_tx(&full[stage], w.half ? 3 * LP_A_BYTES : 4 * LP_A_BYTES);
           if (A_MN) {
             tma_load_3d_pair(sa, &tmA, bar, m0, k0, 0);
             tma_load_3d_pair(sa + LP_A_BYTES / 2, &tmA, bar, m0 + 64, k0, 0);
           } else {
             tma_load_3d_pair(sa, &tmA, bar, k0, m0, 0);
           }
+          // 64 columns a box: one for a half tile, two for a whole one
           if (B_MN) {
             tma_load_3d_pair(sb, &tmB, bar, n0, k0, bb);
-            tma_load_3d_pair(sb + LP_A_BYTES / 2, &tmB, bar, n0 + 64, k0, bb);
+            if (!w.half) tma_load_3d_pair(sb + LP_A_BYTES / 2, &tmB, bar, n0 + 64, k0, bb);
           } else {
             tma_load_3d_pair(sb, &tmB, bar, k0, n0, bb);
+            if (!w.half) tma_load_3d_pair(sb + LP_A_BYTES / 2, &tmB, bar, k0, n0 + 64, bb);
           }
           last[stage] = static_cast<int>(phase);
           if (++stage == S) { stage = 0; phase ^= 1u; }
@@ -306,8 +413,14 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
     }
   } else if (warp == 9) {
     // ------------------------------------------------------ MMA issuer (pair)
-    if (lane == 0 && rank == 0) {
-      constexpr uint32_t idesc = idesc_f16(256, LP_BN, std::is_same<T, __nv_bfloat16>::value, A_MN, B_MN);
+    // The whole warp walks the loop and one elected lane issues, so that the
+    // descriptors stay in uniform registers: with a single lane in the branch
+    // an MMA took ~65 cycles to issue and a k-block, its two commits
+    // included, ~620, against 512 cycles of MMAs (a clock64 trace).
+    if (rank == 0) {
+      constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
+      constexpr uint32_t idesc_whole = idesc_f16(256, 256, kBf16, A_MN, B_MN);
+      constexpr uint32_t idesc_half = idesc_f16(256, 128, kBf16, A_MN, B_MN);
       // K-major: 128-byte rows, 8-row groups 1024 bytes apart, 32 bytes a
       // k-step. MN-major: 64-element atoms 8 KiB apart (the 64 K rows of a
       // box), 8-row K groups 1024 bytes apart, two groups a k-step.
@@ -315,7 +428,7 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
       constexpr uint32_t a_step = A_MN ? 2048u : 32u, b_step = B_MN ? 2048u : 32u;
       const uint64_t a_desc0 = smem_desc(smem_u32(ops), a_lbo, 1024u, 2u);
       const uint64_t b_desc0 = smem_desc(smem_u32(ops) + LP_A_BYTES, b_lbo, 1024u, 2u);
-      const uint32_t empty_peer = mapa_shared(smem_u32(empty), 1), acc_full_peer = mapa_shared(smem_u32(acc_full), 1);
+      const bool leader = elect_one();
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
       bool ok = true, issued = false;
@@ -323,33 +436,41 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
       LpTile w;
       while (ok && walk.next(w)) {
         if (w.kb == 0) continue;
-        if (!mbar_wait_cluster(&acc_empty[acc], acc_phase ^ 1u, ctl, kDevTimeoutAcc)) break;
+        if (!__all_sync(0xffffffffu, mbar_wait_cluster(&acc_empty[acc], acc_phase ^ 1u, ctl, kDevTimeoutAcc))) break;
         tc_fence_after();
-        const uint32_t d = tmem + static_cast<uint32_t>(acc * LP_BN);
-        uint32_t accumulate = 0;
+        const uint32_t d = tmem + static_cast<uint32_t>(acc * 256);
+        const uint32_t idesc = w.half ? idesc_half : idesc_whole;
+        bool ready = mbar_test_wait(smem_u32(&full[stage]), phase);
         for (int kb = 0; kb < w.kb; ++kb) {
-          if (!mbar_wait_cluster(&full[stage], phase, ctl, kDevTimeoutFull)) { ok = false; break; }
+          if (!__all_sync(0xffffffffu, ready))
+            ok = __all_sync(0xffffffffu, mbar_wait_cluster(&full[stage], phase, ctl, kDevTimeoutFull));
+          if (!ok) break;
           tc_fence_after();
-          const uint64_t so = static_cast<uint64_t>(stage) * (LP_STAGE_BYTES >> 4);
-#pragma unroll
-          for (int kk = 0; kk < LP_BK / 16; ++kk) {
-            umma_f16_2sm(d, a_desc0 + so + ((a_step * kk) >> 4), b_desc0 + so + ((b_step * kk) >> 4), idesc, accumulate);
-            accumulate = 1u;
-          }
-          issued = true;
-          umma_commit_2sm(smem_u32(&empty[stage]));
-          umma_commit_2sm(empty_peer + 8u * stage);
+          const int now = stage;
           if (++stage == S) { stage = 0; phase ^= 1u; }
+          // asked before this block's MMAs, so that the answer's latency is theirs
+          ready = mbar_test_wait(smem_u32(&full[stage]), phase);
+          const uint64_t so = static_cast<uint64_t>(now) * (LP_STAGE_BYTES >> 4);
+          if (leader) {
+#pragma unroll
+            for (int kk = 0; kk < LP_BK / 16; ++kk)
+              umma_f16_2sm(d, a_desc0 + so + ((a_step * kk) >> 4), b_desc0 + so + ((b_step * kk) >> 4), idesc,
+                           kk > 0 || kb > 0 ? 1u : 0u);
+            umma_commit_2sm_both(&empty[now]);
+          }
+          __syncwarp();
+          issued = true;
         }
         if (!ok) break;
-        umma_commit_2sm(smem_u32(&acc_full[acc]));
-        umma_commit_2sm(acc_full_peer + 8u * acc);
+        if (leader) umma_commit_2sm_both(&acc_full[acc]);
+        __syncwarp();
         if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
       }
       if (issued) {
         // The pair's MMAs are done before either CTA's memory goes: this wait
         // holds the even CTA, whose cluster barrier holds the odd one.
-        umma_commit_2sm(smem_u32(drain));
+        if (leader) umma_commit_2sm(smem_u32(drain));
+        __syncwarp();
         const uint64_t t0 = globaltimer_ns();
         while (!mbar_try_wait_cluster(smem_u32(drain), 0u))
           if (globaltimer_ns() - t0 > p.timeout_ns) { atomicCAS(p.err, 0, kDevTimeoutDrain); break; }

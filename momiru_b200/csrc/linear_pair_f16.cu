@@ -3,10 +3,10 @@
 
 namespace mmr {
 
-cudaError_t pair_launch_f16(bool a_mn, bool b_mn, int rag, int grid, cudaStream_t s, const CUtensorMap& tm_a,
-                             const CUtensorMap& tm_b, const PairParams& p) {
-  return pair_launch_t<__half>(a_mn, b_mn, rag, grid, s, tm_a, tm_b, p);
+cudaError_t pair_launch_f16(const PairShape& sh, cudaStream_t s, const CUtensorMap& tm_a, const CUtensorMap& tm_b,
+                             const PairParams& p) {
+  return pair_launch_t<__half>(sh, s, tm_a, tm_b, p);
 }
-cudaError_t pair_prepare_f16(bool a_mn, bool b_mn, int rag) { return pair_prepare_t<__half>(a_mn, b_mn, rag); }
+cudaError_t pair_prepare_f16(const PairShape& sh) { return pair_prepare_t<__half>(sh); }
 
 }  // namespace mmr

@@ -9,30 +9,32 @@ namespace mmr {
 using PairKernel = void (*)(const CUtensorMap, const CUtensorMap, const PairParams);
 
 template <typename T>
-PairKernel pair_kernel(bool a_mn, bool b_mn, int rag) {
+PairKernel pair_kernel(const PairShape& sh) {
+  const bool a_mn = sh.a_mn, b_mn = sh.b_mn;
+  const int rag = sh.rag;
   if (rag == 0) {
     if (a_mn) return b_mn ? mmr_linear_pair_kernel<T, true, true, 0> : mmr_linear_pair_kernel<T, true, false, 0>;
     return b_mn ? mmr_linear_pair_kernel<T, false, true, 0> : mmr_linear_pair_kernel<T, false, false, 0>;
   }
-  if (rag == 1 && !a_mn) return b_mn ? mmr_linear_pair_kernel<T, false, true, 1> : mmr_linear_pair_kernel<T, false, false, 1>;
+  if (rag == 1 && !a_mn)
+    return b_mn ? mmr_linear_pair_kernel<T, false, true, 1> : mmr_linear_pair_kernel<T, false, false, 1>;
   if (rag == 2 && a_mn && b_mn) return mmr_linear_pair_kernel<T, true, true, 2>;
   return nullptr;
 }
-
 template <typename T>
-cudaError_t pair_launch_t(bool a_mn, bool b_mn, int rag, int grid, cudaStream_t s, const CUtensorMap& tm_a,
-                          const CUtensorMap& tm_b, const PairParams& p) {
-  const PairKernel k = pair_kernel<T>(a_mn, b_mn, rag);
+cudaError_t pair_launch_t(const PairShape& sh, cudaStream_t s, const CUtensorMap& tm_a, const CUtensorMap& tm_b,
+                          const PairParams& p) {
+  const PairKernel k = pair_kernel<T>(sh);
   if (!k) return cudaErrorInvalidValue;
-  return launch_kernel(k, dim3(grid), dim3(LP_THREADS), lp_smem_bytes(rag), s, dim3(2, 1, 1), tm_a, tm_b, p);
+  return launch_kernel(k, dim3(sh.grid), dim3(LP_THREADS), lp_smem_bytes(sh.rag), s, dim3(2, 1, 1), tm_a, tm_b, p);
 }
 
 template <typename T>
-cudaError_t pair_prepare_t(bool a_mn, bool b_mn, int rag) {
-  const PairKernel k = pair_kernel<T>(a_mn, b_mn, rag);
+cudaError_t pair_prepare_t(const PairShape& sh) {
+  const PairKernel k = pair_kernel<T>(sh);
   if (!k) return cudaErrorInvalidValue;
   return cudaFuncSetAttribute(reinterpret_cast<const void*>(k), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                              lp_smem_bytes(rag));
+                              lp_smem_bytes(sh.rag));
 }
 
 }  // namespace mmr

@@ -6,10 +6,9 @@
 // add their partial sums over distributed shared memory, in rank order, so the
 // result does not depend on timing.
 //
-// Bound: the weights' bytes. A strip's 64 x 128 block of w is 16 KiB whatever
-// mt is, so nothing of the tensor core's 128 rows is wasted on absent tokens,
-// and the split over K is what puts every SM on the stream when N / 128 strips
-// are fewer than the SMs.
+// Bound: the weights' bytes. Nothing of the tensor core is wasted on absent
+// tokens, and the split over K is what puts every SM on the stream when the
+// strips are fewer than the SMs (strip_shape in ops.cu).
 //
 // Ragged rows (expert products): a unit is (expert, mt rows of its segment,
 // strip); each CTA finds its expert from the counts. The rows of a segment's
@@ -50,7 +49,7 @@ struct StripParams {
   unsigned long long timeout_ns = 0;
 };
 
-inline int strip_smem_bytes(int mt, int stages) { return stages * (LS_W_BYTES + mt * 128) + 256 + 1024; }
+constexpr int strip_smem_bytes(int mt, int stages) { return stages * (LS_W_BYTES + mt * 128) + 256 + 1024; }
 
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   float4 v;
@@ -58,6 +57,12 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
                : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
                : "r"(addr)
                : "memory");
+  return v;
+}
+
+__device__ __forceinline__ float ld_cluster_f1(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
 }
 
@@ -88,7 +93,7 @@ __device__ __forceinline__ bool find_expert_unit(const int* counts, int experts,
 }
 
 template <typename T, bool W_MN>
-__global__ void __launch_bounds__(LS_THREADS)
+__global__ void __launch_bounds__(LS_THREADS, 3)
     mmr_linear_strip_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                             const StripParams p) {
   extern __shared__ uint8_t smem_raw[];
@@ -122,6 +127,20 @@ __global__ void __launch_bounds__(LS_THREADS)
   if (warp == 5) {
     tmem_alloc(tmem_slot, p.tmem_cols);
     tmem_relinquish();
+  }
+  // The first k-blocks of plain weights start towards L2 while the previous
+  // kernel drains (an expert's are known only after it).
+  if (warp == 4 && lane == 0 && !p.experts) {
+    const int b0 = static_cast<int>(static_cast<long long>(p.k_blocks) * rank / p.split);
+    const int b1 = static_cast<int>(static_cast<long long>(p.k_blocks) * (rank + 1) / p.split);
+    for (int kb = b0; kb < min(b1, b0 + p.stages); ++kb) {
+      if (W_MN) {
+        tma_prefetch_l2_3d(&tmW, strip * LS_COLS, kb * LS_BK, 0);
+        tma_prefetch_l2_3d(&tmW, strip * LS_COLS + 64, kb * LS_BK, 0);
+      } else {
+        tma_prefetch_l2_3d(&tmW, kb * LS_BK, strip * LS_COLS, 0);
+      }
+    }
   }
   griddep_wait();
   if (p.experts && warp == 0) {
@@ -219,7 +238,20 @@ __global__ void __launch_bounds__(LS_THREADS)
   // one n, so each store of a warp is 32 neighbouring floats. The operand
   // stages are free once the MMAs are done.
   float* red = reinterpret_cast<float*>(ops);
+  const bool vec = epi_vec(p.epi);
   if (warp < 4 && valid > 0) {
+    if (p.epi.residual.p) {  // on its way to L2 until the sums are there
+      const T* res = static_cast<const T*>(p.epi.residual.p) + row0 * p.epi.residual.ld;
+      if (vec) {
+        const int c = rank * LS_THREADS + static_cast<int>(threadIdx.x), m = c / (LS_COLS / 8);
+        const int col = strip * LS_COLS + (c % (LS_COLS / 8)) * 8;
+        if (m < valid && col < p.n) prefetch_l2(res + m * p.epi.residual.ld + col);
+      } else if ((lane & 15) == 0) {
+        const int col = strip * LS_COLS + static_cast<int>(threadIdx.x);
+        for (int m = rank; col < p.n && m < valid; m += p.split)
+          prefetch_l2(res + m * p.epi.residual.ld + col * p.epi.residual.cs);
+      }
+    }
     if (work) {
       mbar_wait(acc_full, 0u, ctl, kDevTimeoutAcc);
       tc_fence_after();
@@ -242,31 +274,71 @@ __global__ void __launch_bounds__(LS_THREADS)
   if (p.split > 1) cluster_sync_all();
 
   const int g0 = rank * LS_THREADS + static_cast<int>(threadIdx.x), gstep = p.split * LS_THREADS;
-  for (int c = g0; c < valid * (LS_COLS / 8); c += gstep) {
-    const int m = c / (LS_COLS / 8), lc = (c % (LS_COLS / 8)) * 8;
-    const int col = strip * LS_COLS + lc;
-    if (col >= p.n) continue;
-    float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-    const uint32_t at = smem_u32(red + m * LS_COLS + lc);
-    for (int r = 0; r < p.split; ++r) {
-      const uint32_t a = p.split > 1 ? mapa_shared(at, static_cast<uint32_t>(r)) : at;
-      const float4 x = ld_cluster_f4(a), y = ld_cluster_f4(a + 16);
-      v[0] += x.x; v[1] += x.y; v[2] += x.z; v[3] += x.w;
-      v[4] += y.x; v[5] += y.y; v[6] += y.z; v[7] += y.w;
+  constexpr int per_row = LS_COLS / 8;  // 8-column pieces of a strip's row
+  if (vec) {
+    for (int c = g0; c < valid * per_row; c += gstep) {
+      const int m = c / per_row, lc = (c - m * per_row) * 8;
+      const int col = strip * LS_COLS + lc;
+      if (col >= p.n) continue;
+      float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+      const uint32_t at = smem_u32(red + m * LS_COLS + lc);
+      // four slices' parts are on their way before the first is added
+      for (int r0 = 0; r0 < p.split; r0 += 4) {
+        float4 part[4][2];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (r0 + r >= p.split) break;
+          const uint32_t a = p.split > 1 ? mapa_shared(at, static_cast<uint32_t>(r0 + r)) : at;
+          part[r][0] = ld_cluster_f4(a);
+          part[r][1] = ld_cluster_f4(a + 16);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (r0 + r >= p.split) break;
+          v[0] += part[r][0].x; v[1] += part[r][0].y; v[2] += part[r][0].z; v[3] += part[r][0].w;
+          v[4] += part[r][1].x; v[5] += part[r][1].y; v[6] += part[r][1].z; v[7] += part[r][1].w;
+        }
+      }
+      float bias[8];
+      load_bias8<T>(p.epi, expert, col, bias);
+      epi_store8<T>(p.epi, 0, row0 + m, col, v, bias);
     }
-    float bias[8];
-    load_bias8<T>(p.epi, expert, col, bias);
-    epi_store8<T>(p.epi, 0, row0 + m, col, v, bias);
+  } else {
+    // one element a lane, four rows' residuals in flight; a strip's 128 columns
+    // are a fixed one per thread of four warps
+    constexpr int kAt = 4;
+    const int lc = static_cast<int>(threadIdx.x) & (LS_COLS - 1), col = strip * LS_COLS + lc;
+    const float bias = warp < 4 && p.epi.bias && col < p.n
+                           ? to_f32<T>(static_cast<const T*>(p.epi.bias)[expert * p.epi.bias_bs + col * p.epi.bias_s])
+                           : 0.0f;
+    for (int m0 = rank; warp < 4 && col < p.n && m0 < valid; m0 += kAt * p.split) {
+      float v[kAt], res[kAt];
+#pragma unroll
+      for (int q = 0; q < kAt; ++q) {
+        const int m = m0 + q * p.split;
+        v[q] = res[q] = 0.0f;
+        if (m >= valid) continue;
+        if (p.epi.residual.p)
+          res[q] = to_f32<T>(static_cast<const T*>(p.epi.residual.p)[(row0 + m) * p.epi.residual.ld + col * p.epi.residual.cs]);
+        const uint32_t at = smem_u32(red + m * LS_COLS + lc);
+        for (int r = 0; r < p.split; ++r)
+          v[q] += ld_cluster_f1(p.split > 1 ? mapa_shared(at, static_cast<uint32_t>(r)) : at);
+      }
+#pragma unroll
+      for (int q = 0; q < kAt; ++q) {
+        const int m = m0 + q * p.split;
+        if (m < valid) epi_store1<T>(p.epi, 0, row0 + m, col, v[q], bias, res[q]);
+      }
+    }
   }
   if (p.experts) {
     // pad rows of the segment, then this unit's share of the rows after the last segment
-    const int c0 = strip * LS_COLS;
     for (int pass = 0; pass < 2; ++pass) {
       const long long from = pass ? p.offsets[p.experts] + static_cast<long long>(mu) : row0 + valid;
       const long long to = pass ? p.rows : zero_end, step = pass ? p.m_units : 1;
-      for (long long c = g0; from + (c / 16) * step < to; c += gstep) {
-        const int col = c0 + static_cast<int>(c % 16) * 8;
-        if (col < p.n) epi_zero8<T>(p.epi, from + (c / 16) * step, col);
+      for (long long c = g0; from + (c / per_row) * step < to; c += gstep) {
+        const int col = strip * LS_COLS + static_cast<int>(c % per_row) * 8;
+        if (col < p.n) epi_zero8<T>(p.epi, from + (c / per_row) * step, col);
       }
     }
   }

@@ -77,10 +77,13 @@ int32_t guarded(F&& f) {
 }
 
 struct DeviceGuard {
-  int prev = -1;
+  int prev = -1;  // to be restored; -1 where the device was current already
   bool ok = false;
   explicit DeviceGuard(int dev) {
-    if (cudaGetDevice(&prev) == cudaSuccess && cudaSetDevice(dev) == cudaSuccess) ok = true;
+    int now = -1;
+    if (cudaGetDevice(&now) != cudaSuccess) return;
+    ok = now == dev || cudaSetDevice(dev) == cudaSuccess;
+    if (ok && now != dev) prev = now;
   }
   ~DeviceGuard() {
     if (prev >= 0) cudaSetDevice(prev);
@@ -370,10 +373,10 @@ bool tma_pitch(uint64_t base, int64_t pitch, int64_t extent, int64_t s_b, int64_
   return batch <= 1 || (s_b > 0 && s_b % 8 == 0 && s_b < (int64_t(1) << 38));
 }
 
-// Makes `o` readable by TMA: as it lies where it can, else packed by a step of
-// each run into rows of a 16-byte pitch. `major`: 0 any, 1 K-major only, 2
-// MN-major only.
-int32_t admit(Handle* h, Operand* o, int major, const char* name) {
+// Makes `o` readable by TMA: as it lies where it can, else packed by each run
+// into rows of a 16-byte pitch (entered in `packs`). `major`: 0 any, 1 K-major
+// only, 2 MN-major only.
+int32_t admit(Handle* h, Operand* o, int major, const char* name, mmr::PackList* packs) {
   if (o->mn == 0 || o->k == 0 || o->batch == 0) return MMR_OK;  // nothing is loaded
   if (major != 2 && (o->s_k == 1 || o->k == 1) && tma_pitch(o->base, o->s_mn, o->mn, o->s_b, o->batch, o->k)) {
     o->mn_major = false;
@@ -395,18 +398,29 @@ int32_t admit(Handle* h, Operand* o, int major, const char* name) {
   q.pitch = (q.cols + 7) / 8 * 8;
   if (o->batch > 65535) return fail(MMR_ERR_UNSUPPORTED_LAYOUT, "%s: more than 65535 matrices to pack", name);
   const int64_t per = int64_t(q.rows) * q.pitch;
+  q.batch = int(o->batch);
   MMR_TRY(workspace(h, size_t(per) * o->batch * 2, &q.dst));
-  const int64_t tiles = int64_t((q.rows + 31) / 32) * ((q.pitch + 31) / 32);
-  const dim3 grid(unsigned(std::min<int64_t>(tiles, 8 * h->sms)), 1, unsigned(o->batch));
-  add_step(h, "mmr_pack_kernel grid %lld x %lld", [q, grid](cudaStream_t s) {
-    return mmr::launch_kernel(mmr::mmr_pack_kernel, grid, dim3(256), 0, s, dim3(1, 1, 1), q);
-  }, grid.x, grid.z);
+  packs->p[packs->n++] = q;
   o->base = reinterpret_cast<uint64_t>(q.dst);
   o->mn_major = mn_major;
   (mn_major ? o->s_k : o->s_mn) = q.pitch;
   (mn_major ? o->s_mn : o->s_k) = 1;
   o->s_b = per;
   return MMR_OK;
+}
+
+// One launch for all operands of a product that have to be packed.
+void add_packs(Handle* h, const mmr::PackList& packs) {
+  if (packs.n == 0) return;
+  int64_t tiles = 1, batch = 1;
+  for (int i = 0; i < packs.n; ++i) {
+    tiles = std::max(tiles, int64_t((packs.p[i].rows + 31) / 32) * ((packs.p[i].pitch + 31) / 32));
+    batch = std::max<int64_t>(batch, packs.p[i].batch);
+  }
+  const dim3 grid(unsigned(std::min<int64_t>(tiles, 8 * h->sms)), unsigned(packs.n), unsigned(batch));
+  add_step(h, "mmr_pack_kernel grid %lld x %lld x %lld", [packs, grid](cudaStream_t s) {
+    return mmr::launch_kernel(mmr::mmr_pack_kernel, grid, dim3(256), 0, s, dim3(1, 1, 1), packs);
+  }, grid.x, grid.y, grid.z);
 }
 
 // Never read by TMA: a valid descriptor for a product without any k-blocks.
@@ -440,11 +454,52 @@ struct Groups {  // ragged rows or contraction
 };
 
 // Up to this many rows the weights' stream bounds the product and the strip
-// kernel takes it; above, the CTA pairs.
-constexpr int64_t kStripRows = 256;
+// kernel takes it; above, the CTA pairs. N = K = 4096: 16.4 us against 21.3 at
+// 64 rows, 24.1 against 21.6 at 128.
+constexpr int64_t kStripRows = 64;
 constexpr int64_t kStripRowsPerExpert = 96;
 
+// How the strip kernel divides `ctas` strips of k_blocks: K slices of a strip
+// and stages of a CTA. The time follows the SM with the most work, CTAs being
+// dealt evenly, ceil(CTAs / SMs) to an SM; in units of a k-block's time (0.28
+// us) a CTA costs its k-blocks, a tenth for every row of its share of the
+// epilogue, and 4 for the join where there are slices; one CTA an SM costs 8
+// more, as nothing hides its start and end. 64 rows through 28 experts of
+// 2048 x 1024 took 18.4 / 22.8 / 33.5 us in 1 / 2 / 4 slices, one row through
+// 4096 x 11008 22.8 / 19.3 in 4 / 8. Narrower strips, which could
+// be dealt more evenly, only lost (27.9 us at 56 columns): an MMA costs its
+// ~100 cycles however few rows of it are used.
+struct StripShape {
+  int split = 1, stages = 3;
+};
+StripShape strip_shape(int sms, int64_t ctas, int k_blocks, int mt) {
+  StripShape best;
+  double best_cost = 0;
+  for (int split = 1; split <= mmr::LS_MAX_SPLIT; split *= 2) {
+    if (k_blocks < split) break;
+    const double per_cta = double((k_blocks + split - 1) / split) + 0.1 * mt / split + (split > 1 ? 4.0 : 0.0);
+    const int64_t deep = (ctas * split + sms - 1) / sms;
+    const double cost = double(deep) * per_cta + (deep == 1 ? 8.0 : 0.0);
+    if (best_cost == 0 || cost < best_cost) {
+      best_cost = cost;
+      best.split = split;
+    }
+  }
+  // Four CTAs an SM where that leaves three stages each, else two, else one.
+  for (int share : {4, 2, 1}) {
+    const int budget = 232448 / share - (share > 1 ? 2048 : 0);
+    best.stages = mmr::LS_MAX_STAGES;
+    while (best.stages > 1 && mmr::strip_smem_bytes(mt, best.stages) > budget) --best.stages;
+    if (best.stages >= 3) break;
+  }
+  return best;
+}
+
 int round16(int64_t v) { return int((v + 15) / 16 * 16); }
+
+int32_t check_tiles(int64_t tiles) {
+  return tiles > (int64_t(1) << 30) ? fail(MMR_ERR_INVALID_SHAPE, "more than 2^30 output tiles") : int32_t(MMR_OK);
+}
 
 // out[m, n] = epilogue(A[m, k] B[k, n]) in 16-bit operands; a.mn = m, b.mn = n.
 // With `g`, the experts' products over ragged rows (b batched).
@@ -456,8 +511,10 @@ int32_t add_product(Handle* h, int dtype, Operand a, Operand b, mmr::EpiParams e
   const int k_blocks = int((k + 63) / 64);
   const int64_t per_expert = g ? (g->assignments + g->experts - 1) / g->experts : 0;
   const bool strip = g ? per_expert <= kStripRowsPerExpert : m <= kStripRows;
-  MMR_TRY(admit(h, &a, strip || g ? 1 : 0, "lhs"));
-  MMR_TRY(admit(h, &b, 0, "rhs"));
+  mmr::PackList packs;
+  MMR_TRY(admit(h, &a, strip || g ? 1 : 0, "lhs", &packs));
+  MMR_TRY(admit(h, &b, 0, "rhs", &packs));
+  add_packs(h, packs);
   if (k == 0) {
     no_operand(h, &a);
     no_operand(h, &b);
@@ -481,10 +538,10 @@ int32_t add_product(Handle* h, int dtype, Operand a, Operand b, mmr::EpiParams e
       p.counts = g->counts;
       p.rows = g->rows;
     }
-    // Two CTAs of about 100 KB of stages share an SM.
-    const int64_t units = int64_t(p.strips) * (g ? std::min<int64_t>(g->experts, g->assignments) : p.m_units);
-    while (p.split < mmr::LS_MAX_SPLIT && units * p.split < 2 * h->sms && k_blocks >= 8 * p.split) p.split *= 2;
-    p.stages = p.mt > 128 ? 4 : std::min(mmr::LS_MAX_STAGES, 102400 / (mmr::LS_W_BYTES + p.mt * 128));
+    const int64_t units = g ? std::min<int64_t>(g->experts, g->assignments) : p.m_units;
+    const StripShape shape = strip_shape(h->sms, units * p.strips, k_blocks, p.mt);
+    p.split = shape.split;
+    p.stages = shape.stages;
     p.tmem_cols = 32;
     while (p.tmem_cols < uint32_t(p.mt)) p.tmem_cols *= 2;
     p.epi = epi;
@@ -503,10 +560,15 @@ int32_t add_product(Handle* h, int dtype, Operand a, Operand b, mmr::EpiParams e
     return MMR_OK;
   }
   mmr::PairParams p;
+  mmr::PairShape sh;
+  sh.bf16 = bf16;
+  sh.rag = g ? 1 : 0;
+  sh.a_mn = a.mn_major;
+  sh.b_mn = b.mn_major;
   p.m = int(m);
   p.n = int(n);
   p.tiles_m = int((m + 255) / 256);
-  p.tiles_n = int((n + mmr::LP_BN - 1) / mmr::LP_BN);
+  p.tiles_n = int((n + 255) / 256);
   p.k_blocks = k_blocks;
   int64_t tiles = int64_t(p.tiles_m) * p.tiles_n;
   if (g) {
@@ -514,23 +576,20 @@ int32_t add_product(Handle* h, int dtype, Operand a, Operand b, mmr::EpiParams e
     p.offsets = g->offsets;
     p.counts = g->counts;
     p.rows = g->rows;
-    tiles = (std::min<int64_t>(g->experts, g->assignments) + g->assignments / 256) * p.tiles_n;
+    tiles = (std::min<int64_t>(g->experts, g->assignments) + g->assignments / 256) * p.tiles_n;  // at most
   }
-  if (tiles > (int64_t(1) << 31) - 1024) return fail(MMR_ERR_INVALID_SHAPE, "more than 2^31 output tiles");
+  MMR_TRY(check_tiles(tiles));
   p.tiles_total = int(tiles);
   p.epi = epi;
   p.err = h->d_err;
   p.timeout_ns = kWaitNs;
   MMR_TRY(encode16(&ta, a, dtype, 128, "lhs"));
-  MMR_TRY(encode16(&tb, b, dtype, 128, "rhs"));
-  const int rag = g ? 1 : 0;
-  const bool a_mn = a.mn_major, b_mn = b.mn_major;
-  const int grid = 2 * int(std::min<int64_t>(h->sms / 2, std::max<int64_t>(tiles, 1)));
-  MMR_CUDA(bf16 ? mmr::pair_prepare_bf16(a_mn, b_mn, rag) : mmr::pair_prepare_f16(a_mn, b_mn, rag));
+  MMR_TRY(encode16(&tb, b, dtype, 64, "rhs"));
+  sh.grid = 2 * int(std::min<int64_t>(h->sms / 2, std::max<int64_t>(2 * tiles, 1)));
+  MMR_CUDA(mmr::pair_prepare(sh));
   add_step(h, "mmr_linear_pair_kernel grid %lld, tiles %lld, k-blocks %lld", [=](cudaStream_t s) {
-    return bf16 ? mmr::pair_launch_bf16(a_mn, b_mn, rag, grid, s, ta, tb, p)
-                : mmr::pair_launch_f16(a_mn, b_mn, rag, grid, s, ta, tb, p);
-  }, grid, tiles, k_blocks);
+    return mmr::pair_launch(sh, s, ta, tb, p);
+  }, sh.grid, tiles, k_blocks);
   return MMR_OK;
 }
 
@@ -541,16 +600,22 @@ int32_t add_segment_product(Handle* h, int dtype, Operand a, Operand b, const Ep
   p.m = int(a.mn);
   p.n = int(b.mn);
   if (p.m == 0 || p.n == 0 || g.experts == 0) return MMR_OK;
-  MMR_TRY(admit(h, &a, 2, "rows"));
-  MMR_TRY(admit(h, &b, 2, "d_out"));
+  mmr::PackList packs;
+  MMR_TRY(admit(h, &a, 2, "rows", &packs));
+  MMR_TRY(admit(h, &b, 2, "d_out", &packs));
+  add_packs(h, packs);
   if (g.rows == 0) {
     no_operand(h, &a);
     no_operand(h, &b);
   }
+  mmr::PairShape sh;
+  sh.bf16 = bf16;
+  sh.rag = 2;
+  sh.a_mn = sh.b_mn = true;
   p.tiles_m = (p.m + 255) / 256;
-  p.tiles_n = (p.n + mmr::LP_BN - 1) / mmr::LP_BN;
+  p.tiles_n = (p.n + 255) / 256;
   const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n * g.experts;
-  if (tiles > (int64_t(1) << 31) - 1024) return fail(MMR_ERR_INVALID_SHAPE, "more than 2^31 output tiles");
+  MMR_TRY(check_tiles(tiles));
   p.tiles_total = int(tiles);
   p.experts = g.experts;
   p.offsets = g.offsets;
@@ -562,14 +627,26 @@ int32_t add_segment_product(Handle* h, int dtype, Operand a, Operand b, const Ep
   p.timeout_ns = kWaitNs;
   CUtensorMap ta, tb;
   MMR_TRY(encode16(&ta, a, dtype, 128, "rows"));
-  MMR_TRY(encode16(&tb, b, dtype, 128, "d_out"));
-  const int grid = 2 * int(std::min<int64_t>(h->sms / 2, tiles));
-  MMR_CUDA(bf16 ? mmr::pair_prepare_bf16(true, true, 2) : mmr::pair_prepare_f16(true, true, 2));
+  MMR_TRY(encode16(&tb, b, dtype, 64, "d_out"));
+  sh.grid = 2 * int(std::min<int64_t>(h->sms / 2, 2 * tiles));
+  MMR_CUDA(mmr::pair_prepare(sh));
   add_step(h, "mmr_linear_pair_kernel (segments) grid %lld, tiles %lld", [=](cudaStream_t s) {
-    return bf16 ? mmr::pair_launch_bf16(true, true, 2, grid, s, ta, tb, p)
-                : mmr::pair_launch_f16(true, true, 2, grid, s, ta, tb, p);
-  }, grid, tiles);
+    return mmr::pair_launch(sh, s, ta, tb, p);
+  }, sh.grid, tiles);
   return MMR_OK;
+}
+
+// Calls f with the activation as a compile-time constant.
+template <typename F>
+auto pick_act(int act, F&& f) {
+  switch (act) {
+    case MMR_ACT_RELU: return f(std::integral_constant<int, MMR_ACT_RELU>());
+    case MMR_ACT_RELU6: return f(std::integral_constant<int, MMR_ACT_RELU6>());
+    case MMR_ACT_GELU_ERF: return f(std::integral_constant<int, MMR_ACT_GELU_ERF>());
+    case MMR_ACT_GELU_TANH: return f(std::integral_constant<int, MMR_ACT_GELU_TANH>());
+    case MMR_ACT_SILU: return f(std::integral_constant<int, MMR_ACT_SILU>());
+    default: return f(std::integral_constant<int, MMR_ACT_NONE>());
+  }
 }
 
 // d_pre (and d_bias) from d_out and pre. Fills `d_pre` with the view that the
@@ -603,12 +680,21 @@ int32_t add_act_grad(Handle* h, int act, const Ref& d_out, const Ref& pre, const
     p.partial = static_cast<float*>(w);
   }
   const int dt = d_out.dtype;
+  const bool vec = n % 8 == 0 && p.d_out.vec && (!through || p.pre.vec);
   const dim3 grid(unsigned((n + mmr::AG_COLS - 1) / mmr::AG_COLS), unsigned(std::min<int64_t>(std::max<int64_t>(chunks, 1), 65535)));
   if (rows > 0)
     add_step(h, "mmr_act_grad_kernel grid %lld x %lld", [=](cudaStream_t s) {
-      auto k = dt == MMR_DTYPE_F32    ? mmr::mmr_act_grad_kernel<float>
-               : dt == MMR_DTYPE_BF16 ? mmr::mmr_act_grad_kernel<__nv_bfloat16>
-                                      : mmr::mmr_act_grad_kernel<__half>;
+      using K = void (*)(const mmr::ActGradParams);
+      const K k = pick_act(p.act, [&](auto a) -> K {
+        constexpr int kAct = decltype(a)::value;
+        if (vec)
+          return dt == MMR_DTYPE_F32    ? mmr::mmr_act_grad_kernel<float, kAct, true>
+                 : dt == MMR_DTYPE_BF16 ? mmr::mmr_act_grad_kernel<__nv_bfloat16, kAct, true>
+                                        : mmr::mmr_act_grad_kernel<__half, kAct, true>;
+        return dt == MMR_DTYPE_F32    ? mmr::mmr_act_grad_kernel<float, kAct, false>
+               : dt == MMR_DTYPE_BF16 ? mmr::mmr_act_grad_kernel<__nv_bfloat16, kAct, false>
+                                      : mmr::mmr_act_grad_kernel<__half, kAct, false>;
+      });
       return mmr::launch_kernel(k, grid, dim3(256), 0, s, dim3(1, 1, 1), p);
     }, grid.x, grid.y);
   if (d_bias.on) {
@@ -787,32 +873,29 @@ int32_t linear_bind(const mmr_linear_desc* d, Handle** out) {
       mmr_view to;
       if (pre.on) {
         to = f32_view(pre, dev);
-        q.pre = reinterpret_cast<const float*>(pre.base);
-        q.pre_ld = pre.s[1];
-        q.pre_cs = pre.s[2];
+        q.pre = epi_mat(pre);
       } else {
         void* w = nullptr;
         const int64_t ld = (n + 3) / 4 * 4;
         MMR_TRY(workspace(h.get(), size_t(m) * ld * 4, &w));
         to = f32_view(w, m, n, ld, dev);
-        q.pre = static_cast<const float*>(w);
-        q.pre_ld = ld;
-        q.pre_cs = 1;
+        q.pre.p = w;
+        q.pre.ld = ld;
+        q.pre.cs = 1;
+        q.pre.vec = 1;
       }
       MMR_TRY(add_f32_product(h.get(), d->math_mode, f32_view(lhs, dev), f32_view(rhs, dev), to, &bias,
                               f32_epilogue(MMR_ACT_NONE, bias.on)));
-      q.residual = reinterpret_cast<const float*>(res.on ? res.base : 0);
-      q.res_ld = res.s[1];
-      q.res_cs = res.s[2];
-      q.out = reinterpret_cast<float*>(o.base);
-      q.out_ld = o.s[1];
-      q.out_cs = o.s[2];
+      q.residual = epi_mat(res);
+      q.out = epi_mat(o);
       q.m = int(m);
       q.n = int(n);
-      q.act = d->activation;
-      const int grid = int(std::min<int64_t>((m * n + 255) / 256, 16 * sms));
+      const int act = d->activation;
+      const int grid = int(std::min<int64_t>((m * ((n + 127) / 128) + 7) / 8, 16 * sms));
       add_step(h.get(), "mmr_act_res_kernel grid %lld", [=](cudaStream_t s) {
-        return mmr::launch_kernel(mmr::mmr_act_res_kernel, dim3(grid), dim3(256), 0, s, dim3(1, 1, 1), q);
+        using K = void (*)(const mmr::ActResParams);
+        const K k = pick_act(act, [](auto a) -> K { return mmr::mmr_act_res_kernel<decltype(a)::value>; });
+        return mmr::launch_kernel(k, dim3(grid), dim3(256), 0, s, dim3(1, 1, 1), q);
       }, grid);
     }
   } else {
@@ -1033,14 +1116,14 @@ int32_t dispatch_bind(const mmr_dispatch_desc* d, Handle** out) {
 }
 
 // Picks the kernel for an element type and vector width.
-#define MMR_PICK(KERNEL, dt, vb)                                                                              \
-  ((dt) == MMR_DTYPE_F32                                                                                      \
-       ? ((vb) == 16 ? KERNEL<float, 16> : (vb) == 8 ? KERNEL<float, 8> : KERNEL<float, 4>)                   \
-   : (dt) == MMR_DTYPE_BF16                                                                                   \
-       ? ((vb) == 16 ? KERNEL<__nv_bfloat16, 16> : (vb) == 8 ? KERNEL<__nv_bfloat16, 8>                       \
-          : (vb) == 4 ? KERNEL<__nv_bfloat16, 4> : KERNEL<__nv_bfloat16, 2>)                                  \
-       : ((vb) == 16 ? KERNEL<__half, 16> : (vb) == 8 ? KERNEL<__half, 8> : (vb) == 4 ? KERNEL<__half, 4>     \
-                                                                                       : KERNEL<__half, 2>))
+#define MMR_PICK(KERNEL, dt, vb, X)                                                                            \
+  ((dt) == MMR_DTYPE_F32                                                                                       \
+       ? ((vb) == 16 ? KERNEL<float, 16, X> : (vb) == 8 ? KERNEL<float, 8, X> : KERNEL<float, 4, X>)           \
+   : (dt) == MMR_DTYPE_BF16                                                                                    \
+       ? ((vb) == 16 ? KERNEL<__nv_bfloat16, 16, X> : (vb) == 8 ? KERNEL<__nv_bfloat16, 8, X>                  \
+          : (vb) == 4 ? KERNEL<__nv_bfloat16, 4, X> : KERNEL<__nv_bfloat16, 2, X>)                             \
+       : ((vb) == 16 ? KERNEL<__half, 16, X> : (vb) == 8 ? KERNEL<__half, 8, X> : (vb) == 4 ? KERNEL<__half, 4, X> \
+                                                                                            : KERNEL<__half, 2, X>))
 
 int32_t combine_bind(const mmr_combine_desc* d, Handle** out) {
   if (!out) return fail(MMR_ERR_INVALID_ARGUMENT, "null output handle pointer");
@@ -1084,7 +1167,7 @@ int32_t combine_bind(const mmr_combine_desc* d, Handle** out) {
     p.row_vecs = int(width * rows.es / vb);
     const int64_t units = l.tokens * ((p.row_vecs + 127) / 128);
     const int grid = int(std::min<int64_t>(units, int64_t(1) << 30));
-    auto kernel = MMR_PICK(mmr::mmr_combine_kernel, rows.dtype, vb);
+    auto kernel = MMR_PICK(mmr::mmr_combine_kernel, rows.dtype, vb, 4);
     add_step(h.get(), "mmr_combine_kernel grid %lld, %lld-byte vectors", [=](cudaStream_t s) {
       return mmr::launch_kernel(kernel, dim3(grid), dim3(128), 0, s, dim3(1, 1, 1), p);
     }, grid, vb);
@@ -1143,9 +1226,12 @@ int32_t combine_grad_bind(const mmr_combine_grad_desc* d, Handle** out) {
   p.dw_t = dw.s[1];
   p.dw_j = dw.s[2];
   p.row_vecs = int(width * dy.es / vb);
-  p.zero_blocks = dr.on && width > 0 ? int(std::min<int64_t>((l.rows + 31) / 32, 4 * sms)) : 0;
-  const int grid = int(l.tokens) + p.zero_blocks;
-  auto kernel = MMR_PICK(mmr::mmr_combine_grad_kernel, dy.dtype, vb);
+  p.zero_blocks = dr.on && width > 0 ? int(std::min<int64_t>((l.rows + 255) / 256, 4 * sms)) : 0;
+  // A warp a token from eight warps an SM on; below that a block a token.
+  const bool warps = l.tokens >= 8 * sms;
+  const int grid = int(warps ? (l.tokens + 7) / 8 : l.tokens) + p.zero_blocks;
+  auto kernel = warps ? MMR_PICK(mmr::mmr_combine_grad_kernel, dy.dtype, vb, 1)
+                      : MMR_PICK(mmr::mmr_combine_grad_kernel, dy.dtype, vb, 8);
   if (grid > 0)
     add_step(h.get(), "mmr_combine_grad_kernel grid %lld, %lld-byte vectors", [=](cudaStream_t s) {
       return mmr::launch_kernel(kernel, dim3(grid), dim3(256), 0, s, dim3(1, 1, 1), p);

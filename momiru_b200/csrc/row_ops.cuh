@@ -17,17 +17,70 @@ struct PackParams {
   const void* src = nullptr;
   void* dst = nullptr;  // [batch][rows][pitch], columns past `cols` zeroed
   long long s_b = 0, s_r = 0, s_c = 0;  // source strides (elements, signed)
-  int rows = 0, cols = 0, pitch = 0;
+  int rows = 0, cols = 0, pitch = 0, batch = 1;
+};
+struct PackList {
+  PackParams p[2];
+  int n = 0;
 };
 
-// 32 x 32 tiles through shared memory: the read runs along whichever source
-// axis has the smaller stride, the write along the rows of the destination.
-__global__ void __launch_bounds__(256) mmr_pack_kernel(const PackParams p) {
+// Eight 16-bit elements from `src`, which may lie on any element: whole 32-bit
+// words, shifted by a half word where they straddle. The words read are inside
+// src[0, 8) and, when they straddle, src[-1, 9): the caller has those.
+__device__ __forceinline__ uint4 pack_load8(const unsigned short* src) {
+  uint4 v;
+  if ((reinterpret_cast<uintptr_t>(src) & 2) == 0) {
+    const unsigned int* w = reinterpret_cast<const unsigned int*>(src);
+    v = make_uint4(__ldg(w), __ldg(w + 1), __ldg(w + 2), __ldg(w + 3));
+  } else {
+    const unsigned int* w = reinterpret_cast<const unsigned int*>(src - 1);
+    const unsigned int a = __ldg(w), b = __ldg(w + 1), c = __ldg(w + 2), d = __ldg(w + 3), e = __ldg(w + 4);
+    v = make_uint4(__funnelshift_r(a, b, 16), __funnelshift_r(b, c, 16), __funnelshift_r(c, d, 16),
+                   __funnelshift_r(d, e, 16));
+  }
+  return v;
+}
+
+// Grid (blocks, operands, matrices). Rows that are contiguous in the source:
+// one 16-byte vector of the destination a thread (2.2 TB/s read and as much
+// written would be the copy's floor; element by element it ran at a sixth of
+// that). Other strides: 32 x 32 tiles through shared memory, the read running
+// along whichever source axis has the smaller stride.
+__global__ void __launch_bounds__(256) mmr_pack_kernel(const PackList list) {
   __shared__ unsigned short tile[32][34];
   griddep_wait();
   griddep_release();
+  const PackParams p = blockIdx.y ? list.p[1] : list.p[0];
+  if (static_cast<int>(blockIdx.z) >= p.batch) return;
   const unsigned short* src = static_cast<const unsigned short*>(p.src) + blockIdx.z * p.s_b;
   unsigned short* dst = static_cast<unsigned short*>(p.dst) + static_cast<long long>(blockIdx.z) * p.rows * p.pitch;
+  if (p.s_c == 1) {
+    const unsigned int vecs = p.pitch / 8;
+    const long long total = static_cast<long long>(p.rows) * vecs, step = gridDim.x * 256ll;
+    for (long long i0 = blockIdx.x * 256ll + threadIdx.x; i0 < total; i0 += 4 * step) {
+      uint4 v[4];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const long long i = i0 + q * step;
+        if (i >= total) continue;
+        const long long r = i / vecs;
+        const int c = static_cast<int>(i - r * vecs) * 8;
+        const unsigned short* s = src + r * p.s_r + c;
+        if (c > 0 && c + 9 <= p.cols) {
+          v[q] = pack_load8(s);
+        } else {
+          unsigned short t[8];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) t[x] = c + x < p.cols ? s[x] : 0;
+          memcpy(&v[q], t, 16);
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q)
+        if (i0 + q * step < total) reinterpret_cast<uint4*>(dst)[i0 + q * step] = v[q];
+    }
+    return;
+  }
   const int x = threadIdx.x & 31, y = threadIdx.x >> 5;
   const long long ar = p.s_r < 0 ? -p.s_r : p.s_r, ac = p.s_c < 0 ? -p.s_c : p.s_c;
   const bool along_rows = ar < ac;
@@ -72,12 +125,12 @@ __device__ __forceinline__ float lact_grad(int act, float x) {
     return fmaf(0.39894228040143f * x, expf(-0.5f * x * x), normcdff(x));
   }
   if (act == ACT_SILU) {
-    const float s = FAST ? __fdividef(1.0f, 1.0f + __expf(-x)) : 1.0f / (1.0f + expf(-x));
+    const float s = FAST ? fast_sigmoid(x) : 1.0f / (1.0f + expf(-x));
     return s * fmaf(x, 1.0f - s, 1.0f);
   }
   // gelu_tanh: with s = (1 + tanh u) / 2, d(x s) = s + 2 x s (1 - s) u'
-  const float u2 = x * fmaf(0.0713548162726f, x * x, 1.5957691216057f);
-  const float s = FAST ? __fdividef(1.0f, 1.0f + __expf(-u2)) : 1.0f / (1.0f + expf(-u2));
+  const float s =
+      FAST ? gelu_gate(x) : 1.0f / (1.0f + expf(-x * fmaf(0.0713548162726f, x * x, 1.5957691216057f)));
   const float du2 = fmaf(0.2140644488178f, x * x, 1.5957691216057f);
   return fmaf(x * s * (1.0f - s), du2, s);
 }
@@ -86,83 +139,93 @@ constexpr int AG_ROWS = 64;   // rows of one block: a chunk of the column sums
 constexpr int AG_COLS = 256;  // columns of one block: 32 threads x 8
 
 struct ActGradParams {
-  EpiMat d_out, pre, d_pre;  // d_pre.p null: only the column sums
+  EpiMat d_out, pre, d_pre;  // without an activation only the column sums are made
   float* partial = nullptr;  // [chunks][n] column sums of 64-row chunks, or null
   long long rows = 0;
   int n = 0, act = 0;
   const int* sources = nullptr;  // sorted rows: a row without a token counts as zero
 };
 
-template <typename T>
-__device__ __forceinline__ void ag_load8(const EpiMat& m, long long row, int col, int n, float (&v)[8]) {
-  const T* q = static_cast<const T*>(m.p) + row * m.ld + col * m.cs;
-  if (m.vec && col + 8 <= n) {
-    constexpr int kVec = sizeof(T) == 4 ? 2 : 1;
-    uint4 w[kVec];
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) w[i] = __ldg(reinterpret_cast<const uint4*>(q) + i);
-    const T* t = reinterpret_cast<const T*>(w);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = to_f32<T>(t[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = col + i < n ? to_f32<T>(q[i * m.cs]) : 0.0f;
-  }
-}
-template <typename T>
-__device__ __forceinline__ void ag_store8(const EpiMat& m, long long row, int col, int n, const float (&v)[8]) {
-  T* q = static_cast<T*>(m.p) + row * m.ld + col * m.cs;
-  T t[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) t[i] = from_f32<T>(v[i]);
-  if (m.vec && col + 8 <= n) {
-    constexpr int kVec = sizeof(T) == 4 ? 2 : 1;
-    uint4 w[kVec];
-    memcpy(w, t, sizeof w);
-#pragma unroll
-    for (int i = 0; i < kVec; ++i) reinterpret_cast<uint4*>(q)[i] = w[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (col + i < n) q[i * m.cs] = t[i];
-  }
-}
-
-// Grid (column strips, row chunks). The sums are of the f32 values, before
-// d_pre is rounded. Chunk sums go out in f32 and are added in chunk order by
+// Grid (column strips, row chunks). A thread has eight columns of a strip: with
+// VEC neighbouring ones, one 16-byte vector (two in f32) a row, several rows'
+// loads in flight together; without, every 32nd, so that a warp's accesses stay
+// contiguous for any pitch. The sums are of the f32 values, before d_pre is
+// rounded. Chunk sums go out in f32 and are added in chunk order by
 // mmr_col_sum_kernel, so the result does not depend on which block ran first.
-template <typename T>
-__global__ void __launch_bounds__(256) mmr_act_grad_kernel(const ActGradParams p) {
+template <typename T, int ACT, bool VEC>
+__global__ void __launch_bounds__(256, 3) mmr_act_grad_kernel(const ActGradParams p) {
+  constexpr int kRows = VEC ? (sizeof(T) == 2 ? 4 : 2) : 1;
+  constexpr int kVec = sizeof(T) / 2;
+  union Raw {
+    uint4 w[kVec];
+    T t[8];
+    __device__ Raw() {}
+  };
   __shared__ float sums[8][AG_COLS];
   griddep_wait();
   griddep_release();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-  const int col = static_cast<int>(blockIdx.x) * AG_COLS + tx * 8;
+  const int c0 = static_cast<int>(blockIdx.x) * AG_COLS;
+  auto col = [&](int i) { return VEC ? tx * 8 + i : tx + 32 * i; };
+  auto load = [&](const EpiMat& m, long long row, Raw& r) {
+    const T* q = static_cast<const T*>(m.p) + row * m.ld;
+    if (VEC) {
+#pragma unroll
+      for (int i = 0; i < kVec; ++i) r.w[i] = __ldg(reinterpret_cast<const uint4*>(q + c0 + tx * 8) + i);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r.t[i] = c0 + col(i) < p.n ? q[(c0 + col(i)) * m.cs] : from_f32<T>(0.0f);
+    }
+  };
   for (long long chunk = blockIdx.y; chunk * AG_ROWS < p.rows; chunk += gridDim.y) {
     float s[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 4
-    for (int i = 0; i < AG_ROWS / 8; ++i) {
-      const long long row = chunk * AG_ROWS + i * 8 + ty;
-      if (row >= p.rows || col >= p.n) continue;
-      float d[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-      if (!p.sources || p.sources[row] >= 0) {
-        ag_load8<T>(p.d_out, row, col, p.n, d);
-        if (p.act != ACT_NONE) {
-          float x[8];
-          ag_load8<T>(p.pre, row, col, p.n, x);
+    if (!VEC || c0 + tx * 8 < p.n) {
+#pragma unroll 1
+      for (int i = 0; i < AG_ROWS / 8; i += kRows) {
+        Raw d[kRows], x[kRows];
+        bool held[kRows];
 #pragma unroll
-          for (int q = 0; q < 8; ++q) d[q] *= lact_grad<sizeof(T) == 2>(p.act, x[q]);
+        for (int q = 0; q < kRows; ++q) {
+          const long long row = chunk * AG_ROWS + (i + q) * 8 + ty;
+          held[q] = row < p.rows && (!p.sources || p.sources[row] >= 0);
+          if (held[q]) {
+            load(p.d_out, row, d[q]);
+            if (ACT != ACT_NONE) load(p.pre, row, x[q]);
+          }
+        }
+#pragma unroll
+        for (int q = 0; q < kRows; ++q) {
+          const long long row = chunk * AG_ROWS + (i + q) * 8 + ty;
+          Raw o;
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            float v = 0.0f;
+            if (held[q]) {
+              v = to_f32<T>(d[q].t[c]);
+              if (ACT != ACT_NONE) v *= lact_grad<sizeof(T) == 2>(ACT, to_f32<T>(x[q].t[c]));
+            }
+            s[c] += v;
+            o.t[c] = from_f32<T>(v);
+          }
+          if (ACT != ACT_NONE && row < p.rows) {
+            T* to = static_cast<T*>(p.d_pre.p) + row * p.d_pre.ld + c0;  // the workspace: dense rows
+            if (VEC) {
+#pragma unroll
+              for (int w = 0; w < kVec; ++w) reinterpret_cast<uint4*>(to + tx * 8)[w] = o.w[w];
+            } else {
+#pragma unroll
+              for (int c = 0; c < 8; ++c)
+                if (c0 + col(c) < p.n) to[col(c)] = o.t[c];
+            }
+          }
         }
       }
-      if (p.d_pre.p) ag_store8<T>(p.d_pre, row, col, p.n, d);
-#pragma unroll
-      for (int q = 0; q < 8; ++q) s[q] += d[q];
     }
     if (p.partial) {
 #pragma unroll
-      for (int q = 0; q < 8; ++q) sums[ty][tx * 8 + q] = s[q];
+      for (int q = 0; q < 8; ++q) sums[ty][col(q)] = s[q];
       __syncthreads();
-      const int c = static_cast<int>(blockIdx.x) * AG_COLS + static_cast<int>(threadIdx.x);
+      const int c = c0 + static_cast<int>(threadIdx.x);
       float t = 0.0f;
 #pragma unroll
       for (int y = 0; y < 8; ++y) t += sums[y][threadIdx.x];
@@ -209,22 +272,40 @@ __global__ void __launch_bounds__(256) mmr_col_sum_kernel(const ColSumParams p) 
 // out = act(pre) + residual over an f32 product that was left in `out` or kept
 // in `pre` (the f32 linear node with a residual or a kept pre).
 struct ActResParams {
-  const float* pre = nullptr;
-  const float* residual = nullptr;
-  float* out = nullptr;
-  long long pre_ld = 0, res_ld = 0, res_cs = 0, out_ld = 0, out_cs = 0, pre_cs = 0;
-  int m = 0, n = 0, act = 0;
+  EpiMat pre, residual, out;  // residual.p may be null
+  int m = 0, n = 0;
 };
 
+// A warp per row piece of 128 columns, four columns a thread where all three
+// are 16-byte vectors.
+template <int ACT>
 __global__ void __launch_bounds__(256) mmr_act_res_kernel(const ActResParams p) {
   griddep_wait();
   griddep_release();
-  const long long total = static_cast<long long>(p.m) * p.n;
-  for (long long i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-    const long long r = i / p.n, c = i - r * p.n;
-    float x = act_apply(p.act, p.pre[r * p.pre_ld + c * p.pre_cs]);
-    if (p.residual) x += p.residual[r * p.res_ld + c * p.res_cs];
-    p.out[r * p.out_ld + c * p.out_cs] = x;
+  const int lane = threadIdx.x & 31;
+  const int pieces = (p.n + 127) / 128;
+  const long long units = static_cast<long long>(p.m) * pieces, step = static_cast<long long>(gridDim.x) * 8;
+  const bool vec = p.pre.vec && p.out.vec && (!p.residual.p || p.residual.vec);
+  const float *pre = static_cast<const float*>(p.pre.p), *res = static_cast<const float*>(p.residual.p);
+  float* out = static_cast<float*>(p.out.p);
+  for (long long u = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5); u < units; u += step) {
+    const long long row = u / pieces;
+    const int c0 = static_cast<int>(u - row * pieces) * 128;
+    if (vec && c0 + 128 <= p.n) {
+      const int c = c0 + lane * 4;
+      const float4 x = __ldg(reinterpret_cast<const float4*>(pre + row * p.pre.ld + c));
+      float4 r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (res) r = *reinterpret_cast<const float4*>(res + row * p.residual.ld + c);
+      *reinterpret_cast<float4*>(out + row * p.out.ld + c) =
+          make_float4(act_apply(ACT, x.x) + r.x, act_apply(ACT, x.y) + r.y, act_apply(ACT, x.z) + r.z,
+                      act_apply(ACT, x.w) + r.w);
+    } else {
+      for (int c = c0 + lane; c < min(c0 + 128, p.n); c += 32) {
+        float x = act_apply(ACT, pre[row * p.pre.ld + c * p.pre.cs]);
+        if (res) x += res[row * p.residual.ld + c * p.residual.cs];
+        out[row * p.out.ld + c * p.out.cs] = x;
+      }
+    }
   }
 }
 
