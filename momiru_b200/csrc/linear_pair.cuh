@@ -42,6 +42,8 @@
 namespace mmr {
 
 constexpr int LP_THREADS = 384;
+constexpr int LP_LAUNCH_REGS = 168, LP_EPI_REGS = 208, LP_OTHER_REGS = 80;
+static_assert(256 * LP_EPI_REGS + 128 * LP_OTHER_REGS <= LP_THREADS * LP_LAUNCH_REGS, "register split exceeds the launch");
 constexpr int LP_BK = 64;
 constexpr int LP_A_BYTES = 128 * LP_BK * 2;
 constexpr int LP_CSTAGE_BYTES = 4096;  // per epilogue warp: 32 rows x 32 f32
@@ -215,6 +217,8 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
   griddep_release();
   const uint32_t tmem = *tmem_slot;
 
+  if (warp < 8) reg_alloc<LP_EPI_REGS>();
+  else reg_dealloc<LP_OTHER_REGS>();
   if (warp < 8) {
     // ------------------------------------------------------------- epilogue
     const int quarter = warp & 3, half = warp >> 2;
@@ -225,6 +229,15 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
     LpWalk<RAG> walk(p, table, pair, npairs);
     LpTile w;
     const bool vec = epi_vec(p.epi);
+    // The bias eight columns at a time: n and the experts' rows multiples of 8,
+    // loaded a box ahead.
+    const bool vec_bias = vec && p.epi.bias && p.epi.bias_s == 1 && (p.n & 7) == 0 && (p.epi.bias_bs & 7) == 0 &&
+                          (reinterpret_cast<uintptr_t>(p.epi.bias) & 15) == 0;
+    auto load_bias16 = [&](const LpTile& w, int col0) {
+      const int col = col0 + (lane & 3) * 8;
+      const T* q = static_cast<const T*>(p.epi.bias) + w.batch * p.epi.bias_bs + col;
+      return vec_bias && col < p.n ? __ldg(reinterpret_cast<const uint4*>(q)) : make_uint4(0, 0, 0, 0);
+    };
     // The residual of one 32 x 32 box, in the layout it is added in: vector `it`
     // of lane l is row 8 it + l / 4, columns 8 (l % 4) of the box.
     auto load_residual = [&](const LpTile& w, int row0, int col0, uint4 (&res)[4]) {
@@ -238,13 +251,19 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
     // Stores one staged 32 x 32 box (row r: 16-byte chunk q at q ^ (r & 7)). All
     // 32 of a lane's values go through each step together: with two warps a
     // scheduler, their independence is what hides the latencies.
-    auto store_box = [&](const LpTile& w, int row0, int col0, const uint4 (&res)[4]) {
+    auto store_box = [&](const LpTile& w, int row0, int col0, const uint4 (&res)[4], const uint4& bias16) {
       const long long batch = RAG == 2 ? w.batch : 0;
       if (vec) {
         const int c2 = (lane & 3) * 2, col = col0 + (lane & 3) * 8, r0 = lane >> 2;
         if (col >= p.n) return;
         float bias[8];
-        load_bias8<T>(p.epi, w.batch, col, bias);
+        if (vec_bias) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) bias[i] = 0.0f;
+          add8<T>(bias, bias16);
+        } else {
+          load_bias8<T>(p.epi, w.batch, col, bias);
+        }
         if (col + 8 <= p.n && row0 + 32 <= w.row_end) {
           float v[32];
 #pragma unroll
@@ -285,25 +304,36 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
         if (col >= p.n) return;
         const float bias =
             p.epi.bias ? to_f32<T>(static_cast<const T*>(p.epi.bias)[w.batch * p.epi.bias_bs + col * p.epi.bias_s]) : 0.0f;
-        const T* res = p.epi.residual.p ? static_cast<const T*>(p.epi.residual.p) + col * p.epi.residual.cs : nullptr;
-        const int rows = min(max(w.row_end, w.zero_end) - row0, 32);
-        for (int r0 = 0; r0 < rows; r0 += 8) {
-          float add[8];
+        const int rows = min(w.row_end - row0, 32);  // rows past the tokens are zeroed below
+        float add[32];
+        if (p.epi.residual.p) {
+          const T* q = static_cast<const T*>(p.epi.residual.p) + row0 * p.epi.residual.ld + col * p.epi.residual.cs;
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
-            add[q] = res && row0 + r0 + q < w.row_end ? to_f32<T>(res[(row0 + r0 + q) * p.epi.residual.ld]) : 0.0f;
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            const int rr = r0 + q, row = row0 + rr;
-            const float v = *reinterpret_cast<const float*>(buf + rr * 128 + ((((lane >> 2) ^ (rr & 7)) << 4) | ((lane & 3) << 2)));
-            if (row < w.row_end) {
-              epi_store1<T>(p.epi, batch, row, col, v, bias, add[q]);
-            } else if (RAG == 1 && row < w.zero_end) {
-              if (p.epi.pre.p) static_cast<T*>(p.epi.pre.p)[row * p.epi.pre.ld + col * p.epi.pre.cs] = from_f32<T>(0.0f);
-              static_cast<T*>(p.epi.out.p)[row * p.epi.out.ld + col * p.epi.out.cs] = from_f32<T>(0.0f);
-            }
+          for (int r = 0; r < 32; ++r) {
+            add[r] = r < rows ? to_f32<T>(*q) : 0.0f;
+            q += p.epi.residual.ld;
           }
         }
+        float v[32];
+#pragma unroll
+        for (int r = 0; r < 32; ++r)
+          v[r] = bias + *reinterpret_cast<const float*>(buf + r * 128 + ((((lane >> 2) ^ (r & 7)) << 4) | ((lane & 3) << 2)));
+        auto put = [&](const EpiMat& m) {
+          T* q = static_cast<T*>(m.p) + batch * m.bs + row0 * m.ld + col * m.cs;
+#pragma unroll
+          for (int r = 0; r < 32; ++r) {
+            if (r < rows) *q = from_f32<T>(v[r]);
+            else if (RAG == 1 && row0 + r < w.zero_end) *q = from_f32<T>(0.0f);
+            q += m.ld;
+          }
+        };
+        if (p.epi.pre.p) put(p.epi.pre);
+        lact_apply(p.epi.act, v);
+        if (p.epi.residual.p) {
+#pragma unroll
+          for (int r = 0; r < 32; ++r) v[r] += add[r];
+        }
+        put(p.epi.out);
       }
     };
     while (walk.next(w)) {
@@ -313,14 +343,14 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
       const int cbase = w.col0 + half * boxes * 32;
       const bool adds = vec && p.epi.residual.p && cbase < p.n && row0 < w.row_end;
       uint4 res[2][4];
-      if (adds) {
-        // under the MMAs: the tile's residual to L2, its first box to registers
-        if (row0 + lane < w.row_end) {
-          const T* q = static_cast<const T*>(p.epi.residual.p) + (row0 + lane) * p.epi.residual.ld + cbase;
-          for (int c = 0; c < boxes * 32 && cbase + c < p.n; c += 64) prefetch_l2(q + c);
-        }
-        load_residual(w, row0, cbase, res[0]);
+      // under the MMAs: the tile's residual to L2, its first box to registers
+      if (p.epi.residual.p && row0 + lane < w.row_end) {
+        const T* q = static_cast<const T*>(p.epi.residual.p) + (row0 + lane) * p.epi.residual.ld;
+        for (int c = cbase; c < min(cbase + boxes * 32, p.n); c += 64) prefetch_l2(q + c * p.epi.residual.cs);
       }
+      if (adds) load_residual(w, row0, cbase, res[0]);
+      uint4 bias16[2];
+      bias16[0] = load_bias16(w, cbase);
       if (sums) {
         if (!mbar_wait_cluster(&acc_full[acc], acc_phase, ctl, kDevTimeoutAcc)) break;
         tc_fence_after();
@@ -331,7 +361,10 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           const int j = j2 + b, col0 = cbase + j * 32;
-          if (adds && j + 1 < boxes) load_residual(w, row0, col0 + 32, res[b ^ 1]);
+          if (j + 1 < boxes) {
+            if (adds) load_residual(w, row0, col0 + 32, res[b ^ 1]);
+            bias16[b ^ 1] = load_bias16(w, col0 + 32);
+          }
           uint32_t r[32];
           if (sums) {
             tmem_ld_32x32b_x32(tb + j * 32, r);
@@ -352,7 +385,7 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
             *reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) << 4)) =
                 make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
           __syncwarp();
-          store_box(w, row0, col0, res[b]);
+          store_box(w, row0, col0, res[b], bias16[b]);
         }
       }
       if (sums && ++acc == 2) { acc = 0; acc_phase ^= 1u; }

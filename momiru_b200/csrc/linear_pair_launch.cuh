@@ -33,6 +33,12 @@ template <typename T>
 cudaError_t pair_prepare_t(const PairShape& sh) {
   const PairKernel k = pair_kernel<T>(sh);
   if (!k) return cudaErrorInvalidValue;
+  // setmaxnreg.inc waits for registers that the launch has to have: a build
+  // compiled with fewer is refused here instead of launched.
+  cudaFuncAttributes fa;
+  const cudaError_t e = cudaFuncGetAttributes(&fa, reinterpret_cast<const void*>(k));
+  if (e != cudaSuccess) return e;
+  if (fa.numRegs * LP_THREADS < 256 * LP_EPI_REGS + 128 * LP_OTHER_REGS) return cudaErrorInvalidConfiguration;
   return cudaFuncSetAttribute(reinterpret_cast<const void*>(k), cudaFuncAttributeMaxDynamicSharedMemorySize,
                               lp_smem_bytes(sh.rag));
 }

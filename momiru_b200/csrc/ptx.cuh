@@ -302,6 +302,17 @@ __host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool bf16, bool a
          (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
 }
 
+// Registers of a warpgroup's threads, moved between warpgroups within what the
+// block was launched with.
+template <int N>
+__device__ __forceinline__ void reg_alloc() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void reg_dealloc() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N));
+}
+
 // ------------------------------------------------- clusters / CTA pairs --
 __device__ __forceinline__ uint32_t cluster_ctarank() {
   uint32_t r;

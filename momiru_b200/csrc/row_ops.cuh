@@ -153,7 +153,7 @@ struct ActGradParams {
 // rounded. Chunk sums go out in f32 and are added in chunk order by
 // mmr_col_sum_kernel, so the result does not depend on which block ran first.
 template <typename T, int ACT, bool VEC>
-__global__ void __launch_bounds__(256, 3) mmr_act_grad_kernel(const ActGradParams p) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) mmr_act_grad_kernel(const ActGradParams p) {
   constexpr int kRows = VEC ? (sizeof(T) == 2 ? 4 : 2) : 1;
   constexpr int kVec = sizeof(T) / 2;
   union Raw {
@@ -167,58 +167,64 @@ __global__ void __launch_bounds__(256, 3) mmr_act_grad_kernel(const ActGradParam
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int c0 = static_cast<int>(blockIdx.x) * AG_COLS;
   auto col = [&](int i) { return VEC ? tx * 8 + i : tx + 32 * i; };
-  auto load = [&](const EpiMat& m, long long row, Raw& r) {
-    const T* q = static_cast<const T*>(m.p) + row * m.ld;
+  auto load = [&](const T* q, const EpiMat& m, Raw& r) {
     if (VEC) {
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) r.w[i] = __ldg(reinterpret_cast<const uint4*>(q + c0 + tx * 8) + i);
+      for (int i = 0; i < kVec; ++i) r.w[i] = __ldg(reinterpret_cast<const uint4*>(q + tx * 8) + i);
     } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) r.t[i] = c0 + col(i) < p.n ? q[(c0 + col(i)) * m.cs] : from_f32<T>(0.0f);
+      for (int i = 0; i < 8; ++i) r.t[i] = c0 + col(i) < p.n ? q[col(i) * m.cs] : from_f32<T>(0.0f);
     }
   };
   for (long long chunk = blockIdx.y; chunk * AG_ROWS < p.rows; chunk += gridDim.y) {
     float s[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
     if (!VEC || c0 + tx * 8 < p.n) {
+      const long long row0 = chunk * AG_ROWS + ty;
+      const int left = static_cast<int>(min(p.rows - row0, static_cast<long long>(AG_ROWS)));  // rows 0, 8, .. below this
+      const T* dq = static_cast<const T*>(p.d_out.p) + row0 * p.d_out.ld + c0 * p.d_out.cs;
+      const T* xq = static_cast<const T*>(p.pre.p) + row0 * p.pre.ld + c0 * p.pre.cs;
+      T* oq = static_cast<T*>(p.d_pre.p) + row0 * p.d_pre.ld + c0;  // the workspace: dense rows
 #pragma unroll 1
-      for (int i = 0; i < AG_ROWS / 8; i += kRows) {
+      for (int i = 0; i < AG_ROWS; i += 8 * kRows) {
         Raw d[kRows], x[kRows];
         bool held[kRows];
 #pragma unroll
         for (int q = 0; q < kRows; ++q) {
-          const long long row = chunk * AG_ROWS + (i + q) * 8 + ty;
-          held[q] = row < p.rows && (!p.sources || p.sources[row] >= 0);
+          held[q] = i + 8 * q < left && (!p.sources || p.sources[row0 + i + 8 * q] >= 0);
           if (held[q]) {
-            load(p.d_out, row, d[q]);
-            if (ACT != ACT_NONE) load(p.pre, row, x[q]);
+            load(dq + 8 * q * p.d_out.ld, p.d_out, d[q]);
+            if (ACT != ACT_NONE) load(xq + 8 * q * p.pre.ld, p.pre, x[q]);
           }
         }
 #pragma unroll
         for (int q = 0; q < kRows; ++q) {
-          const long long row = chunk * AG_ROWS + (i + q) * 8 + ty;
-          Raw o;
+          float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+          if (held[q]) {
 #pragma unroll
-          for (int c = 0; c < 8; ++c) {
-            float v = 0.0f;
-            if (held[q]) {
-              v = to_f32<T>(d[q].t[c]);
-              if (ACT != ACT_NONE) v *= lact_grad<sizeof(T) == 2>(ACT, to_f32<T>(x[q].t[c]));
+            for (int c = 0; c < 8; ++c) {
+              v[c] = to_f32<T>(d[q].t[c]);
+              if (ACT != ACT_NONE) v[c] *= lact_grad<sizeof(T) == 2>(ACT, to_f32<T>(x[q].t[c]));
+              s[c] += v[c];
             }
-            s[c] += v;
-            o.t[c] = from_f32<T>(v);
           }
-          if (ACT != ACT_NONE && row < p.rows) {
-            T* to = static_cast<T*>(p.d_pre.p) + row * p.d_pre.ld + c0;  // the workspace: dense rows
-            if (VEC) {
+          if (ACT != ACT_NONE && i + 8 * q < left) {
+            T* to = oq + 8 * q * p.d_pre.ld;
+            if constexpr (VEC && sizeof(T) == 2) {
+              *reinterpret_cast<uint4*>(to + tx * 8) = pack8<T>(v);
+            } else if (VEC) {
 #pragma unroll
-              for (int w = 0; w < kVec; ++w) reinterpret_cast<uint4*>(to + tx * 8)[w] = o.w[w];
+              for (int c = 0; c < 8; c += 4)
+                *reinterpret_cast<float4*>(to + tx * 8 + c) = make_float4(v[c], v[c + 1], v[c + 2], v[c + 3]);
             } else {
 #pragma unroll
               for (int c = 0; c < 8; ++c)
-                if (c0 + col(c) < p.n) to[col(c)] = o.t[c];
+                if (c0 + col(c) < p.n) to[col(c)] = from_f32<T>(v[c]);
             }
           }
         }
+        dq += 8 * kRows * p.d_out.ld;
+        xq += 8 * kRows * p.pre.ld;
+        oq += 8 * kRows * p.d_pre.ld;
       }
     }
     if (p.partial) {

@@ -205,15 +205,6 @@ __device__ __forceinline__ void tc_tile_coords(const TcParams& p, int t, int& mt
   nt = q / gsize;
 }
 
-template <int N>
-__device__ __forceinline__ void reg_alloc() {
-  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;\n" ::"n"(N));
-}
-template <int N>
-__device__ __forceinline__ void reg_dealloc() {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;\n" ::"n"(N));
-}
-
 template <int MODE, bool A_MN, bool B_MN>
 __global__ void __launch_bounds__(TcConfig<MODE>::kThreads, 1)
     mmr_tc_gemm_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
