@@ -1334,6 +1334,19 @@ int32_t mmr_gemm_run_on(mmr_gemm_handle* h, void* stream) {
   return MMR_OK;
 }
 
+}  // extern "C"
+
+namespace mmr {
+// For the linear layer's f32 products: K chunks of `k` elements in tensor
+// memory instead of 256 (3xTF32 only; no effect on other handles).
+void gemm_set_chunk(mmr_gemm_handle* h, int k) {
+  if (h->family == MMR_FAMILY_TCGEN05 && h->mode == 1)
+    h->tcp.chunk_kb = std::max(1, std::min(k / int(h->launch.bk), h->tcp.k_blocks));
+}
+}  // namespace mmr
+
+extern "C" {
+
 int32_t mmr_gemm_run(mmr_gemm_handle* h) {
   if (!h) return fail(MMR_ERR_INVALID_ARGUMENT, "null handle");
   return mmr_gemm_run_on(h, h->stream);

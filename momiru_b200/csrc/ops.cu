@@ -27,7 +27,9 @@
 #include "row_ops.cuh"
 
 namespace mmr {
-int32_t set_last_error(int32_t code, const char* message);  // momiru_gemm.cu
+// momiru_gemm.cu
+int32_t set_last_error(int32_t code, const char* message);
+void gemm_set_chunk(mmr_gemm_handle* h, int k);
 }
 
 struct mmr_op_handle {
@@ -746,6 +748,12 @@ mmr_view transposed(mmr_view v) {
   return v;
 }
 
+// K elements summed in tensor memory at a time. The tensor core's additions
+// truncate, and the error of a product is that of one chunk: 2.1e-6 relative at
+// the node's 256, 1.2e-6 at 128, 7.9e-7 at 64, 5.7e-7 at 32, for 256 / 272 / 290
+// / 323 us at 2048 x 4096 x 4096. A layer's f32 sums are kept below 1e-6.
+constexpr int kF32Chunk = 64;
+
 int32_t add_f32_product(Handle* h, int math, const mmr_view& lhs, const mmr_view& rhs, const mmr_view& out,
                         const Ref* bias, int epilogue) {
   mmr_matmul_desc d{};
@@ -769,20 +777,10 @@ int32_t add_f32_product(Handle* h, int math, const mmr_view& lhs, const mmr_view
   mmr_gemm_handle* g = nullptr;
   MMR_TRY(mmr_gemm_bind(&d, &g));
   h->products.push_back(g);
+  mmr::gemm_set_chunk(g, kF32Chunk);
   h->plan += "matmul node (f32)\n";
   h->steps.push_back({"matmul node (f32)", [g](cudaStream_t s) { return mmr_gemm_run_on(g, s); }});
   return MMR_OK;
-}
-
-int f32_epilogue(int act, bool bias) {
-  switch (act) {
-    case MMR_ACT_RELU: return bias ? MMR_EPI_BIAS_RELU : MMR_EPI_RELU;
-    case MMR_ACT_RELU6: return bias ? MMR_EPI_BIAS_RELU6 : MMR_EPI_RELU6;
-    case MMR_ACT_GELU_ERF: return bias ? MMR_EPI_BIAS_GELU_ERF : MMR_EPI_GELU_ERF;
-    case MMR_ACT_GELU_TANH: return bias ? MMR_EPI_BIAS_GELU_TANH : MMR_EPI_GELU_TANH;
-    case MMR_ACT_SILU: return bias ? MMR_EPI_BIAS_SILU : MMR_EPI_SILU;
-    default: return bias ? MMR_EPI_BIAS : MMR_EPI_NONE;
-  }
 }
 
 int32_t check_math(int dtype, int math) {
@@ -863,31 +861,37 @@ int32_t linear_bind(const mmr_linear_desc* d, Handle** out) {
     return MMR_OK;
   }
   if (lhs.dtype == MMR_DTYPE_F32) {
-    if (!res.on && !pre.on) {
-      MMR_TRY(add_f32_product(h.get(), d->math_mode, f32_view(lhs, dev), f32_view(rhs, dev), f32_view(o, dev), &bias,
-                              f32_epilogue(d->activation, bias.on)));
+    const mmr_view a = f32_view(lhs, dev), b = f32_view(rhs, dev);
+    if (!res.on && !pre.on && d->activation == MMR_ACT_NONE) {
+      MMR_TRY(add_f32_product(h.get(), d->math_mode, a, b, f32_view(o, dev), &bias, bias.on ? MMR_EPI_BIAS : MMR_EPI_NONE));
     } else {
-      // The node leaves pre in its own buffer (or a workspace), and one pass
-      // applies the activation and adds the residual.
+      // The bare product goes to pre, or to out, or (where out is the residual)
+      // to a workspace, and one pass does the rest. The node's own epilogue takes
+      // an activation as a call per element: 2048 x 4096 x 4096 with bias and
+      // SiLU took 375 us in it, 256 bare.
       mmr::ActResParams q;
       mmr_view to;
       if (pre.on) {
         to = f32_view(pre, dev);
-        q.pre = epi_mat(pre);
+        q.x = q.pre = epi_mat(pre);
+      } else if (!res.on || !overlap(o, res)) {
+        to = f32_view(o, dev);
+        q.x = epi_mat(o);
       } else {
         void* w = nullptr;
         const int64_t ld = (n + 3) / 4 * 4;
         MMR_TRY(workspace(h.get(), size_t(m) * ld * 4, &w));
         to = f32_view(w, m, n, ld, dev);
-        q.pre.p = w;
-        q.pre.ld = ld;
-        q.pre.cs = 1;
-        q.pre.vec = 1;
+        q.x.p = w;
+        q.x.ld = ld;
+        q.x.cs = 1;
+        q.x.vec = 1;
       }
-      MMR_TRY(add_f32_product(h.get(), d->math_mode, f32_view(lhs, dev), f32_view(rhs, dev), to, &bias,
-                              f32_epilogue(MMR_ACT_NONE, bias.on)));
+      MMR_TRY(add_f32_product(h.get(), d->math_mode, a, b, to, nullptr, MMR_EPI_NONE));
       q.residual = epi_mat(res);
       q.out = epi_mat(o);
+      q.bias = reinterpret_cast<const float*>(bias.on ? bias.base : 0);
+      q.bias_s = bias.s[2];
       q.m = int(m);
       q.n = int(n);
       const int act = d->activation;

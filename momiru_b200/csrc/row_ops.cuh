@@ -274,42 +274,68 @@ __global__ void __launch_bounds__(256) mmr_col_sum_kernel(const ColSumParams p) 
   }
 }
 
-// ---------------------------------------------- activation and residual --
-// out = act(pre) + residual over an f32 product that was left in `out` or kept
-// in `pre` (the f32 linear node with a residual or a kept pre).
+// ------------------------------------- bias, activation and residual (f32) --
+// pre = x + bias; out = act(pre) + residual over a bare f32 product x, which may
+// lie in pre's or out's own storage (each element is read and written by one
+// thread). Bound by memory.
 struct ActResParams {
-  EpiMat pre, residual, out;  // residual.p may be null
+  EpiMat x, pre, residual, out;  // pre.p and residual.p may be null
+  const float* bias = nullptr;
+  long long bias_s = 0;
   int m = 0, n = 0;
 };
 
-// A warp per row piece of 128 columns, four columns a thread where all three
-// are 16-byte vectors.
+// The activations in f32, inlined (the matmul node's epilogue calls them out of
+// line): the formulas of linear_epi.cuh on CUDA's expf and normcdff and correctly
+// rounded divisions.
+template <int ACT>
+__device__ __forceinline__ float act_f32(float x) {
+  if (ACT == ACT_RELU) return act_relu(x);
+  if (ACT == ACT_RELU6) return x != x ? x : fminf(fmaxf(x, 0.0f), 6.0f);
+  if (ACT == ACT_SILU) return no_inf(x, __fdiv_rn(x, 1.0f + expf(-x)));
+  if (ACT == ACT_GELU_TANH) return no_inf(x, __fdiv_rn(x, 1.0f + expf(-x * fmaf(0.0713548162726f, x * x, 1.5957691216057f))));
+  if (ACT == ACT_GELU_ERF) return no_inf(x, x * normcdff(x));
+  return x;
+}
+
+// A warp takes 128 columns of a row, four columns a thread where everything is
+// 16-byte vectors.
 template <int ACT>
 __global__ void __launch_bounds__(256) mmr_act_res_kernel(const ActResParams p) {
   griddep_wait();
   griddep_release();
   const int lane = threadIdx.x & 31;
-  const int pieces = (p.n + 127) / 128;
+  const unsigned int pieces = (p.n + 127) / 128;
   const long long units = static_cast<long long>(p.m) * pieces, step = static_cast<long long>(gridDim.x) * 8;
-  const bool vec = p.pre.vec && p.out.vec && (!p.residual.p || p.residual.vec);
-  const float *pre = static_cast<const float*>(p.pre.p), *res = static_cast<const float*>(p.residual.p);
-  float* out = static_cast<float*>(p.out.p);
+  const bool vec = p.x.vec && p.out.vec && (!p.residual.p || p.residual.vec) && (!p.pre.p || p.pre.vec);
+  const float *x = static_cast<const float*>(p.x.p), *res = static_cast<const float*>(p.residual.p);
+  float *out = static_cast<float*>(p.out.p), *pre = static_cast<float*>(p.pre.p);
   for (long long u = static_cast<long long>(blockIdx.x) * 8 + (threadIdx.x >> 5); u < units; u += step) {
     const long long row = u / pieces;
     const int c0 = static_cast<int>(u - row * pieces) * 128;
     if (vec && c0 + 128 <= p.n) {
       const int c = c0 + lane * 4;
-      const float4 x = __ldg(reinterpret_cast<const float4*>(pre + row * p.pre.ld + c));
+      float4 v = *reinterpret_cast<const float4*>(x + row * p.x.ld + c);
       float4 r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (res) r = *reinterpret_cast<const float4*>(res + row * p.residual.ld + c);
-      *reinterpret_cast<float4*>(out + row * p.out.ld + c) =
-          make_float4(act_apply(ACT, x.x) + r.x, act_apply(ACT, x.y) + r.y, act_apply(ACT, x.z) + r.z,
-                      act_apply(ACT, x.w) + r.w);
+      if (p.bias) {
+        v.x = __fadd_rn(v.x, p.bias[c * p.bias_s]);
+        v.y = __fadd_rn(v.y, p.bias[(c + 1) * p.bias_s]);
+        v.z = __fadd_rn(v.z, p.bias[(c + 2) * p.bias_s]);
+        v.w = __fadd_rn(v.w, p.bias[(c + 3) * p.bias_s]);
+      }
+      if (pre) *reinterpret_cast<float4*>(pre + row * p.pre.ld + c) = v;
+      v = make_float4(act_f32<ACT>(v.x), act_f32<ACT>(v.y), act_f32<ACT>(v.z), act_f32<ACT>(v.w));
+      if (res) v = make_float4(v.x + r.x, v.y + r.y, v.z + r.z, v.w + r.w);
+      *reinterpret_cast<float4*>(out + row * p.out.ld + c) = v;
     } else {
       for (int c = c0 + lane; c < min(c0 + 128, p.n); c += 32) {
-        float x = act_apply(ACT, pre[row * p.pre.ld + c * p.pre.cs]);
-        if (res) x += res[row * p.residual.ld + c * p.residual.cs];
-        out[row * p.out.ld + c * p.out.cs] = x;
+        float v = x[row * p.x.ld + c * p.x.cs];
+        if (p.bias) v = __fadd_rn(v, p.bias[c * p.bias_s]);
+        if (pre) pre[row * p.pre.ld + c * p.pre.cs] = v;
+        v = act_f32<ACT>(v);
+        if (res) v += res[row * p.residual.ld + c * p.residual.cs];
+        out[row * p.out.ld + c * p.out.cs] = v;
       }
     }
   }
