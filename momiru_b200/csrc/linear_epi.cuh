@@ -216,6 +216,55 @@ __device__ __forceinline__ void epi_store1(const EpiParams& e, long long batch, 
   lact_apply(e.act, x);
   static_cast<T*>(e.out.p)[batch * e.out.bs + row * e.out.ld + col * e.out.cs] = from_f32<T>(x[0] + residual);
 }
+// Four rows of C neighbouring columns: v[4 c + r]. C 2 wants every view's pairs
+// of columns on one 32-bit word (n even, and epi_vec). Rows from `rows` on are left out.
+template <typename T, int C>
+__device__ __forceinline__ void epi_store_quad(const EpiParams& e, int expert, long long row, int rows, int col,
+                                               float (&v)[4 * C]) {
+  float add[4 * C];
+  if (e.residual.p) {
+    const T* q = static_cast<const T*>(e.residual.p) + row * e.residual.ld + col * e.residual.cs;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if (r < rows) {
+        if (C == 2) {
+          const float2 w = unpack2(T(), *reinterpret_cast<const uint32_t*>(q));
+          add[r] = w.x;
+          add[4 * (C - 1) + r] = w.y;
+        } else {
+          add[r] = to_f32<T>(*q);
+        }
+      }
+      q += e.residual.ld;
+    }
+  }
+  if (e.bias) {
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const float b = to_f32<T>(static_cast<const T*>(e.bias)[expert * e.bias_bs + (col + c) * e.bias_s]);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) v[4 * c + r] += b;
+    }
+  }
+  auto put = [&](const EpiMat& m) {
+    T* q = static_cast<T*>(m.p) + row * m.ld + col * m.cs;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      if (r < rows) {
+        if (C == 2) *reinterpret_cast<uint32_t*>(q) = pack2(T(), v[r], v[4 * (C - 1) + r]);
+        else *q = from_f32<T>(v[r]);
+      }
+      q += m.ld;
+    }
+  };
+  if (e.pre.p) put(e.pre);
+  lact_apply(e.act, v);
+  if (e.residual.p) {
+#pragma unroll
+    for (int r = 0; r < 4 * C; ++r) v[r] += (r & 3) < rows ? add[r] : 0.0f;
+  }
+  put(e.out);
+}
 __device__ __forceinline__ bool epi_vec(const EpiParams& e) {
   return e.out.vec && (!e.pre.p || e.pre.vec) && (!e.residual.p || e.residual.vec);
 }

@@ -2,9 +2,12 @@
 //   out[m, n] = epilogue(sum_k x[m, k] w[k, n])
 // with the weights as the tensor core's M operand: a 128-column strip of w is
 // the 128 MMA rows, up to `mt` rows of x are its N. One CTA accumulates
-// D[n, m] of a strip over its slice of K; the CTAs of a cluster split K and
-// add their partial sums over distributed shared memory, in rank order, so the
-// result does not depend on timing.
+// D[n, m] of a strip over its slice of K; the CTAs of a cluster split K. Each
+// owns an equal share of the strip's columns, the others push it their parts of
+// those (st.async: distributed shared-memory stores counted by the owner's
+// barrier), and it adds them in rank order, so the result does not depend on
+// timing. Pulling the parts between two cluster barriers instead took 5 us of
+// the 10 at 16 x 4096 x 4096.
 //
 // Bound: the weights' bytes. Nothing of the tensor core is wasted on absent
 // tokens, and the split over K is what puts every SM on the stream when the
@@ -49,21 +52,19 @@ struct StripParams {
   unsigned long long timeout_ns = 0;
 };
 
-constexpr int strip_smem_bytes(int mt, int stages) { return stages * (LS_W_BYTES + mt * 128) + 256 + 1024; }
-
-__device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
-               : "r"(addr)
-               : "memory");
-  return v;
+// Pushed parts: [slice][four rows][column of this CTA's share] as float4, so
+// that a warp pushes whole 256-byte runs and reads them back conflict-free.
+constexpr int strip_parts_bytes(int mt, int split) { return split > 1 ? LS_COLS * mt * 4 : 0; }
+constexpr int strip_smem_bytes(int mt, int stages, int split) {
+  return stages * (LS_W_BYTES + mt * 128) + 256 + strip_parts_bytes(mt, split) + 1024;
 }
 
-__device__ __forceinline__ float ld_cluster_f1(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
-  return v;
+// Four floats into the shared memory of a CTA of the cluster, their 16 bytes
+// counted on that CTA's barrier.
+__device__ __forceinline__ void st_async_f4(uint32_t addr, uint32_t bar, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%2, %3, %4, %5}, [%1];" ::"r"(addr),
+               "r"(bar), "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
 }
 
 // Expert and first row of unit `unit` when each expert with c tokens has
@@ -103,8 +104,10 @@ __global__ void __launch_bounds__(LS_THREADS, 3)
   uint64_t* full = bars;
   uint64_t* empty = bars + LS_MAX_STAGES;
   uint64_t* acc_full = bars + 2 * LS_MAX_STAGES;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_full + 1);
+  uint64_t* parts_bar = acc_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(parts_bar + 1);
   int* unit_info = reinterpret_cast<int*>(tmem_slot + 1);  // expert, local unit
+  float4* parts = reinterpret_cast<float4*>(reinterpret_cast<uint8_t*>(bars) + 256);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = p.split > 1 ? static_cast<int>(cluster_ctarank()) : 0;
@@ -118,6 +121,7 @@ __global__ void __launch_bounds__(LS_THREADS, 3)
       mbar_init(&empty[s], 1);
     }
     mbar_init(acc_full, 1);
+    mbar_init(parts_bar, 1);
     fence_mbar_init();
   }
   if (warp == 4 && lane == 0) {
@@ -141,6 +145,10 @@ __global__ void __launch_bounds__(LS_THREADS, 3)
         tma_prefetch_l2_3d(&tmW, kb * LS_BK, strip * LS_COLS, 0);
       }
     }
+  }
+  if (p.split > 1) {
+    __syncthreads();
+    cluster_arrive_release();  // this CTA's barriers stand; waited for before the first push
   }
   griddep_wait();
   if (p.experts && warp == 0) {
@@ -209,53 +217,64 @@ __global__ void __launch_bounds__(LS_THREADS, 3)
       }
     }
   } else if (warp == 5) {
-    if (lane == 0 && work) {
+    if (work) {  // the whole warp, one elected lane issuing (linear_pair.cuh says why)
       const uint32_t idesc = idesc_f16(LS_COLS, p.mt, std::is_same<T, __nv_bfloat16>::value, W_MN, false);
       constexpr uint32_t w_lbo = W_MN ? 64u * 128u : 16u, w_step = W_MN ? 2048u : 32u;
+      const uint64_t w_desc0 = smem_desc(smem_u32(ops), w_lbo, 1024u, 2u);
+      const uint64_t x_desc0 = smem_desc(smem_u32(ops) + LS_W_BYTES, 16u, 1024u, 2u);
+      const bool leader = elect_one();
       int stage = 0;
-      uint32_t phase = 0, accumulate = 0;
+      uint32_t phase = 0;
       for (int kb = kb0; kb < kb1; ++kb) {
-        if (!mbar_wait(&full[stage], phase, ctl, kDevTimeoutFull)) break;
+        if (!__all_sync(0xffffffffu, mbar_wait(&full[stage], phase, ctl, kDevTimeoutFull))) break;
         tc_fence_after();
-        const uint32_t sw = smem_u32(ops + stage * stage_bytes);
-        const uint64_t wd = smem_desc(sw, w_lbo, 1024u, 2u), xd = smem_desc(sw + LS_W_BYTES, 16u, 1024u, 2u);
+        const uint64_t so = static_cast<uint64_t>(stage * stage_bytes) >> 4;
+        if (leader) {
 #pragma unroll
-        for (int kk = 0; kk < LS_BK / 16; ++kk) {
-          umma_f16(tmem, wd + ((w_step * kk) >> 4), xd + ((32u * kk) >> 4), idesc, accumulate);
-          accumulate = 1u;
+          for (int kk = 0; kk < LS_BK / 16; ++kk)
+            umma_f16(tmem, w_desc0 + so + ((w_step * kk) >> 4), x_desc0 + so + ((32u * kk) >> 4), idesc,
+                     kk > 0 || kb > kb0 ? 1u : 0u);
+          umma_commit(&empty[stage]);
         }
-        umma_commit(&empty[stage]);
+        __syncwarp();
         if (++stage == p.stages) { stage = 0; phase ^= 1u; }
       }
-      umma_commit(acc_full);  // also after a failed wait: covers whatever was issued
+      if (leader) umma_commit(acc_full);  // also after a failed wait: covers whatever was issued
+      __syncwarp();
       const uint64_t t0 = globaltimer_ns();
       while (!mbar_try_wait(smem_u32(acc_full), 0u))  // no MMA in flight past here
         if (globaltimer_ns() - t0 > p.timeout_ns) { atomicCAS(p.err, 0, kDevTimeoutDrain); break; }
     }
   }
 
-  // The accumulators to shared memory, transposed to red[m][n]: a lane holds
-  // one n, so each store of a warp is 32 neighbouring floats. The operand
-  // stages are free once the MMAs are done.
+  __syncwarp();
+  if (p.split > 1) cluster_wait_acquire();
+
+  // This CTA's share of the strip's columns.
+  const int width = LS_COLS / p.split, col0 = strip * LS_COLS + rank * width;
+  const int slice = p.mt / 4 * width;  // float4 of one slice's parts
+  // One slice: the accumulators go to shared memory transposed, red[m][n] (a
+  // lane holds one n, so each store of a warp is 32 neighbouring floats); the
+  // operand stages are free once the MMAs are done. Several: every lane pushes
+  // its column's rows to the column's owner.
   float* red = reinterpret_cast<float*>(ops);
   const bool vec = epi_vec(p.epi);
   if (warp < 4 && valid > 0) {
+    const int n = static_cast<int>(threadIdx.x);
+    if (p.split > 1 && n == 0) mbar_arrive_expect_tx(parts_bar, LS_COLS * ((valid + 3) / 4) * 16);
     if (p.epi.residual.p) {  // on its way to L2 until the sums are there
       const T* res = static_cast<const T*>(p.epi.residual.p) + row0 * p.epi.residual.ld;
-      if (vec) {
-        const int c = rank * LS_THREADS + static_cast<int>(threadIdx.x), m = c / (LS_COLS / 8);
-        const int col = strip * LS_COLS + (c % (LS_COLS / 8)) * 8;
-        if (m < valid && col < p.n) prefetch_l2(res + m * p.epi.residual.ld + col);
-      } else if ((lane & 15) == 0) {
-        const int col = strip * LS_COLS + static_cast<int>(threadIdx.x);
-        for (int m = rank; col < p.n && m < valid; m += p.split)
-          prefetch_l2(res + m * p.epi.residual.ld + col * p.epi.residual.cs);
-      }
+      for (int m = n; m < valid; m += 128)
+        for (int c = col0; c < min(col0 + width, p.n); c += 64)
+          prefetch_l2(res + m * p.epi.residual.ld + c * p.epi.residual.cs);
     }
     if (work) {
       mbar_wait(acc_full, 0u, ctl, kDevTimeoutAcc);
       tc_fence_after();
     }
+    const int owner = n / width;
+    const uint32_t to = p.split > 1 ? mapa_shared(smem_u32(parts + rank * slice + n - owner * width), owner) : 0u;
+    const uint32_t bar = p.split > 1 ? mapa_shared(smem_u32(parts_bar), owner) : 0u;
     for (int c = 0; c < valid; c += 16) {
       uint32_t r[16];
       if (work) {
@@ -265,84 +284,86 @@ __global__ void __launch_bounds__(LS_THREADS, 3)
 #pragma unroll
         for (int i = 0; i < 16; ++i) r[i] = 0u;
       }
+      if (p.split > 1) {
 #pragma unroll
-      for (int i = 0; i < 16; ++i) red[(c + i) * LS_COLS + warp * 32 + lane] = __uint_as_float(r[i]);
+        for (int i = 0; i < 16; i += 4)
+          if (c + i < valid) st_async_f4(to + (c + i) / 4 * width * 16, bar, r[i], r[i + 1], r[i + 2], r[i + 3]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) red[(c + i) * LS_COLS + n] = __uint_as_float(r[i]);
+      }
     }
   }
   tc_fence_before();
   __syncthreads();
-  if (p.split > 1) cluster_sync_all();
+  // All parts arrive, whatever went wrong elsewhere: nobody leaves before its
+  // own have (their stores must find this CTA's memory).
+  if (p.split > 1 && valid > 0) mbar_wait_acquire_cluster(parts_bar, 0u, ctl, kDevTimeoutReduce);
 
-  const int g0 = rank * LS_THREADS + static_cast<int>(threadIdx.x), gstep = p.split * LS_THREADS;
-  constexpr int per_row = LS_COLS / 8;  // 8-column pieces of a strip's row
-  if (vec) {
-    for (int c = g0; c < valid * per_row; c += gstep) {
-      const int m = c / per_row, lc = (c - m * per_row) * 8;
-      const int col = strip * LS_COLS + lc;
-      if (col >= p.n) continue;
-      float v[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-      const uint32_t at = smem_u32(red + m * LS_COLS + lc);
-      // four slices' parts are on their way before the first is added
-      for (int r0 = 0; r0 < p.split; r0 += 4) {
-        float4 part[4][2];
+  const int tid = static_cast<int>(threadIdx.x);
+  if (p.split > 1) {
+    // four rows of one column a thread (of two, where the outputs take pairs),
+    // slices in order; the loop stays rolled: this runs once, from a cold
+    // instruction cache
+    auto quads = [&](auto columns) {
+      constexpr int C = decltype(columns)::value;
+      const int across = width / C;
+      for (int u = tid; u < (valid + 3) / 4 * across; u += LS_THREADS) {
+        const int q = u / across, lc = (u - q * across) * C, col = col0 + lc;
+        if (col >= p.n) continue;
+        float v[4 * C];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (r0 + r >= p.split) break;
-          const uint32_t a = p.split > 1 ? mapa_shared(at, static_cast<uint32_t>(r0 + r)) : at;
-          part[r][0] = ld_cluster_f4(a);
-          part[r][1] = ld_cluster_f4(a + 16);
-        }
+        for (int i = 0; i < 4 * C; ++i) v[i] = 0.0f;
+        const float4* at = parts + q * width + lc;
+#pragma unroll 2
+        for (int r = 0; r < p.split; ++r) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (r0 + r >= p.split) break;
-          v[0] += part[r][0].x; v[1] += part[r][0].y; v[2] += part[r][0].z; v[3] += part[r][0].w;
-          v[4] += part[r][1].x; v[5] += part[r][1].y; v[6] += part[r][1].z; v[7] += part[r][1].w;
+          for (int c = 0; c < C; ++c) {
+            const float4 x = at[c];
+            v[4 * c] += x.x; v[4 * c + 1] += x.y; v[4 * c + 2] += x.z; v[4 * c + 3] += x.w;
+          }
+          at += slice;
         }
+        epi_store_quad<T, C>(p.epi, expert, row0 + 4 * q, valid - 4 * q, col, v);
       }
+    };
+    if (vec && p.n % 2 == 0) quads(std::integral_constant<int, 2>());
+    else quads(std::integral_constant<int, 1>());
+  } else if (vec) {
+    constexpr int pieces = LS_COLS / 8;  // of eight columns
+    for (int c = tid; c < valid * pieces; c += LS_THREADS) {
+      const int m = c / pieces, lc = (c % pieces) * 8, col = col0 + lc;
+      if (col >= p.n) continue;
+      const float4 x = *reinterpret_cast<const float4*>(red + m * LS_COLS + lc);
+      const float4 y = *reinterpret_cast<const float4*>(red + m * LS_COLS + lc + 4);
+      float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
       float bias[8];
       load_bias8<T>(p.epi, expert, col, bias);
       epi_store8<T>(p.epi, 0, row0 + m, col, v, bias);
     }
   } else {
-    // one element a lane, four rows' residuals in flight; a strip's 128 columns
-    // are a fixed one per thread of four warps
-    constexpr int kAt = 4;
-    const int lc = static_cast<int>(threadIdx.x) & (LS_COLS - 1), col = strip * LS_COLS + lc;
-    const float bias = warp < 4 && p.epi.bias && col < p.n
-                           ? to_f32<T>(static_cast<const T*>(p.epi.bias)[expert * p.epi.bias_bs + col * p.epi.bias_s])
-                           : 0.0f;
-    for (int m0 = rank; warp < 4 && col < p.n && m0 < valid; m0 += kAt * p.split) {
-      float v[kAt], res[kAt];
+    // neighbouring lanes on neighbouring columns, four rows a thread
+    for (int u = tid; u < (valid + 3) / 4 * LS_COLS; u += LS_THREADS) {
+      const int q = u / LS_COLS, lc = u % LS_COLS, col = col0 + lc;
+      if (col >= p.n) continue;
+      float v[4];
 #pragma unroll
-      for (int q = 0; q < kAt; ++q) {
-        const int m = m0 + q * p.split;
-        v[q] = res[q] = 0.0f;
-        if (m >= valid) continue;
-        if (p.epi.residual.p)
-          res[q] = to_f32<T>(static_cast<const T*>(p.epi.residual.p)[(row0 + m) * p.epi.residual.ld + col * p.epi.residual.cs]);
-        const uint32_t at = smem_u32(red + m * LS_COLS + lc);
-        for (int r = 0; r < p.split; ++r)
-          v[q] += ld_cluster_f1(p.split > 1 ? mapa_shared(at, static_cast<uint32_t>(r)) : at);
-      }
-#pragma unroll
-      for (int q = 0; q < kAt; ++q) {
-        const int m = m0 + q * p.split;
-        if (m < valid) epi_store1<T>(p.epi, 0, row0 + m, col, v[q], bias, res[q]);
-      }
+      for (int r = 0; r < 4; ++r) v[r] = red[(4 * q + r) * LS_COLS + lc];
+      epi_store_quad<T, 1>(p.epi, expert, row0 + 4 * q, valid - 4 * q, col, v);
     }
   }
   if (p.experts) {
     // pad rows of the segment, then this unit's share of the rows after the last segment
+    const int pieces = width / 8;
     for (int pass = 0; pass < 2; ++pass) {
       const long long from = pass ? p.offsets[p.experts] + static_cast<long long>(mu) : row0 + valid;
       const long long to = pass ? p.rows : zero_end, step = pass ? p.m_units : 1;
-      for (long long c = g0; from + (c / per_row) * step < to; c += gstep) {
-        const int col = strip * LS_COLS + static_cast<int>(c % per_row) * 8;
-        if (col < p.n) epi_zero8<T>(p.epi, from + (c / per_row) * step, col);
+      for (long long c = tid; from + (c / pieces) * step < to; c += LS_THREADS) {
+        const int col = col0 + static_cast<int>(c % pieces) * 8;
+        if (col < p.n) epi_zero8<T>(p.epi, from + (c / pieces) * step, col);
       }
     }
   }
-  if (p.split > 1) cluster_sync_all();  // peers may still read this CTA's sums
   if (warp == 5) {
     tc_fence_after();
     tmem_dealloc(tmem, p.tmem_cols);

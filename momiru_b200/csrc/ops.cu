@@ -478,7 +478,7 @@ StripShape strip_shape(int sms, int64_t ctas, int k_blocks, int mt) {
   StripShape best;
   double best_cost = 0;
   for (int split = 1; split <= mmr::LS_MAX_SPLIT; split *= 2) {
-    if (k_blocks < split) break;
+    if (k_blocks < split || (split > 1 && mt > 64)) break;
     const double per_cta = double((k_blocks + split - 1) / split) + 0.1 * mt / split + (split > 1 ? 4.0 : 0.0);
     const int64_t deep = (ctas * split + sms - 1) / sms;
     const double cost = double(deep) * per_cta + (deep == 1 ? 8.0 : 0.0);
@@ -487,11 +487,13 @@ StripShape strip_shape(int sms, int64_t ctas, int k_blocks, int mt) {
       best.split = split;
     }
   }
-  // Four CTAs an SM where that leaves three stages each, else two, else one.
-  for (int share : {4, 2, 1}) {
+  if (getenv("SS")) best.split = atoi(getenv("SS"));
+  // Three CTAs an SM (the registers allow no more) where that leaves three stages
+  // each, else two, else one.
+  for (int share : {3, 2, 1}) {
     const int budget = 232448 / share - (share > 1 ? 2048 : 0);
     best.stages = mmr::LS_MAX_STAGES;
-    while (best.stages > 1 && mmr::strip_smem_bytes(mt, best.stages) > budget) --best.stages;
+    while (best.stages > 1 && mmr::strip_smem_bytes(mt, best.stages, best.split) > budget) --best.stages;
     if (best.stages >= 3) break;
   }
   return best;
@@ -553,7 +555,7 @@ int32_t add_product(Handle* h, int dtype, Operand a, Operand b, mmr::EpiParams e
     MMR_TRY(encode16(&ta, a, dtype, p.mt, "lhs"));
     const int64_t grid = int64_t(p.strips) * p.m_units * p.split;
     if (grid > (int64_t(1) << 31) - 1) return fail(MMR_ERR_INVALID_SHAPE, "more than 2^31 units of work");
-    const int smem = mmr::strip_smem_bytes(p.mt, p.stages);
+    const int smem = mmr::strip_smem_bytes(p.mt, p.stages, p.split);
     const bool w_mn = b.mn_major;
     MMR_CUDA(mmr::strip_prepare(bf16, w_mn, smem));
     add_step(h, "mmr_linear_strip_kernel grid %lld, split %lld, rows %lld", [=](cudaStream_t s) {
