@@ -12,7 +12,7 @@ namespace mmr {
 // w_mn: the weights are contiguous along n (row-major k x n).
 cudaError_t strip_launch(bool bf16, bool w_mn, int grid, int smem, cudaStream_t s, const CUtensorMap& tm_w,
                          const CUtensorMap& tm_x, const StripParams& p);
-cudaError_t strip_prepare(bool bf16, bool w_mn, int smem);
+cudaError_t strip_prepare(bool bf16, bool w_mn);
 
 // a_mn / b_mn: the operand is contiguous along m / n. RAG 1 takes a K-major A,
 // RAG 2 both operands MN-major (cudaErrorInvalidValue otherwise).

@@ -17,9 +17,11 @@ cudaError_t strip_launch(bool bf16, bool w_mn, int grid, int smem, cudaStream_t 
                        p);
 }
 
-cudaError_t strip_prepare(bool bf16, bool w_mn, int smem) {
+// The limit belongs to the function, which handles of many sizes share: always
+// all that a block may have.
+cudaError_t strip_prepare(bool bf16, bool w_mn) {
   return cudaFuncSetAttribute(reinterpret_cast<const void*>(strip_kernel(bf16, w_mn)),
-                              cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+                              cudaFuncAttributeMaxDynamicSharedMemorySize, 232448);
 }
 
 }  // namespace mmr

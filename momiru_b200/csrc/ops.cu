@@ -455,48 +455,68 @@ struct Groups {  // ragged rows or contraction
   int64_t rows = 0, assignments = 0;
 };
 
-// Up to this many rows the weights' stream bounds the product and the strip
-// kernel takes it; above, the CTA pairs. N = K = 4096: 16.4 us against 21.3 at
-// 64 rows, 24.1 against 21.6 at 128.
-constexpr int64_t kStripRows = 64;
-constexpr int64_t kStripRowsPerExpert = 96;
-
-// How the strip kernel divides `ctas` strips of k_blocks: K slices of a strip
-// and stages of a CTA. The time follows the SM with the most work, CTAs being
-// dealt evenly, ceil(CTAs / SMs) to an SM; in units of a k-block's time (0.28
-// us) a CTA costs its k-blocks, a tenth for every row of its share of the
-// epilogue, and 4 for the join where there are slices; one CTA an SM costs 8
-// more, as nothing hides its start and end. 64 rows through 28 experts of
-// 2048 x 1024 took 18.4 / 22.8 / 33.5 us in 1 / 2 / 4 slices, one row through
-// 4096 x 11008 22.8 / 19.3 in 4 / 8. Narrower strips, which could
-// be dealt more evenly, only lost (27.9 us at 56 columns): an MMA costs its
-// ~100 cycles however few rows of it are used.
+// ---- which kernel, and how the strip kernel divides its work: the least of the
+// times estimated (us) for `mats` weight matrices of n columns and k_blocks, each
+// met by `rows` rows (expert products: the mean). Both estimates were fitted to
+// products of 1 to 1024 rows with N and K of 512 to 11008 and are within about
+// 2 us of what was measured there.
+//
+// Strip: 5.5 for launch, first bytes and last store; then the longer of the
+// weights' way from memory and the k-blocks of the SM with the most CTAs (its
+// MMAs bound one at 0.235 up to 64 rows and 0.21 at 128, where another CTA hides
+// its latencies; alone 0.25 and 0.33); 3 for every further wave of CTAs; the join
+// of K slices and the epilogue by rows. A narrower strip than 128 columns only lost:
+// an MMA costs its ~100 cycles however few rows of it are used.
+//
+// Pairs: 6.5, and the longer of the weights' way (at three quarters of memory's
+// rate) and the rounds: per k-block 0.3 for every full round of tiles, 0.34 for a
+// partial one, 0.234 where that is cut into half tiles.
+//
+// 128 x 4096 x 4096 takes 13.1 us as 128-row strips in 4 slices, 16.4 in 2 and
+// 21.6 on pairs; 128 x 11008 x 4096 32 us on strips, 28.5 on pairs; 1024 rows
+// over 32 experts of 2048 x 1024 29.5 us on strips, 39.3 on pairs.
 struct StripShape {
-  int split = 1, stages = 3;
+  int mt = 16, split = 1, stages = 3;
+  double us = 0;
 };
-StripShape strip_shape(int sms, int64_t ctas, int k_blocks, int mt) {
+
+StripShape strip_shape(int sms, int64_t mats, double rows, bool ragged, int64_t n, int k_blocks) {
   StripShape best;
-  double best_cost = 0;
-  for (int split = 1; split <= mmr::LS_MAX_SPLIT; split *= 2) {
-    if (k_blocks < split || (split > 1 && mt > 64)) break;
-    const double per_cta = double((k_blocks + split - 1) / split) + 0.1 * mt / split + (split > 1 ? 4.0 : 0.0);
-    const int64_t deep = (ctas * split + sms - 1) / sms;
-    const double cost = double(deep) * per_cta + (deep == 1 ? 8.0 : 0.0);
-    if (best_cost == 0 || cost < best_cost) {
-      best_cost = cost;
-      best.split = split;
+  const int64_t strips = (n + mmr::LS_COLS - 1) / mmr::LS_COLS;
+  for (int mt = 16; mt <= 128; mt *= 2) {
+    const int64_t units = mats * (ragged ? int64_t(rows / mt) + 1 : (int64_t(rows) + mt - 1) / mt) * strips;
+    for (int split = 1; split <= mmr::LS_MAX_SPLIT && split <= std::max(k_blocks, 1); split *= 2) {
+      // three CTAs an SM (the registers allow no more) where each has three stages
+      int share = 3, stages = 0;
+      for (;; --share) {
+        const int budget = 232448 / share - (share > 1 ? 2048 : 0);
+        stages = mmr::LS_MAX_STAGES;
+        while (stages > 1 && mmr::strip_smem_bytes(mt, stages, split) > budget) --stages;
+        if (stages >= 3 || share == 1) break;
+      }
+      const int64_t ctas = units * split;
+      // clusters of one CTA an SM do not fill the GPU, whose parts have no whole
+      // number of clusters of SMs: what does not fit runs as a second wave
+      if (share == 1 && ctas > sms * (split == 8 ? 11 : split == 4 ? 14 : split == 2 ? 15 : 16) / 16 && split > 1) continue;
+      const int64_t deep = (ctas + sms - 1) / sms, waves = (ctas + sms * share - 1) / (sms * share);
+      const int64_t blocks = (k_blocks + split - 1) / split;
+      const double stream = double(deep * blocks) * (mt <= 64 ? (deep > 1 ? 0.235 : 0.25) : deep > 1 ? 0.21 : 0.33);
+      const double memory = double(mats) * double(n) * k_blocks * 128 / 6.4e6;
+      const double us = 5.5 + std::max(stream, memory) + 3.0 * double(waves - 1) +
+                        (split > 1 ? 0.5 + 0.012 * mt : 0.02 * mt);
+      if (best.us == 0 || us < best.us - 0.05) best = {mt, split, stages, us};
     }
-  }
-  if (getenv("SS")) best.split = atoi(getenv("SS"));
-  // Three CTAs an SM (the registers allow no more) where that leaves three stages
-  // each, else two, else one.
-  for (int share : {3, 2, 1}) {
-    const int budget = 232448 / share - (share > 1 ? 2048 : 0);
-    best.stages = mmr::LS_MAX_STAGES;
-    while (best.stages > 1 && mmr::strip_smem_bytes(mt, best.stages, best.split) > budget) --best.stages;
-    if (best.stages >= 3) break;
+    if (!ragged && mt >= rows) break;
   }
   return best;
+}
+
+double pair_us(int sms, int64_t mats, double rows, bool ragged, int64_t n, int k_blocks) {
+  const int64_t pairs = sms / 2;
+  const int64_t tiles = mats * (ragged ? int64_t(rows / 256) + 1 : (int64_t(rows) + 255) / 256) * ((n + 255) / 256);
+  const int64_t rem = tiles % pairs;
+  const double rounds = k_blocks * (0.3 * double(tiles / pairs) + (rem == 0 ? 0.0 : 2 * rem <= pairs ? 0.234 : 0.34));
+  return 6.5 + std::max(rounds, double(mats) * double(n) * k_blocks * 128 / 4.9e6);
 }
 
 int round16(int64_t v) { return int((v + 15) / 16 * 16); }
@@ -513,8 +533,10 @@ int32_t add_product(Handle* h, int dtype, Operand a, Operand b, mmr::EpiParams e
   epi.n = int(n);
   if (m == 0 || n == 0) return MMR_OK;
   const int k_blocks = int((k + 63) / 64);
-  const int64_t per_expert = g ? (g->assignments + g->experts - 1) / g->experts : 0;
-  const bool strip = g ? per_expert <= kStripRowsPerExpert : m <= kStripRows;
+  const int64_t mats = g ? std::min<int64_t>(g->experts, g->assignments) : 1;
+  const double rows = g ? double(g->assignments) / double(mats) : double(m);
+  const StripShape shape = strip_shape(h->sms, mats, rows, g != nullptr, n, k_blocks);
+  const bool strip = rows <= 1024 && shape.us < pair_us(h->sms, mats, rows, g != nullptr, n, k_blocks);
   mmr::PackList packs;
   MMR_TRY(admit(h, &a, strip || g ? 1 : 0, "lhs", &packs));
   MMR_TRY(admit(h, &b, 0, "rhs", &packs));
@@ -529,10 +551,7 @@ int32_t add_product(Handle* h, int dtype, Operand a, Operand b, mmr::EpiParams e
     p.m = int(m);
     p.n = int(n);
     p.k_blocks = k_blocks;
-    p.mt = 16;
-    const int64_t cover = g ? 2 * per_expert : m;
-    while (p.mt < 256 && p.mt < cover) p.mt *= 2;
-    if (!g) p.mt = std::min(p.mt, round16(m));
+    p.mt = g ? shape.mt : std::min(shape.mt, round16(m));
     p.strips = int((n + mmr::LS_COLS - 1) / mmr::LS_COLS);
     p.m_units = g ? int(std::min<int64_t>(g->experts, g->assignments) + g->assignments / p.mt)
                   : int((m + p.mt - 1) / p.mt);
@@ -542,8 +561,6 @@ int32_t add_product(Handle* h, int dtype, Operand a, Operand b, mmr::EpiParams e
       p.counts = g->counts;
       p.rows = g->rows;
     }
-    const int64_t units = g ? std::min<int64_t>(g->experts, g->assignments) : p.m_units;
-    const StripShape shape = strip_shape(h->sms, units * p.strips, k_blocks, p.mt);
     p.split = shape.split;
     p.stages = shape.stages;
     p.tmem_cols = 32;
@@ -557,7 +574,7 @@ int32_t add_product(Handle* h, int dtype, Operand a, Operand b, mmr::EpiParams e
     if (grid > (int64_t(1) << 31) - 1) return fail(MMR_ERR_INVALID_SHAPE, "more than 2^31 units of work");
     const int smem = mmr::strip_smem_bytes(p.mt, p.stages, p.split);
     const bool w_mn = b.mn_major;
-    MMR_CUDA(mmr::strip_prepare(bf16, w_mn, smem));
+    MMR_CUDA(mmr::strip_prepare(bf16, w_mn));
     add_step(h, "mmr_linear_strip_kernel grid %lld, split %lld, rows %lld", [=](cudaStream_t s) {
       return mmr::strip_launch(bf16, w_mn, int(grid), smem, s, tb, ta, p);
     }, grid, p.split, p.mt);
@@ -1112,8 +1129,9 @@ int32_t dispatch_bind(const mmr_dispatch_desc* d, Handle** out) {
   const int smem = mmr::dispatch_smem_bytes(p.experts);
   auto kernel = vb == 16 ? mmr::mmr_dispatch_kernel<16> : vb == 8 ? mmr::mmr_dispatch_kernel<8>
                 : vb == 4 ? mmr::mmr_dispatch_kernel<4> : mmr::mmr_dispatch_kernel<2>;
-  if (smem > 48 * 1024)
-    MMR_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+  if (smem > 48 * 1024)  // the function's limit, shared by handles of every size
+    MMR_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  mmr::dispatch_smem_bytes(mmr::ES_MAX_EXPERTS)));
   add_step(h.get(), "mmr_dispatch_kernel grid %lld, %lld-byte vectors", [=](cudaStream_t s) {
     return mmr::launch_kernel(kernel, dim3(grid), dim3(mmr::ES_THREADS), smem, s, dim3(1, 1, 1), p);
   }, grid, vb);

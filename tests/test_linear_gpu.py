@@ -201,6 +201,27 @@ def test_activations_at_infinity():
         assert col[3] == (high or 60000.0) and col[4] == 0 and col[5] == 0
 
 
+def test_handles_of_many_sizes_live_together():
+    """Products of different shapes, all bound before the first runs, in both orders."""
+    t, u = TYPES["bf16"]
+    g = gen(13)
+    made = []
+    for m, n, k in [(128, 1024, 512), (1, 512, 512), (40, 2048, 256), (300, 512, 64), (16, 128, 4096)]:
+        lhs, rhs = rand(g, m, k, dtype=t), rand(g, k, n, dtype=t, scale=k ** -0.5)
+        out = torch.zeros(m, n, dtype=t, device="cuda")
+        made.append((mb.BoundLinear(mb.LinearNode(), V(lhs), V(rhs), V(out)), lhs, rhs, out))
+    for order in (made, made[::-1]):
+        for op, lhs, rhs, out in order:
+            out.zero_()
+            torch.cuda.synchronize()
+            op.replay()
+        for op, lhs, rhs, out in order:
+            op.quiesce_or_abort(20)
+            check_forward(t, u, lhs, rhs, None, None, ACT.NONE, out, None)
+    for op, *_ in made:
+        op.close()
+
+
 def test_offsets_past_32_bits():
     """Rows whose element offsets pass 2^31: output, residual and lhs by row pitch."""
     t, u = TYPES["bf16"]
