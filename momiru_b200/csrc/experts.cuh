@@ -63,6 +63,11 @@ __device__ __forceinline__ int es_id(const DispatchParams& p, int i) {
   return id >= 0 && id < p.experts ? id : -1;
 }
 
+// First token of CTA b's run.
+__device__ __forceinline__ int run_start(const DispatchParams& p, long long b) {
+  return static_cast<int>(min(b * p.run, static_cast<long long>(p.tokens)));
+}
+
 // One histogram of expert ids per CTA's run.
 static __global__ void __launch_bounds__(ES_THREADS) mmr_expert_hist_kernel(const DispatchParams p) {
   extern __shared__ int hist[];
@@ -70,8 +75,7 @@ static __global__ void __launch_bounds__(ES_THREADS) mmr_expert_hist_kernel(cons
   griddep_wait();
   griddep_release();
   __syncthreads();
-  const int i0 = static_cast<int>(blockIdx.x) * p.run * p.top_k;
-  const int i1 = min(i0 + p.run * p.top_k, p.tokens * p.top_k);
+  const int i0 = run_start(p, blockIdx.x) * p.top_k, i1 = run_start(p, blockIdx.x + 1ll) * p.top_k;
   for (int i = i0 + static_cast<int>(threadIdx.x); i < i1; i += ES_THREADS) {
     const int id = es_id(p, i);
     if (id >= 0) atomicAdd(&hist[id], 1);
@@ -100,8 +104,9 @@ __global__ void __launch_bounds__(ES_THREADS) mmr_dispatch_kernel(const Dispatch
   griddep_wait();
   griddep_release();
   __syncthreads();
-  const int n = p.tokens * p.top_k, span = p.run * p.top_k;
-  const int i0 = static_cast<int>(blockIdx.x) * span, i1 = min(i0 + span, n);
+  const int n = p.tokens * p.top_k;
+  const int t0 = run_start(p, blockIdx.x), t1 = run_start(p, blockIdx.x + 1ll);
+  const int i0 = t0 * p.top_k, i1 = t1 * p.top_k;
   if (p.hist) {
     // columns of the histograms, the CTAs' rows dealt to `groups` of threads
     const int groups = max(1, ES_THREADS / E);
@@ -112,7 +117,7 @@ __global__ void __launch_bounds__(ES_THREADS) mmr_dispatch_kernel(const Dispatch
       int all = 0, pre = 0;
 #pragma unroll 8
       for (int b = b0; b < b1; ++b) {
-        const int c = __ldg(p.hist + static_cast<long long>(b) * E + e);
+        const int c = *(p.hist + static_cast<long long>(b) * E + e);
         all += c;
         pre += b < static_cast<int>(blockIdx.x) ? c : 0;
       }
@@ -215,7 +220,6 @@ __global__ void __launch_bounds__(ES_THREADS) mmr_dispatch_kernel(const Dispatch
   }
   // The rows of this run's tokens, in pieces of 32 vectors: four pieces' loads in
   // flight in a warp where there are enough of them.
-  const int t0 = static_cast<int>(blockIdx.x) * p.run, t1 = min(t0 + p.run, p.tokens);
   const int pieces = (p.row_vecs + 31) / 32;
   const bool many = (t1 - t0) * pieces >= 4 * ES_WARPS;
   const int group = many ? 4 : 1, groups = (pieces + group - 1) / group;
@@ -225,7 +229,7 @@ __global__ void __launch_bounds__(ES_THREADS) mmr_dispatch_kernel(const Dispatch
     Vec v[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-      if (q < group && c + 32 * q < p.row_vecs) v[q] = __ldg(src + c + 32 * q);
+      if (q < group && c + 32 * q < p.row_vecs) v[q] = *(src + c + 32 * q);
     for (int j0 = 0; j0 < p.top_k; j0 += 4) {
       int slot[4];
 #pragma unroll
@@ -246,6 +250,7 @@ __global__ void __launch_bounds__(ES_THREADS) mmr_dispatch_kernel(const Dispatch
 struct CombineParams {
   const int* slots = nullptr;
   int tokens = 0, top_k = 0;
+  int n_rows = 0;  // a slot outside [0, n_rows) counts as dropped
   const float* weights = nullptr;  // null: all one
   long long w_t = 0, w_j = 0;
   RowMat rows, residual, out;  // residual.p may be null
@@ -294,8 +299,9 @@ __global__ void __launch_bounds__(128) mmr_combine_kernel(const CombineParams p)
       int my_slot = -1;
       float my_scale = 1.0f;
       if (lane < many) {
-        my_slot = __ldg(p.slots + static_cast<long long>(t) * p.top_k + jb + lane);
-        if (p.weights && my_slot >= 0) my_scale = __ldg(p.weights + t * p.w_t + (jb + lane) * p.w_j);
+        my_slot = p.slots[static_cast<long long>(t) * p.top_k + jb + lane];
+        if (my_slot >= p.n_rows) my_slot = -1;
+        if (p.weights && my_slot >= 0) my_scale = *(p.weights + t * p.w_t + (jb + lane) * p.w_j);
       }
       for (int j0 = 0; j0 < many; j0 += kChoices) {
         Vec w[kChoices];
@@ -307,7 +313,7 @@ __global__ void __launch_bounds__(128) mmr_combine_kernel(const CombineParams p)
           scale[q] = __shfl_sync(0xffffffffu, my_scale, (j0 + q) & 31);
           if (j0 + q >= many || c >= p.row_vecs) slot[q] = -1;
           if (slot[q] >= 0)
-            w[q] = __ldg(reinterpret_cast<const Vec*>(static_cast<const char*>(p.rows.p) + slot[q] * p.rows.ld) + c);
+            w[q] = *(reinterpret_cast<const Vec*>(static_cast<const char*>(p.rows.p) + slot[q] * p.rows.ld) + c);
         }
 #pragma unroll
         for (int q = 0; q < kChoices; ++q) {
@@ -382,6 +388,7 @@ __global__ void __launch_bounds__(256) mmr_combine_grad_kernel(const CombineGrad
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       slot[q] = j0 + q < p.top_k ? p.slots[static_cast<long long>(t) * p.top_k + j0 + q] : -1;
+      if (slot[q] >= p.n_rows) slot[q] = -1;
       scale[q] = slot[q] >= 0 ? (p.weights ? p.weights[t * p.w_t + (j0 + q) * p.w_j] : 1.0f) : 0.0f;
       dot[q] = 0.0f;
     }
@@ -391,11 +398,11 @@ __global__ void __launch_bounds__(256) mmr_combine_grad_kernel(const CombineGrad
       for (int x = 0; x < U; ++x) {
         const int c = c0 + x * 32 * W;
         if (c >= p.row_vecs) continue;
-        dv[x] = __ldg(d_out + c);
+        dv[x] = *(d_out + c);
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           if (slot[q] >= 0 && p.d_weights)
-            w[x][q] = __ldg(reinterpret_cast<const Vec*>(static_cast<const char*>(p.rows.p) + slot[q] * p.rows.ld) + c);
+            w[x][q] = *(reinterpret_cast<const Vec*>(static_cast<const char*>(p.rows.p) + slot[q] * p.rows.ld) + c);
       }
 #pragma unroll
       for (int x = 0; x < U; ++x) {

@@ -175,7 +175,7 @@ __device__ __forceinline__ void load_bias8(const EpiParams& e, int batch, int co
   if (!e.bias) return;
   const T* q = static_cast<const T*>(e.bias) + batch * e.bias_bs + col * e.bias_s;
   if (e.bias_s == 1 && col + 8 <= e.n && (reinterpret_cast<uintptr_t>(q) & 15) == 0) {
-    add8<T>(b, __ldg(reinterpret_cast<const uint4*>(q)));
+    add8<T>(b, *(reinterpret_cast<const uint4*>(q)));
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i)

@@ -190,7 +190,12 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
     int base = 0;
     for (int e0 = 0; e0 < p.experts; e0 += 32) {
       const int e = e0 + lane;
-      const int c = e < p.experts ? p.counts[e] : 0;
+      // (the layout is data: whatever it says, nothing outside the rows is touched)
+      int c = 0, o = 0;
+      if (e < p.experts) {
+        o = static_cast<int>(min(static_cast<long long>(max(p.offsets[e], 0)), p.rows));
+        c = static_cast<int>(min(static_cast<long long>(max(p.counts[e], 0)), p.rows - o));
+      }
       int incl = ((c + 255) >> 8) * p.tiles_n;
       const int own = incl;
 #pragma unroll
@@ -200,14 +205,14 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
       }
       if (e < p.experts) {
         first[e] = base + incl - own;
-        off[e] = p.offsets[e];
+        off[e] = o;
         cnt[e] = c;
       }
       base += __shfl_sync(0xffffffffu, incl, 31);
     }
     if (lane == 0) {
       first[p.experts] = base;
-      off[p.experts] = p.offsets[p.experts];
+      off[p.experts] = static_cast<int>(min(static_cast<long long>(max(p.offsets[p.experts], 0)), p.rows));
     }
   }
   tc_fence_before();
@@ -236,7 +241,7 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
     auto load_bias16 = [&](const LpTile& w, int col0) {
       const int col = col0 + (lane & 3) * 8;
       const T* q = static_cast<const T*>(p.epi.bias) + w.batch * p.epi.bias_bs + col;
-      return vec_bias && col < p.n ? __ldg(reinterpret_cast<const uint4*>(q)) : make_uint4(0, 0, 0, 0);
+      return vec_bias && col < p.n ? *(reinterpret_cast<const uint4*>(q)) : make_uint4(0, 0, 0, 0);
     };
     // The residual of one 32 x 32 box, in the layout it is added in: vector `it`
     // of lane l is row 8 it + l / 4, columns 8 (l % 4) of the box.

@@ -73,7 +73,7 @@ __device__ __forceinline__ bool find_expert_unit(const int* counts, int experts,
                                                  int* local) {
   int base = 0;
   for (int e0 = 0; e0 < experts; e0 += 32) {
-    const int c = e0 + lane < experts ? counts[e0 + lane] : 0;
+    const int c = e0 + lane < experts ? max(counts[e0 + lane], 0) : 0;
     const int units = (c + mt - 1) / mt;
     int incl = units;
 #pragma unroll
@@ -173,10 +173,11 @@ __global__ void __launch_bounds__(LS_THREADS, 3)
     expert = unit_info[0];
     valid = 0;
     if (expert >= 0) {
+      // (the layout is data: whatever it says, nothing outside the rows is touched)
       const int local = unit_info[1], count = p.counts[expert];
-      row0 = p.offsets[expert] + static_cast<long long>(local) * p.mt;
-      valid = min(p.mt, count - local * p.mt);
-      if ((local + 1) * p.mt >= count) zero_end = p.offsets[expert + 1];
+      row0 = max(p.offsets[expert], 0) + static_cast<long long>(local) * p.mt;
+      valid = static_cast<int>(max(0ll, min(static_cast<long long>(min(p.mt, count - local * p.mt)), p.rows - row0)));
+      if ((local + 1) * p.mt >= count) zero_end = min(static_cast<long long>(p.offsets[expert + 1]), p.rows);
     }
   }
   const int kb0 = static_cast<int>(static_cast<long long>(p.k_blocks) * rank / p.split);
@@ -356,7 +357,7 @@ __global__ void __launch_bounds__(LS_THREADS, 3)
     // pad rows of the segment, then this unit's share of the rows after the last segment
     const int pieces = width / 8;
     for (int pass = 0; pass < 2; ++pass) {
-      const long long from = pass ? p.offsets[p.experts] + static_cast<long long>(mu) : row0 + valid;
+      const long long from = pass ? max(p.offsets[p.experts], 0) + static_cast<long long>(mu) : row0 + valid;
       const long long to = pass ? p.rows : zero_end, step = pass ? p.m_units : 1;
       for (long long c = tid; from + (c / pieces) * step < to; c += LS_THREADS) {
         const int col = col0 + static_cast<int>(c % pieces) * 8;

@@ -1343,6 +1343,9 @@ void gemm_set_chunk(mmr_gemm_handle* h, int k) {
   if (h->family == MMR_FAMILY_TCGEN05 && h->mode == 1)
     h->tcp.chunk_kb = std::max(1, std::min(k / int(h->launch.bk), h->tcp.k_blocks));
 }
+// A product that another handle runs: that one's event covers it (its own may
+// belong to a captured graph), so only its error word is left to read.
+void gemm_forget_run(mmr_gemm_handle* h) { h->ran = false; }
 }  // namespace mmr
 
 extern "C" {
@@ -1366,17 +1369,8 @@ static int32_t poll_event(cudaEvent_t ev, uint64_t timeout_ns) {
   }
 }
 
-int32_t mmr_gemm_quiesce(mmr_gemm_handle* h, uint64_t timeout_ns) {
-  if (!h) return fail(MMR_ERR_INVALID_ARGUMENT, "null handle");
-  if (!h->ran) return MMR_OK;
-  DeviceGuard guard(h->device);
-  int32_t rc = poll_event(h->done, timeout_ns);
-  if (rc) return rc;
-  if (h->host) {  // every copy has landed; now each panel GEMM's error word
-    for (mmr_gemm_handle* sub : h->panel)
-      if ((rc = mmr_gemm_quiesce(sub, timeout_ns))) return rc;
-    return MMR_OK;
-  }
+static int32_t read_error_word(mmr_gemm_handle* h, uint64_t timeout_ns) {
+  int32_t rc = MMR_OK;
   // Read the device error word (asynchronously, then poll: never block forever).
   MMR_CUDA_TRY(cudaMemcpyAsync(h->h_err, h->d_err, sizeof(int), cudaMemcpyDeviceToHost, h->stream));
   MMR_CUDA_TRY(cudaEventRecord(h->err_ev, h->stream));
@@ -1394,6 +1388,20 @@ int32_t mmr_gemm_quiesce(mmr_gemm_handle* h, uint64_t timeout_ns) {
                 "kernel reported device error word %d (a bounded wait expired)", code);
   }
   return MMR_OK;
+}
+
+int32_t mmr_gemm_quiesce(mmr_gemm_handle* h, uint64_t timeout_ns) {
+  if (!h) return fail(MMR_ERR_INVALID_ARGUMENT, "null handle");
+  if (!h->ran) return MMR_OK;
+  DeviceGuard guard(h->device);
+  int32_t rc = poll_event(h->done, timeout_ns);
+  if (rc) return rc;
+  if (h->host) {  // every copy has landed; now each panel GEMM's error word
+    for (mmr_gemm_handle* sub : h->panel)
+      if ((rc = mmr_gemm_quiesce(sub, timeout_ns))) return rc;
+    return MMR_OK;
+  }
+  return read_error_word(h, timeout_ns);
 }
 
 int32_t mmr_gemm_destroy(mmr_gemm_handle* h) {
@@ -1428,6 +1436,14 @@ int32_t mmr_gemm_destroy(mmr_gemm_handle* h) {
   delete h;
   return rc;
 }
+
+}  // extern "C"
+
+namespace mmr {
+int32_t gemm_read_error(mmr_gemm_handle* h, uint64_t timeout_ns) { return read_error_word(h, timeout_ns); }
+}  // namespace mmr
+
+extern "C" {
 
 namespace {
 __global__ void mmr_bounded_wait_probe_kernel(int* err, unsigned long long limit_ns) {

@@ -30,6 +30,8 @@ namespace mmr {
 // momiru_gemm.cu
 int32_t set_last_error(int32_t code, const char* message);
 void gemm_set_chunk(mmr_gemm_handle* h, int k);
+void gemm_forget_run(mmr_gemm_handle* h);
+int32_t gemm_read_error(mmr_gemm_handle* h, uint64_t timeout_ns);
 }
 
 struct mmr_op_handle {
@@ -47,7 +49,7 @@ struct mmr_op_handle {
   int* d_err = nullptr;                    // device error word (256 bytes)
   int* h_err = nullptr;                    // pinned copy
   cudaEvent_t done = nullptr, err_ev = nullptr;
-  bool ran = false;      // `done` was recorded (a run outside stream capture)
+  bool ran = false;       // `done` was recorded (a run outside stream capture)
   bool launched = false;
 };
 
@@ -798,7 +800,11 @@ int32_t add_f32_product(Handle* h, int math, const mmr_view& lhs, const mmr_view
   h->products.push_back(g);
   mmr::gemm_set_chunk(g, kF32Chunk);
   h->plan += "matmul node (f32)\n";
-  h->steps.push_back({"matmul node (f32)", [g](cudaStream_t s) { return mmr_gemm_run_on(g, s); }});
+  h->steps.push_back({"matmul node (f32)", [g](cudaStream_t s) {
+                        const int32_t rc = mmr_gemm_run_on(g, s);
+                        mmr::gemm_forget_run(g);
+                        return rc;
+                      }});
   return MMR_OK;
 }
 
@@ -1182,6 +1188,7 @@ int32_t combine_bind(const mmr_combine_desc* d, Handle** out) {
     p.slots = l.p(l.slots);
     p.tokens = int(l.tokens);
     p.top_k = int(l.top_k);
+    p.n_rows = int(l.rows);
     p.weights = reinterpret_cast<const float*>(w.on ? w.base : 0);
     p.w_t = w.s[1];
     p.w_j = w.s[2];
@@ -1411,7 +1418,7 @@ int32_t quiesce(Handle* h, uint64_t timeout_ns) {
   if (!h->launched) return MMR_OK;
   DeviceGuard guard(h->device);
   if (h->ran) MMR_TRY(poll_event(h->done, timeout_ns));
-  for (mmr_gemm_handle* g : h->products) MMR_TRY(mmr_gemm_quiesce(g, timeout_ns));
+  for (mmr_gemm_handle* g : h->products) MMR_TRY(mmr::gemm_read_error(g, timeout_ns));
   MMR_CUDA(cudaMemcpyAsync(h->h_err, h->d_err, sizeof(int), cudaMemcpyDeviceToHost, h->stream));
   MMR_CUDA(cudaEventRecord(h->err_ev, h->stream));
   MMR_TRY(poll_event(h->err_ev, timeout_ns));

@@ -31,10 +31,10 @@ __device__ __forceinline__ uint4 pack_load8(const unsigned short* src) {
   uint4 v;
   if ((reinterpret_cast<uintptr_t>(src) & 2) == 0) {
     const unsigned int* w = reinterpret_cast<const unsigned int*>(src);
-    v = make_uint4(__ldg(w), __ldg(w + 1), __ldg(w + 2), __ldg(w + 3));
+    v = make_uint4(*(w), *(w + 1), *(w + 2), *(w + 3));
   } else {
     const unsigned int* w = reinterpret_cast<const unsigned int*>(src - 1);
-    const unsigned int a = __ldg(w), b = __ldg(w + 1), c = __ldg(w + 2), d = __ldg(w + 3), e = __ldg(w + 4);
+    const unsigned int a = *(w), b = *(w + 1), c = *(w + 2), d = *(w + 3), e = *(w + 4);
     v = make_uint4(__funnelshift_r(a, b, 16), __funnelshift_r(b, c, 16), __funnelshift_r(c, d, 16),
                    __funnelshift_r(d, e, 16));
   }
@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) mmr_act_grad_kern
   auto load = [&](const T* q, const EpiMat& m, Raw& r) {
     if (VEC) {
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) r.w[i] = __ldg(reinterpret_cast<const uint4*>(q + tx * 8) + i);
+      for (int i = 0; i < kVec; ++i) r.w[i] = *(reinterpret_cast<const uint4*>(q + tx * 8) + i);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) r.t[i] = c0 + col(i) < p.n ? q[col(i) * m.cs] : from_f32<T>(0.0f);
@@ -258,7 +258,8 @@ __global__ void __launch_bounds__(256) mmr_col_sum_kernel(const ColSumParams p) 
   griddep_release();
   const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
   const int c = static_cast<int>(blockIdx.x) * 32 + tx, e = static_cast<int>(blockIdx.y);
-  const int c0 = p.offsets ? p.offsets[e] / AG_ROWS : 0, c1 = p.offsets ? p.offsets[e + 1] / AG_ROWS : p.chunks;
+  const int c0 = p.offsets ? max(p.offsets[e], 0) / AG_ROWS : 0;
+  const int c1 = p.offsets ? min(p.offsets[e + 1] / AG_ROWS, p.chunks) : p.chunks;
   float s = 0.0f;
   if (c < p.n) {
 #pragma unroll 4

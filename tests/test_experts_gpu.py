@@ -265,6 +265,35 @@ def test_equal_runs_give_equal_bits():
         assert all(torch.equal(a, b) for a, b in zip(o, outs[0]))
 
 
+def test_a_layout_of_nonsense_touches_nothing_outside():
+    """Counts, offsets and slots that no sort made (out of range either way):
+    every access is bounded by the buffers, whose guard rows keep their values."""
+    tokens, k, n, experts = 64, 64, 136, 4
+    t = torch.bfloat16
+    g = gen(15)
+    rows_n = mb.ExpertLayout.capacity(tokens, 2, experts, 64)
+    bad = torch.tensor([2 ** 30, -5, rows_n + 7, 10 ** 9], dtype=torch.int32, device="cuda")
+    offsets = torch.tensor([rows_n - 3, -64, 10 ** 9, 64, 2 ** 30], dtype=torch.int32, device="cuda")
+    slots = torch.full((tokens, 2), 10 ** 9, dtype=torch.int32, device="cuda")
+    slots[::2] = rows_n
+    sources = torch.full((rows_n,), -1, dtype=torch.int32, device="cuda")
+    lay = mb.ExpertLayout(tokens, 2, experts, 64, V(slots), V(sources), V(offsets), V(bad))
+    rows = rand(g, rows_n, k, dtype=t)
+    for experts_rows in (1, 2):  # twice: nothing is left behind either
+        w = rand(g, experts, k, n, dtype=t)
+        buf = torch.full((rows_n + 512, n), 7.0, dtype=t, device="cuda")
+        replay(mb.BoundExpertLinear(mb.LinearNode(), lay, V(rows), V(w), V(buf[256:256 + rows_n])))
+        assert bool((buf[:256] == 7).all()) and bool((buf[256 + rows_n:] == 7).all())
+        d_w, d_b = torch.empty_like(w), torch.empty(experts, n, dtype=t, device="cuda")
+        replay(mb.BoundExpertLinearGrad(mb.LinearNode(), lay, V(buf[256:256 + rows_n]), V(rows), V(w), d_weights=V(d_w), d_bias=V(d_b)))
+    y = torch.ones(tokens, k, dtype=t, device="cuda")
+    replay(mb.BoundCombine(lay, V(rows), V(y)))
+    assert not y.any()
+    d_rows, d_wt = torch.ones_like(rows), torch.ones(tokens, 2, device="cuda")
+    replay(mb.BoundCombineGrad(lay, V(rand(g, tokens, k, dtype=t)), V(rows), None, d_rows=V(d_rows), d_weights=V(d_wt)))
+    assert not d_rows.any() and not d_wt.any()
+
+
 def test_layout_changes_between_replays():
     """One bound chain, other ids on every replay: nothing of the previous routing stays."""
     tokens, k, n, experts = 50, 72, 136, 6

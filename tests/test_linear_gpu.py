@@ -367,6 +367,28 @@ def test_f32_operands(m, n, k, act):
     assert rel(x, want + r.double()) <= 1e-5
 
 
+def test_f32_capture():
+    """A captured f32 run, replayed after others; waiting and closing work as before it."""
+    g = gen(14)
+    lhs, rhs, r = rand(g, 300, 256), rand(g, 256, 264, scale=0.06), rand(g, 300, 264)
+    out = torch.zeros(300, 264, device="cuda")
+    op = mb.BoundLinear(mb.LinearNode(activation=ACT.SILU), V(lhs), V(rhs), V(out), residual=V(r))
+    want = act64(ACT.SILU, lhs.double() @ rhs.double())[0] + r.double()
+    op.replay()
+    op.quiesce_or_abort(20)
+    assert rel(out, want) <= 1e-5
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        op.replay(torch.cuda.current_stream().cuda_stream)
+    out.zero_()
+    graph.replay()
+    torch.cuda.synchronize()
+    assert rel(out, want) <= 1e-5
+    op.quiesce_or_abort(20)
+    del graph
+    op.close()
+
+
 @pytest.mark.parametrize("tr", [False, True])
 def test_f32_gradient(tr):
     g = gen(10)
