@@ -117,7 +117,7 @@ __global__ void __launch_bounds__(ES_THREADS) mmr_dispatch_kernel(const Dispatch
       int all = 0, pre = 0;
 #pragma unroll 8
       for (int b = b0; b < b1; ++b) {
-        const int c = *(p.hist + static_cast<long long>(b) * E + e);
+        const int c = __ldcg(p.hist + static_cast<long long>(b) * E + e);
         all += c;
         pre += b < static_cast<int>(blockIdx.x) ? c : 0;
       }
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(ES_THREADS) mmr_dispatch_kernel(const Dispatch
     Vec v[4];
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-      if (q < group && c + 32 * q < p.row_vecs) v[q] = *(src + c + 32 * q);
+      if (q < group && c + 32 * q < p.row_vecs) v[q] = __ldcg(src + c + 32 * q);
     for (int j0 = 0; j0 < p.top_k; j0 += 4) {
       int slot[4];
 #pragma unroll
@@ -313,7 +313,7 @@ __global__ void __launch_bounds__(128) mmr_combine_kernel(const CombineParams p)
           scale[q] = __shfl_sync(0xffffffffu, my_scale, (j0 + q) & 31);
           if (j0 + q >= many || c >= p.row_vecs) slot[q] = -1;
           if (slot[q] >= 0)
-            w[q] = *(reinterpret_cast<const Vec*>(static_cast<const char*>(p.rows.p) + slot[q] * p.rows.ld) + c);
+            w[q] = __ldcg(reinterpret_cast<const Vec*>(static_cast<const char*>(p.rows.p) + slot[q] * p.rows.ld) + c);
         }
 #pragma unroll
         for (int q = 0; q < kChoices; ++q) {
@@ -398,11 +398,11 @@ __global__ void __launch_bounds__(256) mmr_combine_grad_kernel(const CombineGrad
       for (int x = 0; x < U; ++x) {
         const int c = c0 + x * 32 * W;
         if (c >= p.row_vecs) continue;
-        dv[x] = *(d_out + c);
+        dv[x] = __ldcg(d_out + c);
 #pragma unroll
         for (int q = 0; q < 4; ++q)
           if (slot[q] >= 0 && p.d_weights)
-            w[x][q] = *(reinterpret_cast<const Vec*>(static_cast<const char*>(p.rows.p) + slot[q] * p.rows.ld) + c);
+            w[x][q] = __ldcg(reinterpret_cast<const Vec*>(static_cast<const char*>(p.rows.p) + slot[q] * p.rows.ld) + c);
       }
 #pragma unroll
       for (int x = 0; x < U; ++x) {

@@ -464,7 +464,7 @@ struct Groups {  // ragged rows or contraction
 // 2 us of what was measured there.
 //
 // Strip: 5.5 for launch, first bytes and last store; then the longer of the
-// weights' way from memory and the k-blocks of the SM with the most CTAs (its
+// weights' way from memory (6.4 TB/s, 5.3 with one CTA an SM) and the k-blocks of the SM with the most CTAs (its
 // MMAs bound one at 0.235 up to 64 rows and 0.21 at 128, where another CTA hides
 // its latencies; alone 0.25 and 0.33); 3 for every further wave of CTAs; the join
 // of K slices and the epilogue by rows. A narrower strip than 128 columns only lost:
@@ -503,7 +503,7 @@ StripShape strip_shape(int sms, int64_t mats, double rows, bool ragged, int64_t 
       const int64_t deep = (ctas + sms - 1) / sms, waves = (ctas + sms * share - 1) / (sms * share);
       const int64_t blocks = (k_blocks + split - 1) / split;
       const double stream = double(deep * blocks) * (mt <= 64 ? (deep > 1 ? 0.235 : 0.25) : deep > 1 ? 0.21 : 0.33);
-      const double memory = double(mats) * double(n) * k_blocks * 128 / 6.4e6;
+      const double memory = double(mats) * double(n) * k_blocks * 128 / (deep > 1 ? 6.4e6 : 5.3e6);
       const double us = 5.5 + std::max(stream, memory) + 3.0 * double(waves - 1) +
                         (split > 1 ? 0.5 + 0.012 * mt : 0.02 * mt);
       if (best.us == 0 || us < best.us - 0.05) best = {mt, split, stages, us};

@@ -171,9 +171,9 @@ __device__ __forceinline__ void fence_proxy_async_global() {
 // no-op when the launch had no programmatic predecessor). griddep_release()
 // lets the next such launch start its own prologue; it only schedules CTAs,
 // whose global accesses still wait for this grid to complete. A kernel that is
-// resident while its input is still being written reads it with plain loads, not
-// through the read-only path (ld.global.nc), which supposes that nothing writes
-// the data while the kernel lives.
+// resident while its input is still being written reads it with plain loads or
+// past L1 (__ldcg), not through the read-only path (ld.global.nc), which supposes
+// that nothing writes the data while the kernel lives.
 __device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void griddep_release() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -170,7 +170,7 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 3) mmr_act_grad_kern
   auto load = [&](const T* q, const EpiMat& m, Raw& r) {
     if (VEC) {
 #pragma unroll
-      for (int i = 0; i < kVec; ++i) r.w[i] = *(reinterpret_cast<const uint4*>(q + tx * 8) + i);
+      for (int i = 0; i < kVec; ++i) r.w[i] = __ldcg(reinterpret_cast<const uint4*>(q + tx * 8) + i);
     } else {
 #pragma unroll
       for (int i = 0; i < 8; ++i) r.t[i] = c0 + col(i) < p.n ? q[col(i) * m.cs] : from_f32<T>(0.0f);
