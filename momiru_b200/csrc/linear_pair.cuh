@@ -22,14 +22,15 @@
 // Work split: whole rounds of tiles, one a pair. Where the tiles of the last
 // round fill at most half the pairs they are cut into two 256 x 128 halves
 // (64 columns a CTA), one a pair, so the round ends after half the MMAs and a
-// product of few tiles reaches twice the SMs: 512 x 4096 x 4096 23 us against
-// 29 uncut, 4096^3 (3.46 rounds) 96 us before. Dividing those tiles along K
+// product of few tiles reaches twice the SMs: 512 x 4096 x 4096 22.5 us against
+// 29 uncut; 4096^3 (3.46 rounds) 96 us. Dividing those tiles along K
 // instead, with parts parked in memory and joined by the last to finish, cost
 // more than it saved (104 and 36 us): a part's 256 KB go out and come back.
 //
 // Bound: the tensor pipe. A tile of 4096 k takes 33.3 thousand cycles against
-// 32.8 of MMAs; the clock under that load is the power cap's (1.63 GHz where it
-// was traced), 1.53 PFLOP/s at 4096 x 11008 x 4096.
+// 32.8 of MMAs; the clock under that load is the power cap's. 4096 x 11008 x
+// 4096: 1.53 PFLOP/s in a short run (1.63 GHz), 1.29 after a second of it (1.27
+// GHz; the library's product 1.30 on the same box).
 //
 // Warps: 0-7 epilogue (TMEM lane quarter x column half), 8 TMA producer, 9 MMA
 // issuer (even CTA), 10-11 idle.
