@@ -12,7 +12,10 @@ use std::env;
 use std::path::{Path, PathBuf};
 use std::process::Command;
 
-const UNITS: [&str; 5] = ["momiru_gemm", "tc_strict_pair", "tc_tf32_pair", "tc_strict_1cta", "tc_tf32_1cta"];
+const UNITS: [&str; 9] = [
+    "momiru_gemm", "tc_strict_pair", "tc_tf32_pair", "tc_strict_1cta", "tc_tf32_1cta", "ops", "linear_strip",
+    "linear_pair_bf16", "linear_pair_f16",
+];
 const FLAGS: [&str; 16] = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-O3", "-lineinfo", "-std=c++17", "-ftz=false",
     "-prec-div=true", "-prec-sqrt=true", "-fmad=true", "-Xcompiler", "-fPIC", "-Xcompiler",
@@ -32,7 +35,9 @@ pub fn build_gpu_gemm() {
     let root = PathBuf::from(env::var("CARGO_MANIFEST_DIR").expect("manifest dir"));
     let csrc = root.join("momiru_b200").join("csrc");
     println!("cargo:rerun-if-changed={}", csrc.display());
-    println!("cargo:rerun-if-changed={}", root.join("include").join("momiru_gemm.h").display());
+    for header in ["momiru_gemm.h", "momiru_ops.h"] {
+        println!("cargo:rerun-if-changed={}", root.join("include").join(header).display());
+    }
     let out = PathBuf::from(env::var("OUT_DIR").expect("out dir"));
     let objs: Vec<PathBuf> = UNITS.iter().map(|u| out.join(format!("{u}.o"))).collect();
     let children: Vec<_> = UNITS

@@ -27,6 +27,7 @@
 
 pub mod collective;
 pub mod ffi;
+pub mod ops_ffi;
 pub mod validate;
 
 use core::ptr;

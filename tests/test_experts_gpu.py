@@ -252,6 +252,32 @@ def test_expert_gradient(kind, tokens, top_k, experts, align, k, n):
             check(d_b[e], want, u * want.abs() + (2.0 ** -18 + (c + 1) * 2.0 ** -24) * (dp.abs() + y.abs()).sum(0) + TINY, "d_bias")
 
 
+def test_offsets_past_32_bits():
+    """Sorted rows a long pitch apart: the last ones lie beyond 2^31 elements."""
+    pitch, h, tokens = 3 << 28, 64, 3
+    ids = np.array([[0, 1], [1, 0], [1, -1]], np.int32)
+    x = rand(gen(16), tokens, h, dtype=torch.bfloat16)
+    lay = mb.ExpertLayout.empty(tokens, 2, 2, 1)
+    big = torch.empty((lay.rows - 1) * pitch + h, dtype=torch.bfloat16, device="cuda")
+    rows = big.as_strided((lay.rows, h), (pitch, 1))
+    replay(mb.BoundDispatch(lay, V(torch.from_numpy(ids).cuda()), V(x), V(rows)))
+    check_dispatch(ids, 2, 1, x, lay, rows)
+    y, w = torch.empty_like(x), torch.ones(tokens, 2, device="cuda")
+    replay(mb.BoundCombine(lay, V(rows), V(y), weights=V(w)))
+    assert torch.equal(y, x * torch.tensor([[2.0], [2.0], [1.0]], device="cuda", dtype=torch.bfloat16))
+    d_w = torch.empty_like(w)
+    replay(mb.BoundCombineGrad(lay, V(x), V(rows), V(w), d_rows=V(rows.clone()), d_weights=V(d_w)))
+    square = (x.double() ** 2).sum(1)
+    want = torch.stack((square, square * torch.tensor([1, 1, 0], device="cuda")), 1)
+    check(d_w, want, (h + 1) * 2.0 ** -24 * want + 1e-30, "d_weights")
+    k = rand(gen(17), 2, h, 24, dtype=torch.bfloat16)
+    out = torch.empty(lay.rows, 24, dtype=torch.bfloat16, device="cuda")
+    replay(mb.BoundExpertLinear(mb.LinearNode(), lay, V(rows), V(k), V(out)))
+    same = torch.empty_like(out)
+    replay(mb.BoundExpertLinear(mb.LinearNode(), lay, V(rows.contiguous()), V(k), V(same)))
+    assert torch.equal(out, same)
+
+
 def test_equal_runs_give_equal_bits():
     t, u, g, lay, rows, w = expert_setup("bf16", "few", 600, 2, 5, 64, 136, 264, False)
     outs = []

@@ -61,6 +61,24 @@ def test_exports_and_structs_follow_the_header():
         assert names == [f for f, _ in struct._fields_], name
 
 
+def test_rust_binding_follows_the_header():
+    with open(os.path.join(ROOT, "rust", "src", "gpu_gemm", "ops_ffi.rs")) as f:
+        rust = f.read()
+    consts = dict(re.findall(r"\b(MMR_(?:DTYPE|ACT)_\w+) = (\d+)", HEADER))
+    assert dict(re.findall(r"pub const (MMR_\w+): i32 = (\d+);", rust)) == consts
+    assert set(re.findall(r"pub fn (mmr_\w+)\(", rust)) == set(_ops_abi.EXPORTED)
+    structs = re.findall(r"pub struct (mmr_\w+) \{(.*?)\n\}", rust, re.S)
+    mirror = {"Mmr" + "".join(w.title() for w in n.split("_")[1:]): re.findall(r"pub (\w+):", body) for n, body in structs
+              if n != "mmr_op_handle"}
+    assert len(mirror) == 9
+    for name, fields in mirror.items():
+        assert fields == [f for f, _ in getattr(_ops_abi, name)._fields_], name
+    with open(os.path.join(ROOT, "rust", "build_gpu.rs")) as f:
+        units = re.search(r"UNITS: \[&str; \d+\] = \[(.*?)\];", f.read(), re.S).group(1)
+    from momiru_b200 import build
+    assert sorted(re.findall(r'"(\w+)"', units)) == sorted(os.path.splitext(u)[0] for u in build.SOURCES)
+
+
 @pytest.mark.parametrize("tokens,top_k,experts,align", [
     (0, 1, 1, 1), (1, 1, 1, 1), (1, 1, 8, 128), (3, 2, 64, 16), (100, 8, 64, 64), (4099, 4, 24, 64), (7, 1, 1024, 1)])
 def test_capacity_holds_the_worst_routing(tokens, top_k, experts, align):
