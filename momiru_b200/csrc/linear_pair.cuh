@@ -1,38 +1,42 @@
 // linear_pair.cuh -- the 16-bit product on CTA pairs (tcgen05 cta_group::2):
 //   out = epilogue(A B), A m x k, B k x n, both bf16 or both f16, f32 sums.
 //
-// A pair computes a 256 x 256 tile with one 256 x 256 x 16 instruction per
-// k-step: each CTA stages its 128 rows of A and its half of B's columns in
-// 64-wide k-blocks (128-byte swizzled rows, 32 KiB a stage), and keeps two
-// 128 x 256 f32 accumulators in tensor memory, so that the epilogue of one tile
-// runs under the MMAs of the next.
+// A pair computes a tile of 256 columns by up to 256 rows with one instruction
+// per 16 of K: the columns (B, the weights) are the instruction's 256 rows, 128 a
+// CTA, and the rows of A its columns, any multiple of 32, half a CTA. So a tile
+// costs what its rows need: 300 rows are two tiles of 160, an expert's last tile
+// ends with its tokens. Each CTA stages its 128 columns of B and its half of the
+// rows of A in 64-wide k-blocks (128-byte swizzled rows, 32 KiB a stage), and
+// keeps two 128 x 256 f32 accumulators in tensor memory, so that the epilogue of
+// one tile runs under the MMAs of the next.
 //
 // RAG 0: one product; tiles walk in groups of LP_GROUP row tiles so that the
-//        pairs running together share panels in L2.
+//        pairs running together share panels in L2 (4 or 16 lost 1 to 7 %).
 // RAG 1: ragged rows, the experts' products: expert e multiplies rows
 //        [offsets[e], offsets[e] + counts[e]) of A by its own B (the tensor
-//        map's batch). Tiles start at the segment, rows past its tokens are
-//        stored as zeros up to the segment's end, and so are the rows after
-//        the last segment.
+//        map's batch). Tiles start at the segment; the rows past its tokens, up
+//        to the segment's end, are stored as zeros, and so are the rows after the
+//        last segment.
 // RAG 2: ragged contraction, the experts' weight gradients: out[e] = A_e^T B_e
 //        over the segment's rows. Segments are multiples of 64 rows whose pad
 //        rows are zero, so a k-block never meets another expert's rows; an
 //        expert without tokens gets zeros.
 //
 // Work split: whole rounds of tiles, one a pair. Where the tiles of the last
-// round fill at most half the pairs they are cut into two 256 x 128 halves
-// (64 columns a CTA), one a pair, so the round ends after half the MMAs and a
-// product of few tiles reaches twice the SMs: 512 x 4096 x 4096 22.5 us against
-// 29 uncut; 4096^3 (3.46 rounds) 96 us. Dividing those tiles along K
-// instead, with parts parked in memory and joined by the last to finish, cost
-// more than it saved (104 and 36 us): a part's 256 KB go out and come back.
+// round fill at most half the pairs, each is cut into two of half its rows, so
+// the round ends after half the MMAs and a product of few tiles reaches twice the
+// SMs: 512 x 4096 x 4096 22.5 us against 29 uncut; 4096^3 (3.46 rounds) 96 us.
+// Dividing those tiles along K instead, with parts parked in memory and joined by
+// the last to finish, cost more than it saved (104 and 36 us): a part's 256 KB
+// go out and come back.
 //
 // Bound: the tensor pipe. A tile of 4096 k takes 33.3 thousand cycles against
 // 32.8 of MMAs; the clock under that load is the power cap's. 4096 x 11008 x
 // 4096: 1.53 PFLOP/s in a short run (1.63 GHz), 1.29 after a second of it (1.27
 // GHz; the library's product 1.30 on the same box).
 //
-// Warps: 0-7 epilogue (TMEM lane quarter x column half), 8 TMA producer, 9 MMA
+// Warps: 0-7 epilogue (TMEM lane quarter = 32 columns, every second box of 32
+// rows), 8 TMA producer, 9 MMA
 // issuer (even CTA), 10-11 idle.
 #pragma once
 #include <type_traits>
@@ -64,6 +68,7 @@ static_assert(lp_smem_bytes(0) <= 232448 && lp_smem_bytes(1) <= 232448, "shared 
 struct PairParams {
   int m = 0, n = 0;
   int tiles_m = 0, tiles_n = 0, tiles_total = 0;  // RAG 1: tiles_n only
+  int tile_rows = 256;                            // rows of a tile, a multiple of 32 (RAG 1: by expert)
   int k_blocks = 0;                               // RAG 2: from the counts
   int experts = 0;
   const int* offsets = nullptr;
@@ -74,14 +79,17 @@ struct PairParams {
   unsigned long long timeout_ns = 0;
 };
 
+// Rows of each of `tiles` equal tiles of `rows` rows; tiles = ceil(rows / 256),
+// so every tile but the last is full and the last has at least one row.
+__host__ __device__ inline int lp_tile_rows(int rows, int tiles) { return ((rows + tiles - 1) / tiles + 31) / 32 * 32; }
+
 // One piece of work, found from its index.
 struct LpTile {
-  int row0, row_end, zero_end;  // output rows: [row0, row_end) computed, up to zero_end zeroed
-  int a_row;                    // row coordinate of A's tile
+  int row0, rows;         // first row, and the instruction's columns: a multiple of 32
+  int row_end, zero_end;  // rows from row_end on are not stored; [row_end, zero_end) are zeroed
   int col0;
-  bool half;                    // 128 columns instead of 256
-  int batch;                    // expert
-  int kb, k_row;                // k-blocks, and the row where the contraction starts (RAG 2)
+  int batch;              // expert
+  int kb, k_row;          // k-blocks, and the row where the contraction starts (RAG 2)
 };
 
 template <int RAG>
@@ -99,32 +107,34 @@ struct LpWalk {
   }
   __device__ __forceinline__ bool next(LpTile& w) {
     if (t >= end) return false;
-    int tile = t, right = 0;
-    w.half = t >= whole;
-    if (w.half) {
+    int tile = t, part = -1;
+    if (t >= whole) {
       tile = whole + ((t - whole) >> 1);
-      right = (t - whole) & 1;
+      part = (t - whole) & 1;
     }
     t += step;
-    int mt, nt;
+    int mt, nt, per, m;
     w.batch = 0;
     w.kb = p.k_blocks;
     w.k_row = 0;
+    w.row0 = 0;
+    w.zero_end = 0;
     if (RAG == 1) {
       while (first[e + 1] <= tile) ++e;
       const int local = tile - first[e], tm = (cnt[e] + 255) >> 8;
       mt = local % tm;
       nt = local / tm;
-      w.row0 = w.a_row = off[e] + mt * 256;
-      w.row_end = off[e] + cnt[e];
-      w.zero_end = off[e + 1];
+      m = cnt[e];
+      per = lp_tile_rows(m, tm);
+      w.row0 = off[e];
       w.batch = e;
+      if (mt == tm - 1 && part != 0) w.zero_end = off[e + 1];
     } else {
       int r = tile;
       if (RAG == 2) {
-        const int per = p.tiles_m * p.tiles_n;
-        w.batch = tile / per;
-        r = tile - w.batch * per;
+        const int each = p.tiles_m * p.tiles_n;
+        w.batch = tile / each;
+        r = tile - w.batch * each;
         w.kb = (cnt[w.batch] + LP_BK - 1) / LP_BK;
         w.k_row = off[w.batch];
       }
@@ -132,11 +142,23 @@ struct LpWalk {
       const int size = min(p.tiles_m - first_m, LP_GROUP), q = r - group * span;
       mt = first_m + q % size;
       nt = q / size;
-      w.row0 = w.a_row = mt * 256;
-      w.row_end = p.m;
-      w.zero_end = 0;
+      m = p.m;
+      per = p.tile_rows;
     }
-    w.col0 = nt * 256 + right * 128;
+    w.row_end = w.row0 + m;
+    w.row0 += mt * per;
+    w.rows = min(per, (w.row_end - w.row0 + 31) / 32 * 32);
+    if (part >= 0) {
+      const int left = (w.rows / 2 + 31) / 32 * 32;
+      if (part == 0) {
+        w.rows = left;
+      } else {
+        w.row0 += left;
+        w.rows -= left;
+      }
+      if (w.rows <= 0) w.kb = 0;  // a tile of 32 rows has no second half
+    }
+    w.col0 = nt * 256;
     return true;
   }
 };
@@ -235,8 +257,7 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
     LpWalk<RAG> walk(p, table, pair, npairs);
     LpTile w;
     const bool vec = epi_vec(p.epi);
-    // The bias eight columns at a time: n and the experts' rows multiples of 8,
-    // loaded a box ahead.
+    // The bias eight columns at a time: n and the experts' rows multiples of 8.
     const bool vec_bias = vec && p.epi.bias && p.epi.bias_s == 1 && (p.n & 7) == 0 && (p.epi.bias_bs & 7) == 0 &&
                           (reinterpret_cast<uintptr_t>(p.epi.bias) & 15) == 0;
     auto load_bias16 = [&](const LpTile& w, int col0) {
@@ -302,7 +323,6 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
           const float4 y = *reinterpret_cast<const float4*>(buf + rr * 128 + (((c2 + 1) ^ r0) << 4));
           float v[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
           if (row < w.row_end) epi_store8<T>(p.epi, batch, row, col, v, bias);
-          else if (RAG == 1 && row < w.zero_end) epi_zero8<T>(p.epi, row, col);
         }
       } else {
         // a lane a column, so that any pitch is stored in whole segments
@@ -310,7 +330,7 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
         if (col >= p.n) return;
         const float bias =
             p.epi.bias ? to_f32<T>(static_cast<const T*>(p.epi.bias)[w.batch * p.epi.bias_bs + col * p.epi.bias_s]) : 0.0f;
-        const int rows = min(w.row_end - row0, 32);  // rows past the tokens are zeroed below
+        const int rows = min(w.row_end - row0, 32);
         float add[32];
         if (p.epi.residual.p) {
           const T* q = static_cast<const T*>(p.epi.residual.p) + row0 * p.epi.residual.ld + col * p.epi.residual.cs;
@@ -329,7 +349,6 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
 #pragma unroll
           for (int r = 0; r < 32; ++r) {
             if (r < rows) *q = from_f32<T>(v[r]);
-            else if (RAG == 1 && row0 + r < w.zero_end) *q = from_f32<T>(0.0f);
             q += m.ld;
           }
         };
@@ -344,57 +363,66 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
     };
     while (walk.next(w)) {
       const bool sums = w.kb > 0;
-      const int row0 = w.row0 + static_cast<int>(rank) * 128 + quarter * 32;
-      const int boxes = w.half ? 2 : 4;  // of 32 columns, in this warp's half of the tile
-      const int cbase = w.col0 + half * boxes * 32;
-      const bool adds = vec && p.epi.residual.p && cbase < p.n && row0 < w.row_end;
+      // This warp's 32 columns, and every second box of 32 rows.
+      const int col0 = w.col0 + static_cast<int>(rank) * 128 + quarter * 32;
+      const int boxes = w.rows / 32;
+      const bool adds = vec && p.epi.residual.p && col0 < p.n;
       uint4 res[2][4];
-      // under the MMAs: the tile's residual to L2, its first box to registers
-      if (p.epi.residual.p && row0 + lane < w.row_end) {
-        const T* q = static_cast<const T*>(p.epi.residual.p) + (row0 + lane) * p.epi.residual.ld;
-        for (int c = cbase; c < min(cbase + boxes * 32, p.n); c += 64) prefetch_l2(q + c * p.epi.residual.cs);
+      // under the MMAs: the residual to L2, its first box to registers
+      if (p.epi.residual.p && col0 < p.n) {
+        for (int r = w.row0 + half * 32 + lane; r < min(w.row0 + w.rows, w.row_end); r += 64)
+          prefetch_l2(static_cast<const T*>(p.epi.residual.p) + r * p.epi.residual.ld + col0 * p.epi.residual.cs);
       }
-      if (adds) load_residual(w, row0, cbase, res[0]);
-      uint4 bias16[2];
-      bias16[0] = load_bias16(w, cbase);
+      if (adds && half < boxes) load_residual(w, w.row0 + half * 32, col0, res[0]);
+      const uint4 bias16 = load_bias16(w, col0);
       if (sums) {
         if (!mbar_wait_cluster(&acc_full[acc], acc_phase, ctl, kDevTimeoutAcc)) break;
         tc_fence_after();
       }
-      const uint32_t tb = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + acc * 256 + half * boxes * 32;
+      const uint32_t tb = tmem + (static_cast<uint32_t>(quarter * 32) << 16) + acc * 256;
+      auto release = [&] {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(acc_empty_leader + 8u * acc);
+      };
 #pragma unroll 1
-      for (int j2 = 0; j2 < boxes; j2 += 2) {
+      for (int j2 = half; j2 < boxes; j2 += 4) {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
-          const int j = j2 + b, col0 = cbase + j * 32;
-          if (j + 1 < boxes) {
-            if (adds) load_residual(w, row0, col0 + 32, res[b ^ 1]);
-            bias16[b ^ 1] = load_bias16(w, col0 + 32);
-          }
+          const int j = j2 + 2 * b, row0 = w.row0 + j * 32;
+          if (j >= boxes) continue;
+          if (adds && j + 2 < boxes) load_residual(w, row0 + 64, col0, res[b ^ 1]);
           uint32_t r[32];
           if (sums) {
             tmem_ld_32x32b_x32(tb + j * 32, r);
             tmem_ld_wait();
-            if (j == boxes - 1) {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive_cluster(acc_empty_leader + 8u * acc);
-            }
+            if (j + 2 >= boxes) release();  // the last of this warp's boxes is in registers
           } else {
 #pragma unroll
             for (int i = 0; i < 32; ++i) r[i] = 0u;
           }
-          if (col0 >= p.n || row0 >= max(w.row_end, w.zero_end)) continue;
+          if (col0 >= p.n || row0 >= w.row_end) continue;
+          // a lane holds a column: transposed on the way in, so that row i's
+          // 16-byte chunk q lies at q ^ (i & 7)
           __syncwarp();  // the box before has been read
 #pragma unroll
-          for (int q = 0; q < 8; ++q)
-            *reinterpret_cast<uint4*>(buf + lane * 128 + ((q ^ (lane & 7)) << 4)) =
-                make_uint4(r[4 * q], r[4 * q + 1], r[4 * q + 2], r[4 * q + 3]);
+          for (int i = 0; i < 32; ++i)
+            *reinterpret_cast<uint32_t*>(buf + i * 128 + ((((lane >> 2) ^ (i & 7)) << 4) | ((lane & 3) << 2))) = r[i];
           __syncwarp();
-          store_box(w, row0, col0, res[b], bias16[b]);
+          store_box(w, row0, col0, res[b], bias16);
         }
       }
-      if (sums && ++acc == 2) { acc = 0; acc_phase ^= 1u; }
+      if (sums) {
+        if (half >= boxes) release();  // 32 rows: nothing for the second four warps
+        if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+      }
+      if (RAG == 1) {
+        // the segment's rows past its tokens, this CTA's 128 columns of them
+        for (int c = static_cast<int>(threadIdx.x); w.row_end + c / 16 < w.zero_end; c += 256) {
+          const int col = w.col0 + static_cast<int>(rank) * 128 + (c % 16) * 8;
+          if (col < p.n) epi_zero8<T>(p.epi, w.row_end + c / 16, col);
+        }
+      }
     }
     if (RAG == 1) {
       const int g = static_cast<int>(blockIdx.x) * 8 + warp, gn = static_cast<int>(gridDim.x) * 8;
@@ -414,27 +442,28 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
       LpWalk<RAG> walk(p, table, pair, npairs);
       LpTile w;
       while (ok && walk.next(w)) {
-        const int m0 = w.a_row + static_cast<int>(rank) * 128, n0 = w.col0 + static_cast<int>(rank) * (w.half ? 64 : 128);
+        // this CTA's 128 columns and its half of the rows, in boxes of 64
+        const int n0 = w.col0 + static_cast<int>(rank) * 128, r0 = w.row0 + static_cast<int>(rank) * (w.rows / 2);
+        const bool two = w.rows > 128;
         for (int kb = 0; kb < w.kb; ++kb) {
           if (!mbar_wait_cluster(&empty[stage], phase ^ 1u, ctl, kDevTimeoutEmpty)) { ok = false; break; }
-          uint8_t* sa = ops + stage * LP_STAGE_BYTES;
-          uint8_t* sb = sa + LP_A_BYTES;
+          uint8_t* sw = ops + stage * LP_STAGE_BYTES;
+          uint8_t* sr = sw + LP_A_BYTES;
           const uint32_t bar = full_leader + 8u * stage;
           const int k0 = w.k_row + kb * LP_BK, bb = RAG == 1 ? w.batch : 0;
-          if (rank == 0) mbar_arrive_expect_tx(&full[stage], w.half ? 3 * LP_A_BYTES : 4 * LP_A_BYTES);
-          if (A_MN) {
-            tma_load_3d_pair(sa, &tmA, bar, m0, k0, 0);
-            tma_load_3d_pair(sa + LP_A_BYTES / 2, &tmA, bar, m0 + 64, k0, 0);
-          } else {
-            tma_load_3d_pair(sa, &tmA, bar, k0, m0, 0);
-          }
-          // 64 columns a box: one for a half tile, two for a whole one
+          if (rank == 0) mbar_arrive_expect_tx(&full[stage], two ? 4 * LP_A_BYTES : 3 * LP_A_BYTES);
           if (B_MN) {
-            tma_load_3d_pair(sb, &tmB, bar, n0, k0, bb);
-            if (!w.half) tma_load_3d_pair(sb + LP_A_BYTES / 2, &tmB, bar, n0 + 64, k0, bb);
+            tma_load_3d_pair(sw, &tmB, bar, n0, k0, bb);
+            tma_load_3d_pair(sw + LP_A_BYTES / 2, &tmB, bar, n0 + 64, k0, bb);
           } else {
-            tma_load_3d_pair(sb, &tmB, bar, k0, n0, bb);
-            if (!w.half) tma_load_3d_pair(sb + LP_A_BYTES / 2, &tmB, bar, k0, n0 + 64, bb);
+            tma_load_3d_pair(sw, &tmB, bar, k0, n0, bb);
+          }
+          if (A_MN) {
+            tma_load_3d_pair(sr, &tmA, bar, r0, k0, 0);
+            if (two) tma_load_3d_pair(sr + LP_A_BYTES / 2, &tmA, bar, r0 + 64, k0, 0);
+          } else {
+            tma_load_3d_pair(sr, &tmA, bar, k0, r0, 0);
+            if (two) tma_load_3d_pair(sr + LP_A_BYTES / 2, &tmA, bar, k0, r0 + 64, 0);
           }
           last[stage] = static_cast<int>(phase);
           if (++stage == S) { stage = 0; phase ^= 1u; }
@@ -458,15 +487,15 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
     // included, ~620, against 512 cycles of MMAs (a clock64 trace).
     if (rank == 0) {
       constexpr bool kBf16 = std::is_same<T, __nv_bfloat16>::value;
-      constexpr uint32_t idesc_whole = idesc_f16(256, 256, kBf16, A_MN, B_MN);
-      constexpr uint32_t idesc_half = idesc_f16(256, 128, kBf16, A_MN, B_MN);
+      // all but the instruction's columns
+      constexpr uint32_t idesc0 = idesc_f16(256, 0, kBf16, B_MN, A_MN);
       // K-major: 128-byte rows, 8-row groups 1024 bytes apart, 32 bytes a
       // k-step. MN-major: 64-element atoms 8 KiB apart (the 64 K rows of a
       // box), 8-row K groups 1024 bytes apart, two groups a k-step.
-      constexpr uint32_t a_lbo = A_MN ? 8192u : 16u, b_lbo = B_MN ? 8192u : 16u;
-      constexpr uint32_t a_step = A_MN ? 2048u : 32u, b_step = B_MN ? 2048u : 32u;
-      const uint64_t a_desc0 = smem_desc(smem_u32(ops), a_lbo, 1024u, 2u);
-      const uint64_t b_desc0 = smem_desc(smem_u32(ops) + LP_A_BYTES, b_lbo, 1024u, 2u);
+      constexpr uint32_t w_lbo = B_MN ? 8192u : 16u, r_lbo = A_MN ? 8192u : 16u;
+      constexpr uint32_t w_step = B_MN ? 2048u : 32u, r_step = A_MN ? 2048u : 32u;
+      const uint64_t w_desc0 = smem_desc(smem_u32(ops), w_lbo, 1024u, 2u);
+      const uint64_t r_desc0 = smem_desc(smem_u32(ops) + LP_A_BYTES, r_lbo, 1024u, 2u);
       const bool leader = elect_one();
       int stage = 0, acc = 0;
       uint32_t phase = 0, acc_phase = 0;
@@ -478,7 +507,7 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
         if (!__all_sync(0xffffffffu, mbar_wait_cluster(&acc_empty[acc], acc_phase ^ 1u, ctl, kDevTimeoutAcc))) break;
         tc_fence_after();
         const uint32_t d = tmem + static_cast<uint32_t>(acc * 256);
-        const uint32_t idesc = w.half ? idesc_half : idesc_whole;
+        const uint32_t idesc = idesc0 | (static_cast<uint32_t>(w.rows >> 3) << 17);
         bool ready = mbar_test_wait(smem_u32(&full[stage]), phase);
         for (int kb = 0; kb < w.kb; ++kb) {
           if (!__all_sync(0xffffffffu, ready))
@@ -493,7 +522,7 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
           if (leader) {
 #pragma unroll
             for (int kk = 0; kk < LP_BK / 16; ++kk)
-              umma_f16_2sm(d, a_desc0 + so + ((a_step * kk) >> 4), b_desc0 + so + ((b_step * kk) >> 4), idesc,
+              umma_f16_2sm(d, w_desc0 + so + ((w_step * kk) >> 4), r_desc0 + so + ((r_step * kk) >> 4), idesc,
                            kk > 0 || kb > 0 ? 1u : 0u);
             umma_commit_2sm_both(&empty[now]);
           }

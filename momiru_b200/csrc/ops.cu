@@ -591,6 +591,7 @@ int32_t add_product(Handle* h, int dtype, Operand a, Operand b, mmr::EpiParams e
   p.m = int(m);
   p.n = int(n);
   p.tiles_m = int((m + 255) / 256);
+  p.tile_rows = mmr::lp_tile_rows(p.m, p.tiles_m);
   p.tiles_n = int((n + 255) / 256);
   p.k_blocks = k_blocks;
   int64_t tiles = int64_t(p.tiles_m) * p.tiles_n;
@@ -606,8 +607,8 @@ int32_t add_product(Handle* h, int dtype, Operand a, Operand b, mmr::EpiParams e
   p.epi = epi;
   p.err = h->d_err;
   p.timeout_ns = kWaitNs;
-  MMR_TRY(encode16(&ta, a, dtype, 128, "lhs"));
-  MMR_TRY(encode16(&tb, b, dtype, 64, "rhs"));
+  MMR_TRY(encode16(&ta, a, dtype, 64, "lhs"));
+  MMR_TRY(encode16(&tb, b, dtype, 128, "rhs"));
   sh.grid = 2 * int(std::min<int64_t>(h->sms / 2, std::max<int64_t>(2 * tiles, 1)));
   MMR_CUDA(mmr::pair_prepare(sh));
   add_step(h, "mmr_linear_pair_kernel grid %lld, tiles %lld, k-blocks %lld", [=](cudaStream_t s) {
@@ -636,6 +637,7 @@ int32_t add_segment_product(Handle* h, int dtype, Operand a, Operand b, const Ep
   sh.rag = 2;
   sh.a_mn = sh.b_mn = true;
   p.tiles_m = (p.m + 255) / 256;
+  p.tile_rows = mmr::lp_tile_rows(p.m, p.tiles_m);
   p.tiles_n = (p.n + 255) / 256;
   const int64_t tiles = int64_t(p.tiles_m) * p.tiles_n * g.experts;
   MMR_TRY(check_tiles(tiles));
@@ -649,8 +651,8 @@ int32_t add_segment_product(Handle* h, int dtype, Operand a, Operand b, const Ep
   p.err = h->d_err;
   p.timeout_ns = kWaitNs;
   CUtensorMap ta, tb;
-  MMR_TRY(encode16(&ta, a, dtype, 128, "rows"));
-  MMR_TRY(encode16(&tb, b, dtype, 64, "d_out"));
+  MMR_TRY(encode16(&ta, a, dtype, 64, "rows"));
+  MMR_TRY(encode16(&tb, b, dtype, 128, "d_out"));
   sh.grid = 2 * int(std::min<int64_t>(h->sms / 2, 2 * tiles));
   MMR_CUDA(mmr::pair_prepare(sh));
   add_step(h, "mmr_linear_pair_kernel (segments) grid %lld, tiles %lld", [=](cudaStream_t s) {
