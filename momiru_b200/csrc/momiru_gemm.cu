@@ -1292,12 +1292,8 @@ static int32_t run_host_pipeline(mmr_gemm_handle* h, cudaStream_t s) {
   return MMR_OK;
 }
 
-int32_t mmr_gemm_run_on(mmr_gemm_handle* h, void* stream) {
-  if (!h) return fail(MMR_ERR_INVALID_ARGUMENT, "null handle");
-  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  DeviceGuard guard(h->device);
-  if (!guard.ok) return fail(MMR_ERR_CUDA, "cudaSetDevice(%d) failed", h->device);
-  if (h->host) return run_host_pipeline(h, s);
+// The launches of one run, on the current device.
+static int32_t enqueue(mmr_gemm_handle* h, cudaStream_t s) {
   cudaError_t e = cudaSuccess;
   if (!h->plan.empty) {
     switch (h->family) {
@@ -1329,6 +1325,16 @@ int32_t mmr_gemm_run_on(mmr_gemm_handle* h, void* stream) {
     e = cudaGetLastError();
   }
   if (e != cudaSuccess) return fail(MMR_ERR_CUDA, "kernel launch: %s", cudaGetErrorString(e));
+  return MMR_OK;
+}
+
+int32_t mmr_gemm_run_on(mmr_gemm_handle* h, void* stream) {
+  if (!h) return fail(MMR_ERR_INVALID_ARGUMENT, "null handle");
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  DeviceGuard guard(h->device);
+  if (!guard.ok) return fail(MMR_ERR_CUDA, "cudaSetDevice(%d) failed", h->device);
+  if (h->host) return run_host_pipeline(h, s);
+  if (int32_t rc = enqueue(h, s)) return rc;
   MMR_CUDA_TRY(cudaEventRecord(h->done, s));
   h->ran = true;
   return MMR_OK;
@@ -1343,9 +1349,9 @@ void gemm_set_chunk(mmr_gemm_handle* h, int k) {
   if (h->family == MMR_FAMILY_TCGEN05 && h->mode == 1)
     h->tcp.chunk_kb = std::max(1, std::min(k / int(h->launch.bk), h->tcp.k_blocks));
 }
-// A product that another handle runs: that one's event covers it (its own may
-// belong to a captured graph), so only its error word is left to read.
-void gemm_forget_run(mmr_gemm_handle* h) { h->ran = false; }
+// A run within another handle's, whose device guard and completion event cover
+// it: only its error word is left to read.
+int32_t gemm_enqueue(mmr_gemm_handle* h, cudaStream_t s) { return enqueue(h, s); }
 }  // namespace mmr
 
 extern "C" {

@@ -30,7 +30,7 @@ namespace mmr {
 // momiru_gemm.cu
 int32_t set_last_error(int32_t code, const char* message);
 void gemm_set_chunk(mmr_gemm_handle* h, int k);
-void gemm_forget_run(mmr_gemm_handle* h);
+int32_t gemm_enqueue(mmr_gemm_handle* h, cudaStream_t s);
 int32_t gemm_read_error(mmr_gemm_handle* h, uint64_t timeout_ns);
 }
 
@@ -400,6 +400,7 @@ int32_t admit(Handle* h, Operand* o, int major, const char* name, mmr::PackList*
   q.s_r = mn_major ? o->s_k : o->s_mn;
   q.s_c = mn_major ? o->s_mn : o->s_k;
   q.pitch = (q.cols + 7) / 8 * 8;
+  q.rows_out = q.rows;
   if (o->batch > 65535) return fail(MMR_ERR_UNSUPPORTED_LAYOUT, "%s: more than 65535 matrices to pack", name);
   const int64_t per = int64_t(q.rows) * q.pitch;
   q.batch = int(o->batch);
@@ -414,16 +415,18 @@ int32_t admit(Handle* h, Operand* o, int major, const char* name, mmr::PackList*
 }
 
 // One launch for all operands of a product that have to be packed.
-void add_packs(Handle* h, const mmr::PackList& packs) {
+void add_packs(Handle* h, const mmr::PackList& packs, int elem_bytes = 2) {
   if (packs.n == 0) return;
   int64_t tiles = 1, batch = 1;
   for (int i = 0; i < packs.n; ++i) {
-    tiles = std::max(tiles, int64_t((packs.p[i].rows + 31) / 32) * ((packs.p[i].pitch + 31) / 32));
+    tiles = std::max(tiles, int64_t((packs.p[i].rows_out + 31) / 32) * ((packs.p[i].pitch + 31) / 32));
     batch = std::max<int64_t>(batch, packs.p[i].batch);
   }
   const dim3 grid(unsigned(std::min<int64_t>(tiles, 8 * h->sms)), unsigned(packs.n), unsigned(batch));
-  add_step(h, "mmr_pack_kernel grid %lld x %lld x %lld", [packs, grid](cudaStream_t s) {
-    return mmr::launch_kernel(mmr::mmr_pack_kernel, grid, dim3(256), 0, s, dim3(1, 1, 1), packs);
+  add_step(h, "mmr_pack_kernel grid %lld x %lld x %lld", [packs, grid, elem_bytes](cudaStream_t s) {
+    return mmr::launch_kernel(
+        elem_bytes == 2 ? mmr::mmr_pack_kernel<unsigned short> : mmr::mmr_pack_kernel<unsigned int>, grid, dim3(256), 0, s,
+        dim3(1, 1, 1), packs);
   }, grid.x, grid.y, grid.z);
 }
 
@@ -757,20 +760,11 @@ mmr_view f32_view(uint64_t base, int64_t rows, int64_t cols, int64_t s_r, int64_
   v.strides[1] = s_c;
   return v;
 }
-mmr_view f32_view(const Ref& r, int device) {
-  return f32_view(r.base, r.d[1], r.d[2], r.s[1], r.s[2], device, r.lo, r.hi);
-}
 // A dense workspace matrix.
 mmr_view f32_view(const void* p, int64_t rows, int64_t cols, int64_t ld, int device) {
   const uint64_t b = reinterpret_cast<uint64_t>(p);
   return f32_view(b, rows, cols, ld, 1, device, b, b + 4 * uint64_t(rows) * ld);
 }
-mmr_view transposed(mmr_view v) {
-  std::swap(v.dims[0], v.dims[1]);
-  std::swap(v.strides[0], v.strides[1]);
-  return v;
-}
-
 // K elements summed in tensor memory at a time. The tensor core's additions
 // truncate, and the error of a product is that of one chunk: 2.1e-6 relative at
 // the node's 256, 1.2e-6 at 128, 7.9e-7 at 64, 5.7e-7 at 32, for 256 / 272 / 290
@@ -802,12 +796,205 @@ int32_t add_f32_product(Handle* h, int math, const mmr_view& lhs, const mmr_view
   h->products.push_back(g);
   mmr::gemm_set_chunk(g, kF32Chunk);
   h->plan += "matmul node (f32)\n";
-  h->steps.push_back({"matmul node (f32)", [g](cudaStream_t s) {
-                        const int32_t rc = mmr_gemm_run_on(g, s);
-                        mmr::gemm_forget_run(g);
-                        return rc;
-                      }});
+  h->steps.push_back({"matmul node (f32)", [g](cudaStream_t s) { return mmr::gemm_enqueue(g, s); }});
   return MMR_OK;
+}
+
+// An f32 matrix as a product reads it: rows x cols with element strides.
+struct F32Mat {
+  uint64_t base = 0;
+  int64_t rows = 0, cols = 0, s_r = 0, s_c = 0;
+  F32Mat t() const { return {base, cols, rows, s_c, s_r}; }
+};
+F32Mat f32_mat(const Ref& r) { return {r.base, r.d[1], r.d[2], r.s[1], r.s[2]}; }
+
+// As TMA wants it: one axis contiguous, the other a pitch of whole 16 bytes.
+bool f32_aligned(const F32Mat& o) {
+  auto ok = [&](int64_t unit, int64_t extent, int64_t pitch, int64_t other) {
+    return (unit == 1 || extent == 1) && (other == 1 || (pitch > 0 && pitch % 4 == 0 && pitch >= extent));
+  };
+  return o.base % 16 == 0 && (ok(o.s_c, o.cols, o.s_r, o.rows) || ok(o.s_r, o.rows, o.s_c, o.cols));
+}
+
+// A batch of `parts` views along the contraction of a (axis `cols`) or b (`rows`).
+mmr_view f32_parts_view(const F32Mat& o, bool along_cols, int parts, int64_t each, int device) {
+  mmr_view v{};
+  const int64_t rows = along_cols ? o.rows : each, cols = along_cols ? each : o.cols;
+  const int64_t step = each * (along_cols ? o.s_c : o.s_r);
+  v.rank = 3;
+  v.device_ordinal = device;
+  v.dims[0] = parts;
+  v.dims[1] = rows;
+  v.dims[2] = cols;
+  v.strides[0] = step;
+  v.strides[1] = o.s_r;
+  v.strides[2] = o.s_c;
+  v.address = o.base;
+  v.bytes = 4 * uint64_t((parts - 1) * step + (rows - 1) * o.s_r + (cols - 1) * o.s_c + 1);
+  return v;
+}
+
+// x = a b, bare, in f32: into `out` where that can hold it, else into a
+// workspace; *x says where, in *parts K parts that the reader adds. *direct: the
+// whole product lies in out. A bias that is all that follows the product may be
+// given; it is added in the node's epilogue, and *biased set, where *direct is.
+//
+// Up to eight rows against a K-contiguous b: the dot kernel (1 x 4096 x 4096 184
+// -> 16 us). Otherwise the MatMul node, with operands that TMA cannot read packed
+// first, and a K that is long for its few tiles divided into a batch of parts
+// (100 x 1000 x 8000: 347 -> 43 us; both, 500 x 77 x 5000: 732 -> 36 us). The parts'
+// number is the one of least estimated time: 0.42 us a 16-wide k-block on the
+// CTA-pair kernel, 0.72 on the one-CTA kernel (up to 128 rows).
+int32_t add_f32_bare(Handle* h, int math, F32Mat a, F32Mat b, const F32Mat& out, bool out_free, const Ref* bias,
+                     EpiMat* x, int* parts, bool* direct, bool* biased) {
+  const int64_t m = a.rows, k = a.cols, n = b.cols;
+  const int dev = h->device;
+  auto use_out = [&] {
+    x->p = reinterpret_cast<void*>(out.base);
+    x->ld = out.s_r;
+    x->cs = out.s_c;
+    x->vec = out.s_c == 1 && out.base % 16 == 0 && (out.s_r % 4 == 0 || m == 1) && n > 1;
+    *parts = 1;
+    *direct = true;
+  };
+  auto use_workspace = [&](int count) -> int32_t {
+    const int64_t ld = (n + 3) / 4 * 4;
+    void* w = nullptr;
+    MMR_TRY(workspace(h, size_t(count) * m * ld * 4, &w));
+    x->p = w;
+    x->bs = m * ld;
+    x->ld = ld;
+    x->cs = 1;
+    x->vec = 1;
+    *parts = count;
+    *direct = false;
+    return MMR_OK;
+  };
+  auto plain_view = [&](const F32Mat& o) {
+    // the view's own bytes, from its lowest element (bounds were checked against its buffer)
+    const int64_t lo = std::min<int64_t>(0, (o.rows - 1) * o.s_r) + std::min<int64_t>(0, (o.cols - 1) * o.s_c);
+    const int64_t hi = std::max<int64_t>(0, (o.rows - 1) * o.s_r) + std::max<int64_t>(0, (o.cols - 1) * o.s_c);
+    return f32_view(o.base, o.rows, o.cols, o.s_r, o.s_c, dev, o.base + 4 * lo, o.base + 4 * (hi + 1));
+  };
+  auto x_view = [&] { return f32_view(x->p, m, n, x->ld, dev); };
+  auto node = [&] {
+    *biased = *direct && bias && bias->on;
+    return add_f32_product(h, math, plain_view(a), plain_view(b), *direct ? plain_view(out) : x_view(),
+                           *biased ? bias : nullptr, *biased ? MMR_EPI_BIAS : MMR_EPI_NONE);
+  };
+  *biased = false;
+  if (k == 0) {
+    MMR_TRY(use_workspace(1));
+    void* w = x->p;
+    const size_t bytes = size_t(m) * x->ld * 4;
+    add_step(h, "zeros", [=](cudaStream_t s) { return cudaMemsetAsync(w, 0, bytes, s); });
+    return MMR_OK;
+  }
+  if (math == MMR_MATH_EXACT) {  // sums in the node's own order
+    if (out_free) use_out();
+    else MMR_TRY(use_workspace(1));
+    return node();
+  }
+  if (m <= 8 && (b.s_r == 1 || k == 1)) {
+    if (out_free) use_out();
+    else MMR_TRY(use_workspace(1));
+    mmr::DotParams p;
+    p.a = reinterpret_cast<const float*>(a.base);
+    p.b = reinterpret_cast<const float*>(b.base);
+    p.x = static_cast<float*>(x->p);
+    p.a_m = a.s_r;
+    p.a_k = a.s_c;
+    p.b_n = b.s_c;
+    p.x_m = x->ld;
+    p.x_n = x->cs;
+    p.m = int(m);
+    p.n = int(n);
+    p.k = int(k);
+    const bool vec = k % 4 == 0 && b.base % 16 == 0 && b.s_c % 4 == 0 && a.s_c == 1 && a.base % 16 == 0 &&
+                     (a.s_r % 4 == 0 || m == 1);
+    using K = void (*)(const mmr::DotParams);
+    const K kernel = m == 1   ? (vec ? mmr::mmr_dot_kernel<1, true> : mmr::mmr_dot_kernel<1, false>)
+                     : m == 2 ? (vec ? mmr::mmr_dot_kernel<2, true> : mmr::mmr_dot_kernel<2, false>)
+                     : m <= 4 ? (vec ? mmr::mmr_dot_kernel<4, true> : mmr::mmr_dot_kernel<4, false>)
+                              : (vec ? mmr::mmr_dot_kernel<8, true> : mmr::mmr_dot_kernel<8, false>);
+    const int grid = int(std::min<int64_t>((n + 7) / 8, 16 * h->sms));
+    add_step(h, "mmr_dot_kernel grid %lld", [=](cudaStream_t s) {
+      return mmr::launch_kernel(kernel, dim3(grid), dim3(256), 0, s, dim3(1, 1, 1), p);
+    }, grid);
+    return MMR_OK;
+  }
+  // The streaming kernels take few rows against a row-major b, and any a.
+  const bool stream = m <= 16 && (b.s_c == 1 || n == 1);
+  int count = 1;
+  if (!stream) {
+    const int64_t tiles = m > 128 ? (m + 255) / 256 * ((n + 255) / 256) : (n + 255) / 256;
+    const int64_t units = m > 128 ? h->sms / 2 : h->sms;
+    const double t = m > 128 ? 0.42 : 0.72;
+    const int64_t blocks = (k + 15) / 16;
+    double best = 0;
+    for (int s = 1; s <= 16 && blocks >= 4 * s; s *= 2) {
+      const double us = double((tiles * s + units - 1) / units) * double((blocks + s - 1) / s) * t +
+                        (s > 1 ? 2.0 + double(s) * m * n * 8 / 4e6 : 0.0) +
+                        (s > 1 && k % (4 * s) ? 3.0 + double(m + n) * k * 8 / 3e6 : 0.0);
+      if (s == 1 || us < best) {
+        best = us;
+        count = s;
+      }
+    }
+  }
+  // K of each part, and the padded K when the parts are not equal as they lie.
+  const bool uneven = count > 1 && k % (4 * count) != 0;
+  const int64_t each = uneven ? ((k + count - 1) / count + 15) / 16 * 16 : k / count, k_padded = uneven ? each * count : k;
+  mmr::PackList packs;
+  auto pack = [&](F32Mat* o, bool k_is_cols) -> int32_t {
+    const bool cols_inner = std::abs(o->s_c) <= std::abs(o->s_r);
+    mmr::PackParams q;
+    q.src = reinterpret_cast<const void*>(o->base);
+    q.rows = int(cols_inner ? o->rows : o->cols);
+    q.cols = int(cols_inner ? o->cols : o->rows);
+    q.s_r = cols_inner ? o->s_r : o->s_c;
+    q.s_c = cols_inner ? o->s_c : o->s_r;
+    const bool k_inner = cols_inner == k_is_cols;
+    q.pitch = int(((k_inner ? k_padded : int64_t(q.cols)) + 3) / 4 * 4);
+    q.rows_out = int(k_inner ? int64_t(q.rows) : k_padded);
+    MMR_TRY(workspace(h, size_t(q.rows_out) * q.pitch * 4, &q.dst));
+    packs.p[packs.n++] = q;
+    o->base = reinterpret_cast<uint64_t>(q.dst);
+    (cols_inner ? o->s_r : o->s_c) = q.pitch;
+    (cols_inner ? o->s_c : o->s_r) = 1;
+    (k_is_cols ? o->cols : o->rows) = k_padded;
+    return MMR_OK;
+  };
+  if (!stream && (uneven || !f32_aligned(a))) MMR_TRY(pack(&a, true));
+  if (uneven || !f32_aligned(b)) MMR_TRY(pack(&b, false));
+  add_packs(h, packs, 4);
+  if (count == 1) {
+    if (out_free && (stream || (out.s_c == 1 && f32_aligned(out)))) use_out();
+    else MMR_TRY(use_workspace(1));
+    return node();
+  }
+  MMR_TRY(use_workspace(count));
+  mmr_view to = x_view();
+  to.rank = 3;
+  to.dims[0] = count;
+  to.dims[1] = m;
+  to.dims[2] = n;
+  to.strides[0] = x->bs;
+  to.strides[1] = x->ld;
+  to.strides[2] = 1;
+  to.bytes = 4 * uint64_t(count) * x->bs;
+  return add_f32_product(h, math, f32_parts_view(a, true, count, each, dev), f32_parts_view(b, false, count, each, dev),
+                         to, nullptr, MMR_EPI_NONE);
+}
+
+// pre = sum of x's parts + bias; out = act(pre) + residual.
+void add_act_res(Handle* h, int act, const mmr::ActResParams& q) {
+  const int grid = int(std::min<int64_t>((int64_t(q.m) * ((q.n + 127) / 128) + 7) / 8, 16 * h->sms));
+  add_step(h, "mmr_act_res_kernel grid %lld, %lld parts", [=](cudaStream_t s) {
+    using K = void (*)(const mmr::ActResParams);
+    const K k = pick_act(act, [](auto a) -> K { return mmr::mmr_act_res_kernel<decltype(a)::value>; });
+    return mmr::launch_kernel(k, dim3(grid), dim3(256), 0, s, dim3(1, 1, 1), q);
+  }, grid, q.parts);
 }
 
 int32_t check_math(int dtype, int math) {
@@ -888,46 +1075,25 @@ int32_t linear_bind(const mmr_linear_desc* d, Handle** out) {
     return MMR_OK;
   }
   if (lhs.dtype == MMR_DTYPE_F32) {
-    const mmr_view a = f32_view(lhs, dev), b = f32_view(rhs, dev);
-    if (!res.on && !pre.on && d->activation == MMR_ACT_NONE) {
-      MMR_TRY(add_f32_product(h.get(), d->math_mode, a, b, f32_view(o, dev), &bias, bias.on ? MMR_EPI_BIAS : MMR_EPI_NONE));
-    } else {
-      // The bare product goes to pre, or to out, or (where out is the residual)
-      // to a workspace, and one pass does the rest. The node's own epilogue takes
-      // an activation as a call per element: 2048 x 4096 x 4096 with bias and
-      // SiLU took 375 us in it, 256 bare.
-      mmr::ActResParams q;
-      mmr_view to;
-      if (pre.on) {
-        to = f32_view(pre, dev);
-        q.x = q.pre = epi_mat(pre);
-      } else if (!res.on || !overlap(o, res)) {
-        to = f32_view(o, dev);
-        q.x = epi_mat(o);
-      } else {
-        void* w = nullptr;
-        const int64_t ld = (n + 3) / 4 * 4;
-        MMR_TRY(workspace(h.get(), size_t(m) * ld * 4, &w));
-        to = f32_view(w, m, n, ld, dev);
-        q.x.p = w;
-        q.x.ld = ld;
-        q.x.cs = 1;
-        q.x.vec = 1;
-      }
-      MMR_TRY(add_f32_product(h.get(), d->math_mode, a, b, to, nullptr, MMR_EPI_NONE));
+    // The bare product, then one pass for what follows it. The node's own
+    // epilogue takes an activation as a call per element: 2048 x 4096 x 4096 with
+    // bias and SiLU took 375 us in it, 256 bare.
+    mmr::ActResParams q;
+    const Ref& to = pre.on ? pre : o;
+    const bool to_free = pre.on || !res.on || !overlap(o, res);
+    const bool more = res.on || pre.on || d->activation != MMR_ACT_NONE;
+    bool direct = false, biased = false;
+    MMR_TRY(add_f32_bare(h.get(), d->math_mode, f32_mat(lhs), f32_mat(rhs), f32_mat(to), to_free, more ? nullptr : &bias,
+                         &q.x, &q.parts, &direct, &biased));
+    if (!direct || more || (bias.on && !biased)) {
+      q.pre = epi_mat(pre);
       q.residual = epi_mat(res);
       q.out = epi_mat(o);
       q.bias = reinterpret_cast<const float*>(bias.on ? bias.base : 0);
       q.bias_s = bias.s[2];
       q.m = int(m);
       q.n = int(n);
-      const int act = d->activation;
-      const int grid = int(std::min<int64_t>((m * ((n + 127) / 128) + 7) / 8, 16 * sms));
-      add_step(h.get(), "mmr_act_res_kernel grid %lld", [=](cudaStream_t s) {
-        using K = void (*)(const mmr::ActResParams);
-        const K k = pick_act(act, [](auto a) -> K { return mmr::mmr_act_res_kernel<decltype(a)::value>; });
-        return mmr::launch_kernel(k, dim3(grid), dim3(256), 0, s, dim3(1, 1, 1), q);
-      }, grid);
+      add_act_res(h.get(), d->activation, q);
     }
   } else {
     mmr::EpiParams epi;
@@ -986,22 +1152,32 @@ int32_t linear_grad_bind(const mmr_linear_grad_desc* d, Handle** out) {
   Ref dp;
   MMR_TRY(add_act_grad(h.get(), d->activation, dy, pre, db, &dp, nullptr, nullptr));
   if (dy.dtype == MMR_DTYPE_F32) {
-    mmr_view dpv = d->activation == MMR_ACT_NONE ? f32_view(dy, dev)
-                                                 : f32_view(reinterpret_cast<const void*>(dp.base), m, n, dp.s[1], dev);
     // out^T = B^T A^T where the gradient's unit stride is its row axis
-    auto product = [&](mmr_view a, mmr_view b, const Ref& o) -> int32_t {
+    auto product = [&](F32Mat a, F32Mat b, const Ref& o) -> int32_t {
       if (o.lo == o.hi) return MMR_OK;
-      mmr_view v = f32_view(o, dev);
-      if (o.s[2] != 1 && o.s[1] == 1) {
+      F32Mat v = f32_mat(o);
+      if (v.s_c != 1 && v.s_r == 1) {
         std::swap(a, b);
-        a = transposed(a);
-        b = transposed(b);
-        v = transposed(v);
+        a = a.t();
+        b = b.t();
+        v = v.t();
       }
-      return add_f32_product(h.get(), d->math_mode, a, b, v, nullptr, MMR_EPI_NONE);
+      mmr::ActResParams q;
+      bool direct = false, biased = false;
+      MMR_TRY(add_f32_bare(h.get(), d->math_mode, a, b, v, true, nullptr, &q.x, &q.parts, &direct, &biased));
+      if (direct) return MMR_OK;
+      q.out.p = reinterpret_cast<void*>(v.base);
+      q.out.ld = v.s_r;
+      q.out.cs = v.s_c;
+      q.out.vec = v.s_c == 1 && v.base % 16 == 0 && (v.s_r % 4 == 0 || v.rows == 1) && v.cols > 1;
+      q.m = int(v.rows);
+      q.n = int(v.cols);
+      add_act_res(h.get(), MMR_ACT_NONE, q);
+      return MMR_OK;
     };
-    if (dl.on) MMR_TRY(product(dpv, transposed(f32_view(rhs, dev)), dl));
-    if (dr.on) MMR_TRY(product(transposed(f32_view(lhs, dev)), dpv, dr));
+    const F32Mat dpm = f32_mat(dp);
+    if (dl.on) MMR_TRY(product(dpm, f32_mat(rhs).t(), dl));
+    if (dr.on) MMR_TRY(product(f32_mat(lhs).t(), dpm, dr));
   } else {
     if (dl.on) MMR_TRY(add_plain_product(h.get(), dy.dtype, operand(dp, true), operand(rhs, true), dl));
     if (dr.on) MMR_TRY(add_plain_product(h.get(), dy.dtype, operand(lhs, false), operand(dp, false), dr));

@@ -15,9 +15,10 @@ namespace mmr {
 // ----------------------------------------------------------------- pack --
 struct PackParams {
   const void* src = nullptr;
-  void* dst = nullptr;  // [batch][rows][pitch], columns past `cols` zeroed
+  void* dst = nullptr;  // [batch][rows_out][pitch], columns past `cols` zeroed
   long long s_b = 0, s_r = 0, s_c = 0;  // source strides (elements, signed)
   int rows = 0, cols = 0, pitch = 0, batch = 1;
+  int rows_out = 0;  // rows written; those from `rows` on are zeros
 };
 struct PackList {
   PackParams p[2];
@@ -41,22 +42,24 @@ __device__ __forceinline__ uint4 pack_load8(const unsigned short* src) {
   return v;
 }
 
-// Grid (blocks, operands, matrices). Rows that are contiguous in the source:
-// one 16-byte vector of the destination a thread (2.2 TB/s read and as much
-// written would be the copy's floor; element by element it ran at a sixth of
-// that). Other strides: 32 x 32 tiles through shared memory, the read running
-// along whichever source axis has the smaller stride.
+// Grid (blocks, operands, matrices). E: the element's bits. Rows that are
+// contiguous in the source: one 16-byte vector of the destination a thread, 4
+// TB/s (element by element it ran at a sixth of that). Other strides: 32 x 32
+// tiles through shared memory, the read running along whichever source axis has
+// the smaller stride.
+template <typename E>
 __global__ void __launch_bounds__(256) mmr_pack_kernel(const PackList list) {
-  __shared__ unsigned short tile[32][34];
+  constexpr int kPer = 16 / sizeof(E);
+  __shared__ E tile[32][33 + (sizeof(E) == 2)];
   griddep_wait();
   griddep_release();
   const PackParams p = blockIdx.y ? list.p[1] : list.p[0];
   if (static_cast<int>(blockIdx.z) >= p.batch) return;
-  const unsigned short* src = static_cast<const unsigned short*>(p.src) + blockIdx.z * p.s_b;
-  unsigned short* dst = static_cast<unsigned short*>(p.dst) + static_cast<long long>(blockIdx.z) * p.rows * p.pitch;
+  const E* src = static_cast<const E*>(p.src) + blockIdx.z * p.s_b;
+  E* dst = static_cast<E*>(p.dst) + static_cast<long long>(blockIdx.z) * p.rows_out * p.pitch;
   if (p.s_c == 1) {
-    const unsigned int vecs = p.pitch / 8;
-    const long long total = static_cast<long long>(p.rows) * vecs, step = gridDim.x * 256ll;
+    const unsigned int vecs = p.pitch / kPer;
+    const long long total = static_cast<long long>(p.rows_out) * vecs, step = gridDim.x * 256ll;
     for (long long i0 = blockIdx.x * 256ll + threadIdx.x; i0 < total; i0 += 4 * step) {
       uint4 v[4];
 #pragma unroll
@@ -64,14 +67,19 @@ __global__ void __launch_bounds__(256) mmr_pack_kernel(const PackList list) {
         const long long i = i0 + q * step;
         if (i >= total) continue;
         const long long r = i / vecs;
-        const int c = static_cast<int>(i - r * vecs) * 8;
-        const unsigned short* s = src + r * p.s_r + c;
-        if (c > 0 && c + 9 <= p.cols) {
-          v[q] = pack_load8(s);
-        } else {
-          unsigned short t[8];
+        const int c = static_cast<int>(i - r * vecs) * kPer;
+        const E* s = src + r * p.s_r + c;
+        bool done = false;
+        if constexpr (sizeof(E) == 2) {
+          if (r < p.rows && c > 0 && c + 9 <= p.cols) {
+            v[q] = pack_load8(s);
+            done = true;
+          }
+        }
+        if (!done) {
+          E t[kPer];
 #pragma unroll
-          for (int x = 0; x < 8; ++x) t[x] = c + x < p.cols ? s[x] : 0;
+          for (int x = 0; x < kPer; ++x) t[x] = r < p.rows && c + x < p.cols ? s[x] : E(0);
           memcpy(&v[q], t, 16);
         }
       }
@@ -85,13 +93,13 @@ __global__ void __launch_bounds__(256) mmr_pack_kernel(const PackList list) {
   const long long ar = p.s_r < 0 ? -p.s_r : p.s_r, ac = p.s_c < 0 ? -p.s_c : p.s_c;
   const bool along_rows = ar < ac;
   const int tiles_c = (p.pitch + 31) / 32;
-  const long long tiles = static_cast<long long>(tiles_c) * ((p.rows + 31) / 32);
+  const long long tiles = static_cast<long long>(tiles_c) * ((p.rows_out + 31) / 32);
   for (long long t = blockIdx.x; t < tiles; t += gridDim.x) {
     const int r0 = static_cast<int>(t / tiles_c) * 32, c0 = static_cast<int>(t % tiles_c) * 32;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int a = y + 8 * i, r = along_rows ? x : a, c = along_rows ? a : x;
-      unsigned short v = 0;
+      E v = 0;
       if (r0 + r < p.rows && c0 + c < p.cols) v = src[(r0 + r) * p.s_r + (c0 + c) * p.s_c];
       tile[r][c] = v;
     }
@@ -99,9 +107,74 @@ __global__ void __launch_bounds__(256) mmr_pack_kernel(const PackList list) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = y + 8 * i;
-      if (r0 + r < p.rows && c0 + x < p.pitch) dst[static_cast<long long>(r0 + r) * p.pitch + c0 + x] = tile[r][x];
+      if (r0 + r < p.rows_out && c0 + x < p.pitch) dst[static_cast<long long>(r0 + r) * p.pitch + c0 + x] = tile[r][x];
     }
     __syncthreads();
+  }
+}
+
+// ------------------------------------------------ f32 products of few rows --
+// x[m, n] = sum_k a[m, k] b[n, k] with b contiguous along k and at most eight
+// rows: a warp takes a row of b, read once, against all rows of a (which stay in
+// L1). Bound by b's bytes: 1 x 4096 x 4096 16.2 us with the pass after it, 4.1
+// TB/s out of L2. The MatMul node's streaming kernels want b row-major; its
+// tensor-core kernel took 184 us.
+struct DotParams {
+  const float *a = nullptr, *b = nullptr;
+  float* x = nullptr;
+  long long a_m = 0, a_k = 0, b_n = 0, x_m = 0, x_n = 0;
+  int m = 0, n = 0, k = 0;
+};
+
+// VEC: every row of a and b is 16-byte vectors (k a multiple of 4).
+template <int M, bool VEC>
+__global__ void __launch_bounds__(256) mmr_dot_kernel(const DotParams p) {
+  constexpr int kStep = VEC ? 4 : 1;  // k a lane takes at a time
+  constexpr int kFly = M <= 2 ? 4 : 2;
+  griddep_wait();
+  griddep_release();
+  const int lane = threadIdx.x & 31;
+  for (long long n = blockIdx.x * 8ll + (threadIdx.x >> 5); n < p.n; n += gridDim.x * 8ll) {
+    const float* b = p.b + n * p.b_n;
+    float s[M];
+#pragma unroll
+    for (int i = 0; i < M; ++i) s[i] = 0.0f;
+    for (int k0 = lane * kStep; k0 < p.k; k0 += 32 * kStep * kFly) {
+      float w[kFly][kStep];
+#pragma unroll
+      for (int q = 0; q < kFly; ++q) {
+        const int k = k0 + 32 * kStep * q;
+#pragma unroll
+        for (int e = 0; e < kStep; ++e) w[q][e] = 0.0f;
+        if (k >= p.k) continue;
+        if constexpr (VEC) *reinterpret_cast<float4*>(w[q]) = __ldcg(reinterpret_cast<const float4*>(b + k));
+        else w[q][0] = __ldcg(b + k);
+      }
+#pragma unroll
+      for (int q = 0; q < kFly; ++q) {
+        const int k = k0 + 32 * kStep * q;
+        if (k >= p.k) continue;
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+          if (i >= p.m) continue;
+          if constexpr (VEC) {
+            const float4 a = *reinterpret_cast<const float4*>(p.a + i * p.a_m + k);
+            s[i] = fmaf(a.x, w[q][0], s[i]);
+            s[i] = fmaf(a.y, w[q][1], s[i]);
+            s[i] = fmaf(a.z, w[q][2], s[i]);
+            s[i] = fmaf(a.w, w[q][3], s[i]);
+          } else {
+            s[i] = fmaf(p.a[i * p.a_m + k * p.a_k], w[q][0], s[i]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+#pragma unroll
+      for (int d = 16; d; d >>= 1) s[i] += __shfl_xor_sync(0xffffffffu, s[i], d);
+      if (lane == 0 && i < p.m) p.x[i * p.x_m + n * p.x_n] = s[i];
+    }
   }
 }
 
@@ -278,9 +351,10 @@ __global__ void __launch_bounds__(256) mmr_col_sum_kernel(const ColSumParams p) 
 // ------------------------------------- bias, activation and residual (f32) --
 // pre = x + bias; out = act(pre) + residual over a bare f32 product x, which may
 // lie in pre's or out's own storage (each element is read and written by one
-// thread). Bound by memory.
+// thread) or in the parts of a divided K, added in order. Bound by memory.
 struct ActResParams {
   EpiMat x, pre, residual, out;  // pre.p and residual.p may be null
+  int parts = 1;                 // x.bs apart
   const float* bias = nullptr;
   long long bias_s = 0;
   int m = 0, n = 0;
@@ -317,6 +391,11 @@ __global__ void __launch_bounds__(256) mmr_act_res_kernel(const ActResParams p) 
     if (vec && c0 + 128 <= p.n) {
       const int c = c0 + lane * 4;
       float4 v = *reinterpret_cast<const float4*>(x + row * p.x.ld + c);
+#pragma unroll 4
+      for (int q = 1; q < p.parts; ++q) {
+        const float4 y = *reinterpret_cast<const float4*>(x + q * p.x.bs + row * p.x.ld + c);
+        v = make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
+      }
       float4 r = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       if (res) r = *reinterpret_cast<const float4*>(res + row * p.residual.ld + c);
       if (p.bias) {
@@ -332,6 +411,7 @@ __global__ void __launch_bounds__(256) mmr_act_res_kernel(const ActResParams p) 
     } else {
       for (int c = c0 + lane; c < min(c0 + 128, p.n); c += 32) {
         float v = x[row * p.x.ld + c * p.x.cs];
+        for (int q = 1; q < p.parts; ++q) v += x[q * p.x.bs + row * p.x.ld + c * p.x.cs];
         if (p.bias) v = __fadd_rn(v, p.bias[c * p.bias_s]);
         if (pre) pre[row * p.pre.ld + c * p.pre.cs] = v;
         v = act_f32<ACT>(v);

@@ -411,3 +411,67 @@ def test_tf32_mode():
     node = mb.LinearNode(math_mode=mb.KernelMathMode.Tf32, accuracy=mb.AccuracyContract.AllowTf32)
     replay(mb.BoundLinear(node, V(lhs), V(rhs), V(out), residual=V(r)))
     assert rel(out, lhs.double() @ rhs.double() + r.double()) <= 2e-3
+
+
+F32_SHAPES = [(1, 64, 64), (1, 1001, 4096), (2, 130, 515), (3, 129, 1), (8, 300, 2048), (9, 515, 77), (16, 500, 4000),
+              (17, 512, 512), (100, 1000, 4000), (129, 77, 5000), (300, 515, 77), (260, 264, 4099), (1, 1, 1), (40, 1, 900)]
+
+
+@pytest.mark.parametrize("m,n,k", F32_SHAPES)
+@pytest.mark.parametrize("tl,tr", [(False, False), (False, True), (True, False)])
+def test_f32_layouts(m, n, k, tl, tr):
+    """Odd pitches, few rows, a long contraction over few tiles: each in both directions."""
+    g = gen(m + n + k)
+    lhs, rhs = rand(g, *((k, m) if tl else (m, k))), rand(g, *((n, k) if tr else (k, n)), scale=k ** -0.5)
+    b, r = rand(g, n), rand(g, m, n)
+    a64, b64 = (lhs.t() if tl else lhs).double(), (rhs.t() if tr else rhs).double()
+    node = mb.LinearNode(transpose_lhs=tl, transpose_rhs=tr)
+    out, pre = torch.full((m, n), float("nan"), device="cuda"), torch.full((m, n), float("nan"), device="cuda")
+    replay(mb.BoundLinear(node, V(lhs), V(rhs), V(out), bias=V(b)))
+    assert rel(out, a64 @ b64 + b.double()) <= 1e-5
+    replay(mb.BoundLinear(node, V(lhs), V(rhs), V(pre)))
+    assert rel(pre, a64 @ b64) <= 1e-5
+    replay(mb.BoundLinear(node, V(lhs), V(rhs), V(out), bias=V(b), residual=V(r), pre=V(pre)))
+    assert rel(out, a64 @ b64 + b.double() + r.double()) <= 1e-5
+    assert rel(pre, a64 @ b64 + b.double()) <= 1e-5
+    dy, d_lhs, d_rhs = rand(g, m, n), torch.full_like(lhs, float("nan")), torch.full_like(rhs, float("nan"))
+    replay(mb.BoundLinearGrad(node, V(dy), V(lhs), V(rhs), d_lhs=V(d_lhs), d_rhs=V(d_rhs)))
+    dy64 = dy.double()
+    assert rel(d_lhs.t() if tl else d_lhs, dy64 @ b64.t()) <= 1e-5
+    assert rel(d_rhs.t() if tr else d_rhs, a64.t() @ dy64) <= 1e-5
+
+
+@pytest.mark.parametrize("m", [4, 12, 200])
+def test_f32_views(m):
+    """Column blocks at odd offsets, reversed rows, a transposed output; what lies between them stays."""
+    g = gen(m)
+    n, k = 140, 2050
+    wide, weights = rand(g, 2 * m, k + 7), rand(g, n + 3, k + 5, scale=k ** -0.5)
+    lhs, rhs = wide[::2, 3:3 + k], weights[1:n + 1, 2:2 + k]
+    buf = torch.full((n, m + 3), 7.0, device="cuda")
+    out = buf[:, 1:m + 1].t()
+    replay(mb.BoundLinear(mb.LinearNode(transpose_rhs=True), V(lhs), V(rhs), V(out)))
+    assert rel(out, lhs.double() @ rhs.double().t()) <= 1e-5
+    assert bool((buf[:, 0] == 7).all()) and bool((buf[:, m + 1:] == 7).all())
+
+
+def test_f32_empty_contraction():
+    g = gen(15)
+    b, r = rand(g, 24), rand(g, 7, 24)
+    out = torch.empty(7, 24, device="cuda")
+    lhs, rhs = torch.empty(7, 0, device="cuda"), torch.empty(0, 24, device="cuda")
+    replay(mb.BoundLinear(mb.LinearNode(activation=ACT.RELU), V(lhs), V(rhs), V(out), bias=V(b), residual=V(r)))
+    assert torch.equal(out, b.relu() + r)
+
+
+@pytest.mark.parametrize("m,n,k", [(5, 64, 512), (100, 264, 4002)])
+def test_f32_infinities_stay_in_their_rows_and_columns(m, n, k):
+    g = gen(16)
+    lhs, rhs = rand(g, m, k), rand(g, n, k)
+    lhs[2, k - 1], rhs[7, 0] = float("inf"), float("nan")
+    out = torch.empty(m, n, device="cuda")
+    replay(mb.BoundLinear(mb.LinearNode(transpose_rhs=True), V(lhs), V(rhs), V(out)))
+    assert not bool(torch.isfinite(out[2]).any()) and bool(torch.isnan(out[:, 7]).all())
+    keep = torch.ones(m, n, dtype=torch.bool, device="cuda")
+    keep[2], keep[:, 7] = False, False
+    assert bool(torch.isfinite(out[keep]).all())
