@@ -206,16 +206,6 @@ __device__ __forceinline__ void epi_store8(const EpiParams& e, long long batch, 
   store8<T>(e.out, batch, row, col, e.n, v);
 }
 
-// The same for one element: what views without 16-byte vectors take, with
-// neighbouring lanes on neighbouring columns. `residual` is read by the caller.
-template <typename T>
-__device__ __forceinline__ void epi_store1(const EpiParams& e, long long batch, long long row, int col, float v,
-                                           float bias, float residual) {
-  float x[1] = {v + bias};
-  if (e.pre.p) static_cast<T*>(e.pre.p)[batch * e.pre.bs + row * e.pre.ld + col * e.pre.cs] = from_f32<T>(x[0]);
-  lact_apply(e.act, x);
-  static_cast<T*>(e.out.p)[batch * e.out.bs + row * e.out.ld + col * e.out.cs] = from_f32<T>(x[0] + residual);
-}
 // Four rows of C neighbouring columns: v[4 c + r]. C 2 wants every view's pairs
 // of columns on one 32-bit word (n even, and epi_vec). Rows from `rows` on are left out.
 template <typename T, int C>

@@ -38,7 +38,7 @@ constexpr int LS_MAX_SPLIT = 8;
 struct StripParams {
   int m = 0, n = 0;
   int k_blocks = 0;
-  int mt = 16;             // rows of x per unit (MMA N), a multiple of 16 up to 256
+  int mt = 16;             // rows of x per unit (MMA N), a multiple of 16 up to 128
   int strips = 0, m_units = 0;
   int split = 1;           // CTAs of a cluster: K slices
   int stages = 0;
