@@ -834,14 +834,40 @@ mmr_view f32_parts_view(const F32Mat& o, bool along_cols, int parts, int64_t eac
   return v;
 }
 
+// Up to eight rows against a K-contiguous b: one launch for all (1 x 4096 x 4096
+// 184 -> 15 us). False: not this kernel's case.
+bool add_f32_dot(Handle* h, int math, const F32Mat& a, const F32Mat& b, int act, const mmr::ActResParams& post) {
+  const int64_t m = a.rows, k = a.cols;
+  if (math == MMR_MATH_EXACT || m > 8 || (b.s_r != 1 && k != 1)) return false;
+  mmr::DotParams p;
+  p.a = reinterpret_cast<const float*>(a.base);
+  p.b = reinterpret_cast<const float*>(b.base);
+  p.a_m = a.s_r;
+  p.a_k = a.s_c;
+  p.b_n = b.s_c;
+  p.k = int(k);
+  p.act = act;
+  p.post = post;
+  const bool vec = k % 4 == 0 && b.base % 16 == 0 && b.s_c % 4 == 0 && a.s_c == 1 && a.base % 16 == 0 &&
+                   (a.s_r % 4 == 0 || m == 1);
+  using K = void (*)(const mmr::DotParams);
+  const K kernel = m == 1   ? (vec ? mmr::mmr_dot_kernel<1, true> : mmr::mmr_dot_kernel<1, false>)
+                   : m == 2 ? (vec ? mmr::mmr_dot_kernel<2, true> : mmr::mmr_dot_kernel<2, false>)
+                   : m <= 4 ? (vec ? mmr::mmr_dot_kernel<4, true> : mmr::mmr_dot_kernel<4, false>)
+                            : (vec ? mmr::mmr_dot_kernel<8, true> : mmr::mmr_dot_kernel<8, false>);
+  const int grid = int(std::min<int64_t>((b.cols + 7) / 8, 16 * h->sms));
+  add_step(h, "mmr_dot_kernel grid %lld", [=](cudaStream_t s) {
+    return mmr::launch_kernel(kernel, dim3(grid), dim3(256), 0, s, dim3(1, 1, 1), p);
+  }, grid);
+  return true;
+}
+
 // x = a b, bare, in f32: into `out` where that can hold it, else into a
 // workspace; *x says where, in *parts K parts that the reader adds. *direct: the
 // whole product lies in out. A bias that is all that follows the product may be
 // given; it is added in the node's epilogue, and *biased set, where *direct is.
 //
-// Up to eight rows against a K-contiguous b: the dot kernel (1 x 4096 x 4096 184
-// -> 16 us). Otherwise the MatMul node, with operands that TMA cannot read packed
-// first, and a K that is long for its few tiles divided into a batch of parts
+// The MatMul node, with operands that TMA cannot read packed first, and a K that is long for its few tiles divided into a batch of parts
 // (100 x 1000 x 8000: 347 -> 43 us; both, 500 x 77 x 5000: 732 -> 36 us). The parts'
 // number is the one of least estimated time: 0.42 us a 16-wide k-block on the
 // CTA-pair kernel, 0.72 on the one-CTA kernel (up to 128 rows).
@@ -894,34 +920,6 @@ int32_t add_f32_bare(Handle* h, int math, F32Mat a, F32Mat b, const F32Mat& out,
     if (out_free) use_out();
     else MMR_TRY(use_workspace(1));
     return node();
-  }
-  if (m <= 8 && (b.s_r == 1 || k == 1)) {
-    if (out_free) use_out();
-    else MMR_TRY(use_workspace(1));
-    mmr::DotParams p;
-    p.a = reinterpret_cast<const float*>(a.base);
-    p.b = reinterpret_cast<const float*>(b.base);
-    p.x = static_cast<float*>(x->p);
-    p.a_m = a.s_r;
-    p.a_k = a.s_c;
-    p.b_n = b.s_c;
-    p.x_m = x->ld;
-    p.x_n = x->cs;
-    p.m = int(m);
-    p.n = int(n);
-    p.k = int(k);
-    const bool vec = k % 4 == 0 && b.base % 16 == 0 && b.s_c % 4 == 0 && a.s_c == 1 && a.base % 16 == 0 &&
-                     (a.s_r % 4 == 0 || m == 1);
-    using K = void (*)(const mmr::DotParams);
-    const K kernel = m == 1   ? (vec ? mmr::mmr_dot_kernel<1, true> : mmr::mmr_dot_kernel<1, false>)
-                     : m == 2 ? (vec ? mmr::mmr_dot_kernel<2, true> : mmr::mmr_dot_kernel<2, false>)
-                     : m <= 4 ? (vec ? mmr::mmr_dot_kernel<4, true> : mmr::mmr_dot_kernel<4, false>)
-                              : (vec ? mmr::mmr_dot_kernel<8, true> : mmr::mmr_dot_kernel<8, false>);
-    const int grid = int(std::min<int64_t>((n + 7) / 8, 16 * h->sms));
-    add_step(h, "mmr_dot_kernel grid %lld", [=](cudaStream_t s) {
-      return mmr::launch_kernel(kernel, dim3(grid), dim3(256), 0, s, dim3(1, 1, 1), p);
-    }, grid);
-    return MMR_OK;
   }
   // The streaming kernels take few rows against a row-major b, and any a.
   const bool stream = m <= 16 && (b.s_c == 1 || n == 1);
@@ -1082,18 +1080,18 @@ int32_t linear_bind(const mmr_linear_desc* d, Handle** out) {
     const Ref& to = pre.on ? pre : o;
     const bool to_free = pre.on || !res.on || !overlap(o, res);
     const bool more = res.on || pre.on || d->activation != MMR_ACT_NONE;
-    bool direct = false, biased = false;
-    MMR_TRY(add_f32_bare(h.get(), d->math_mode, f32_mat(lhs), f32_mat(rhs), f32_mat(to), to_free, more ? nullptr : &bias,
-                         &q.x, &q.parts, &direct, &biased));
-    if (!direct || more || (bias.on && !biased)) {
-      q.pre = epi_mat(pre);
-      q.residual = epi_mat(res);
-      q.out = epi_mat(o);
-      q.bias = reinterpret_cast<const float*>(bias.on ? bias.base : 0);
-      q.bias_s = bias.s[2];
-      q.m = int(m);
-      q.n = int(n);
-      add_act_res(h.get(), d->activation, q);
+    q.pre = epi_mat(pre);
+    q.residual = epi_mat(res);
+    q.out = epi_mat(o);
+    q.bias = reinterpret_cast<const float*>(bias.on ? bias.base : 0);
+    q.bias_s = bias.s[2];
+    q.m = int(m);
+    q.n = int(n);
+    if (!add_f32_dot(h.get(), d->math_mode, f32_mat(lhs), f32_mat(rhs), d->activation, q)) {
+      bool direct = false, biased = false;
+      MMR_TRY(add_f32_bare(h.get(), d->math_mode, f32_mat(lhs), f32_mat(rhs), f32_mat(to), to_free,
+                           more ? nullptr : &bias, &q.x, &q.parts, &direct, &biased));
+      if (!direct || more || (bias.on && !biased)) add_act_res(h.get(), d->activation, q);
     }
   } else {
     mmr::EpiParams epi;
@@ -1163,16 +1161,16 @@ int32_t linear_grad_bind(const mmr_linear_grad_desc* d, Handle** out) {
         v = v.t();
       }
       mmr::ActResParams q;
-      bool direct = false, biased = false;
-      MMR_TRY(add_f32_bare(h.get(), d->math_mode, a, b, v, true, nullptr, &q.x, &q.parts, &direct, &biased));
-      if (direct) return MMR_OK;
       q.out.p = reinterpret_cast<void*>(v.base);
       q.out.ld = v.s_r;
       q.out.cs = v.s_c;
       q.out.vec = v.s_c == 1 && v.base % 16 == 0 && (v.s_r % 4 == 0 || v.rows == 1) && v.cols > 1;
       q.m = int(v.rows);
       q.n = int(v.cols);
-      add_act_res(h.get(), MMR_ACT_NONE, q);
+      if (add_f32_dot(h.get(), d->math_mode, a, b, MMR_ACT_NONE, q)) return MMR_OK;
+      bool direct = false, biased = false;
+      MMR_TRY(add_f32_bare(h.get(), d->math_mode, a, b, v, true, nullptr, &q.x, &q.parts, &direct, &biased));
+      if (!direct) add_act_res(h.get(), MMR_ACT_NONE, q);
       return MMR_OK;
     };
     const F32Mat dpm = f32_mat(dp);

@@ -113,71 +113,6 @@ __global__ void __launch_bounds__(256) mmr_pack_kernel(const PackList list) {
   }
 }
 
-// ------------------------------------------------ f32 products of few rows --
-// x[m, n] = sum_k a[m, k] b[n, k] with b contiguous along k and at most eight
-// rows: a warp takes a row of b, read once, against all rows of a (which stay in
-// L1). Bound by b's bytes: 1 x 16384 x 4096 41.9 us, 6.4 TB/s; 1 x 4096 x 4096
-// 16.2 us with the pass after it. The MatMul node's streaming kernels want b row-major; its
-// tensor-core kernel took 184 us.
-struct DotParams {
-  const float *a = nullptr, *b = nullptr;
-  float* x = nullptr;
-  long long a_m = 0, a_k = 0, b_n = 0, x_m = 0, x_n = 0;
-  int m = 0, n = 0, k = 0;
-};
-
-// VEC: every row of a and b is 16-byte vectors (k a multiple of 4).
-template <int M, bool VEC>
-__global__ void __launch_bounds__(256) mmr_dot_kernel(const DotParams p) {
-  constexpr int kStep = VEC ? 4 : 1;  // k a lane takes at a time
-  constexpr int kFly = M <= 2 ? 4 : 2;
-  griddep_wait();
-  griddep_release();
-  const int lane = threadIdx.x & 31;
-  for (long long n = blockIdx.x * 8ll + (threadIdx.x >> 5); n < p.n; n += gridDim.x * 8ll) {
-    const float* b = p.b + n * p.b_n;
-    float s[M];
-#pragma unroll
-    for (int i = 0; i < M; ++i) s[i] = 0.0f;
-    for (int k0 = lane * kStep; k0 < p.k; k0 += 32 * kStep * kFly) {
-      float w[kFly][kStep];
-#pragma unroll
-      for (int q = 0; q < kFly; ++q) {
-        const int k = k0 + 32 * kStep * q;
-#pragma unroll
-        for (int e = 0; e < kStep; ++e) w[q][e] = 0.0f;
-        if (k >= p.k) continue;
-        if constexpr (VEC) *reinterpret_cast<float4*>(w[q]) = __ldcg(reinterpret_cast<const float4*>(b + k));
-        else w[q][0] = __ldcg(b + k);
-      }
-#pragma unroll
-      for (int q = 0; q < kFly; ++q) {
-        const int k = k0 + 32 * kStep * q;
-        if (k >= p.k) continue;
-#pragma unroll
-        for (int i = 0; i < M; ++i) {
-          if (i >= p.m) continue;
-          if constexpr (VEC) {
-            const float4 a = *reinterpret_cast<const float4*>(p.a + i * p.a_m + k);
-            s[i] = fmaf(a.x, w[q][0], s[i]);
-            s[i] = fmaf(a.y, w[q][1], s[i]);
-            s[i] = fmaf(a.z, w[q][2], s[i]);
-            s[i] = fmaf(a.w, w[q][3], s[i]);
-          } else {
-            s[i] = fmaf(p.a[i * p.a_m + k * p.a_k], w[q][0], s[i]);
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < M; ++i) {
-#pragma unroll
-      for (int d = 16; d; d >>= 1) s[i] += __shfl_xor_sync(0xffffffffu, s[i], d);
-      if (lane == 0 && i < p.m) p.x[i * p.x_m + n * p.x_n] = s[i];
-    }
-  }
-}
-
 // ------------------------------------------------------------- act_grad --
 // Derivatives. 16-bit types take the fast forms of linear_epi.cuh, f32 CUDA's
 // math functions. The argument is clamped to +-1e4, where every derivative has
@@ -418,6 +353,91 @@ __global__ void __launch_bounds__(256) mmr_act_res_kernel(const ActResParams p) 
         if (res) v += res[row * p.residual.ld + c * p.residual.cs];
         out[row * p.out.ld + c * p.out.cs] = v;
       }
+    }
+  }
+}
+
+// ------------------------------------------------ f32 products of few rows --
+// pre = a b^T + bias; out = act(pre) + residual, b contiguous along k and a of at
+// most eight rows: a warp takes a row of b, read once, against all rows of a
+// (which stay in L1), and lane i finishes row i. Bound by b's bytes: 1 x 16384 x
+// 4096 41.9 us, 6.4 TB/s. The MatMul node's streaming kernels want b row-major;
+// its tensor-core kernel took 184 us at 1 x 4096 x 4096.
+struct DotParams {
+  const float *a = nullptr, *b = nullptr;
+  long long a_m = 0, a_k = 0, b_n = 0;
+  int k = 0, act = ACT_NONE;
+  ActResParams post;  // what follows the product; its x is not used
+};
+
+__device__ __forceinline__ float act_f32_any(int act, float x) {
+  switch (act) {
+    case ACT_RELU: return act_f32<ACT_RELU>(x);
+    case ACT_RELU6: return act_f32<ACT_RELU6>(x);
+    case ACT_SILU: return act_f32<ACT_SILU>(x);
+    case ACT_GELU_TANH: return act_f32<ACT_GELU_TANH>(x);
+    case ACT_GELU_ERF: return act_f32<ACT_GELU_ERF>(x);
+    default: return x;
+  }
+}
+
+// VEC: every row of a and b is 16-byte vectors (k a multiple of 4).
+template <int M, bool VEC>
+__global__ void __launch_bounds__(256) mmr_dot_kernel(const DotParams p) {
+  constexpr int kStep = VEC ? 4 : 1;  // k a lane takes at a time
+  constexpr int kFly = M <= 2 ? 4 : 2;
+  griddep_wait();
+  griddep_release();
+  const int lane = threadIdx.x & 31;
+  const ActResParams& e = p.post;
+  for (long long n = blockIdx.x * 8ll + (threadIdx.x >> 5); n < e.n; n += gridDim.x * 8ll) {
+    const float* b = p.b + n * p.b_n;
+    float s[M];
+#pragma unroll
+    for (int i = 0; i < M; ++i) s[i] = 0.0f;
+    for (int k0 = lane * kStep; k0 < p.k; k0 += 32 * kStep * kFly) {
+      float w[kFly][kStep];
+#pragma unroll
+      for (int q = 0; q < kFly; ++q) {
+        const int k = k0 + 32 * kStep * q;
+#pragma unroll
+        for (int c = 0; c < kStep; ++c) w[q][c] = 0.0f;
+        if (k >= p.k) continue;
+        if constexpr (VEC) *reinterpret_cast<float4*>(w[q]) = __ldcg(reinterpret_cast<const float4*>(b + k));
+        else w[q][0] = __ldcg(b + k);
+      }
+#pragma unroll
+      for (int q = 0; q < kFly; ++q) {
+        const int k = k0 + 32 * kStep * q;
+        if (k >= p.k) continue;
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+          if (i >= e.m) continue;
+          if constexpr (VEC) {
+            const float4 a = *reinterpret_cast<const float4*>(p.a + i * p.a_m + k);
+            s[i] = fmaf(a.x, w[q][0], s[i]);
+            s[i] = fmaf(a.y, w[q][1], s[i]);
+            s[i] = fmaf(a.z, w[q][2], s[i]);
+            s[i] = fmaf(a.w, w[q][3], s[i]);
+          } else {
+            s[i] = fmaf(p.a[i * p.a_m + k * p.a_k], w[q][0], s[i]);
+          }
+        }
+      }
+    }
+    float v = 0.0f;  // lane i: row i
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+#pragma unroll
+      for (int d = 16; d; d >>= 1) s[i] += __shfl_xor_sync(0xffffffffu, s[i], d);
+      if (lane == i) v = s[i];
+    }
+    if (lane < e.m) {
+      if (e.bias) v = __fadd_rn(v, e.bias[n * e.bias_s]);
+      if (e.pre.p) static_cast<float*>(e.pre.p)[lane * e.pre.ld + n * e.pre.cs] = v;
+      v = act_f32_any(p.act, v);
+      if (e.residual.p) v += static_cast<const float*>(e.residual.p)[lane * e.residual.ld + n * e.residual.cs];
+      static_cast<float*>(e.out.p)[lane * e.out.ld + n * e.out.cs] = v;
     }
   }
 }
