@@ -148,7 +148,8 @@ int32_t read_tensor(const mmr_tensor& t, const char* name, int device, int rank,
   r->es = elem_size(t.dtype);
   r->address = v.address;
   r->on = true;
-  int64_t lo = 0, hi = 0;
+  // 128 bits: an extent below 2^31 times a stride of up to 2^40 passes 64
+  __int128 lo = 0, hi = 0;
   bool empty = false;
   for (int i = 0; i < rank; ++i) {
     if (v.dims[i] < 0) return fail(MMR_ERR_INVALID_SHAPE, "%s: negative extent on axis %d", name, i);
@@ -162,7 +163,7 @@ int32_t read_tensor(const mmr_tensor& t, const char* name, int device, int rank,
       empty = true;
       continue;
     }
-    const int64_t reach = (v.dims[i] - 1) * v.strides[i];
+    const __int128 reach = __int128(v.dims[i] - 1) * v.strides[i];
     (reach < 0 ? lo : hi) += reach;
   }
   if (v.base_offset_bytes % r->es || v.address % r->es)
@@ -174,12 +175,12 @@ int32_t read_tensor(const mmr_tensor& t, const char* name, int device, int rank,
   r->lo = r->hi = r->base;
   if (!empty) {
     if (v.address == 0) return fail(MMR_ERR_INVALID_ARGUMENT, "%s: null address", name);
-    if (int64_t(v.base_offset_bytes / r->es) + lo < 0)
+    if (v.base_offset_bytes / r->es + lo < 0)
       return fail(MMR_ERR_OUT_OF_BOUNDS, "%s: a negative stride reaches before the buffer", name);
-    const uint64_t need = v.base_offset_bytes + uint64_t(hi + 1) * r->es;
-    if (need > v.bytes)
-      return fail(MMR_ERR_OUT_OF_BOUNDS, "%s: view needs %llu bytes but the buffer has %llu", name,
-                  (unsigned long long)need, (unsigned long long)v.bytes);
+    const __int128 need = v.base_offset_bytes + (hi + 1) * r->es;
+    if (need > v.bytes || need > UINT64_MAX - v.address)
+      return fail(MMR_ERR_OUT_OF_BOUNDS, "%s: view needs %.0f bytes but the buffer has %llu", name, double(need),
+                  (unsigned long long)v.bytes);
     r->lo = r->base + uint64_t(lo * r->es);
     r->hi = r->base + uint64_t((hi + 1) * r->es);
   }
@@ -227,10 +228,10 @@ int32_t check_output(const Ref& o) {
   for (int i = 0; i < 3; ++i)
     if (o.d[i] > 1) ax.emplace_back(o.s[i] < 0 ? -o.s[i] : o.s[i], o.d[i]);
   std::sort(ax.begin(), ax.end());
-  int64_t span = 1;
+  __int128 span = 1;
   for (const auto& [stride, extent] : ax) {
     if (stride < span) return fail(MMR_ERR_UNSAFE_ALIASING, "%s: the output's own elements overlap", o.name);
-    span += stride * (extent - 1);
+    span += __int128(stride) * (extent - 1);
   }
   return MMR_OK;
 }
