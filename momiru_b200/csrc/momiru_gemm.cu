@@ -108,13 +108,14 @@ struct Plan {
 };
 
 // Smallest and largest element offset a view reaches (strides may be
-// negative: a reversed axis); false when some extent is 0 (no element).
-bool view_span(const mmr_view& v, int64_t* lo, int64_t* hi) {
+// negative: a reversed axis); false when some extent is 0 (no element). In 128
+// bits: an extent below 2^31 times a stride of up to 2^40 passes 64.
+bool view_span(const mmr_view& v, __int128* lo, __int128* hi) {
   *lo = 0;
   *hi = 0;
   for (int i = 0; i < v.rank; ++i) {
     if (v.dims[i] == 0) return false;
-    const int64_t reach = (v.dims[i] - 1) * v.strides[i];
+    const __int128 reach = __int128(v.dims[i] - 1) * v.strides[i];
     if (reach < 0) *lo += reach; else *hi += reach;
   }
   return true;
@@ -139,17 +140,17 @@ int32_t check_view(const mmr_view& v, const char* name, int32_t device, bool all
     return fail(MMR_ERR_UNSUPPORTED_LAYOUT, "%s: base offset %llu is not f32-aligned", name,
                 (unsigned long long)v.base_offset_bytes);
   if (v.address % 4 != 0) return fail(MMR_ERR_UNSUPPORTED_LAYOUT, "%s: address is not f32-aligned", name);
-  int64_t lo = 0, hi = 0;
+  __int128 lo = 0, hi = 0;
   if (view_span(v, &lo, &hi)) {
     if (v.address == 0) return fail(MMR_ERR_INVALID_ARGUMENT, "%s: null address", name);
-    const int64_t first = int64_t(v.base_offset_bytes / 4) + lo;
+    const __int128 first = v.base_offset_bytes / 4 + lo;
     if (first < 0)
-      return fail(MMR_ERR_OUT_OF_BOUNDS, "%s: a negative stride reaches %lld elements before the buffer", name,
-                  (long long)-first);
-    const uint64_t need = v.base_offset_bytes + uint64_t(hi + 1) * 4u;
-    if (need > v.bytes)
-      return fail(MMR_ERR_OUT_OF_BOUNDS, "%s: view needs %llu bytes but the buffer has %llu", name,
-                  (unsigned long long)need, (unsigned long long)v.bytes);
+      return fail(MMR_ERR_OUT_OF_BOUNDS, "%s: a negative stride reaches %.0f elements before the buffer", name,
+                  double(-first));
+    const __int128 need = v.base_offset_bytes + (hi + 1) * 4;
+    if (need > v.bytes || need > UINT64_MAX - v.address)
+      return fail(MMR_ERR_OUT_OF_BOUNDS, "%s: view needs %.0f bytes but the buffer has %llu", name, double(need),
+                  (unsigned long long)v.bytes);
   }
   if (v.device_ordinal != device)
     return fail(MMR_ERR_UNSUPPORTED_DEVICE, "%s: device ordinal %d differs from the node's %d", name,
@@ -167,7 +168,7 @@ bool broadcast_extent(int64_t l, int64_t r, int64_t* out) {
 }
 
 void set_range(Operand& o, const mmr_view& v) {
-  int64_t lo = 0, hi = 0;
+  __int128 lo = 0, hi = 0;
   const uint64_t at = v.address + v.base_offset_bytes;
   if (view_span(v, &lo, &hi)) {
     o.lo = at + uint64_t(lo * 4);  // wraps correctly for lo < 0 (bounds checked)
@@ -1788,7 +1789,7 @@ int32_t mmr_gemm_bind_host(const mmr_matmul_desc* d, int32_t panels, mmr_gemm_ha
     if (rows < 0 || cols < 0 || v.strides[v.rank - 1] != 1 || (v.rank == 2 && rows > 1 && pitch < cols))
       return fail(MMR_ERR_UNSUPPORTED_LAYOUT, "%s: host buffer must be row-major with unit column stride", name);
     if (v.base_offset_bytes % 4) return fail(MMR_ERR_UNSUPPORTED_LAYOUT, "%s: base offset not f32-aligned", name);
-    const uint64_t need = rows && cols ? uint64_t((rows - 1) * pitch + cols) * 4u : 0u;
+    const __int128 need = rows && cols ? (__int128(rows - 1) * pitch + cols) * 4 : 0;
     if (v.base_offset_bytes + need > v.bytes) return fail(MMR_ERR_INVALID_SHAPE, "%s: view exceeds its host buffer", name);
     if (need && !v.address) return fail(MMR_ERR_INVALID_ARGUMENT, "%s: null host address", name);
     cudaPointerAttributes a{};

@@ -2,9 +2,12 @@
 multiplied or added: refused as out of bounds, not taken for the wrapped value.
 Nothing here needs a GPU (a view that passed would stop at the missing or
 foreign device instead, with another error)."""
+import ctypes
+
 import pytest
 
 import momiru_b200 as mb
+from momiru_b200 import _abi
 from momiru_b200.execution import OutOfBounds
 
 pytestmark = pytest.mark.usefixtures("cuda_lib")
@@ -53,3 +56,40 @@ def test_operators_refuse_buffers_past_the_address_space():
     ops["lhs"] = view((1 << 64) - 64, (8, 8), (8, 1), 128)
     with pytest.raises(OutOfBounds):
         mb.BoundLinear(mb.LinearNode(), **ops)
+
+
+@pytest.mark.parametrize("name", ["lhs", "out"])
+@pytest.mark.parametrize("rows,stride", [(WRAP, 1 << 40), (WRAP + 1, 1 << 40), (WRAP, -(1 << 40)), (1 << 25, 1 << 39)])
+def test_node_refuses_strides_that_wrap(name, rows, stride):
+    ops = strided(name, rows, stride, F32)
+    with pytest.raises(OutOfBounds):
+        mb.validate(mb.MatMulNode(), ops["lhs"], ops["rhs"], ops["out"])
+
+
+@pytest.mark.parametrize("name", ["lhs", "rhs", "out"])
+@pytest.mark.parametrize("offset", [-1, -8, -(1 << 30), (1 << 62) - 1])
+def test_node_refuses_offsets_that_wrap(name, offset):
+    ops = operands(8, F32)
+    ops[name] = view(4 << 44, (8, 8), (8, 1), 1 << 20, offset, F32)
+    with pytest.raises(OutOfBounds):
+        mb.validate(mb.MatMulNode(), ops["lhs"], ops["rhs"], ops["out"])
+
+
+def test_node_refuses_batches_that_wrap():
+    """2^24 + 1 matrices 2^40 elements apart."""
+    ops = operands(8, F32)
+    lhs = view(4 << 44, (WRAP, 8, 8), (1 << 40, 8, 1), 256, dtype=F32)
+    out = view(5 << 44, (WRAP, 8, 8), (64, 8, 1), WRAP * 256, dtype=F32)
+    with pytest.raises(OutOfBounds):
+        mb.validate(mb.MatMulNode(), lhs, ops["rhs"], out)
+
+
+def test_host_entry_refuses_pitches_that_wrap():
+    """2^31 + 1 rows, 2^31 elements apart."""
+    lib = _abi.load()
+    ops = operands(8, F32)
+    d = _abi.MmrMatmulDesc()
+    d.lhs, d.rhs, d.out = (ops[n].to_abi() for n in ("lhs", "rhs", "out"))
+    d.lhs.dims[0], d.lhs.strides[0], d.lhs.bytes = (1 << 31) + 1, 1 << 31, 32  # (rows - 1) * pitch * 4 is 2^64
+    h = ctypes.c_void_p()
+    assert lib.mmr_gemm_bind_host(ctypes.byref(d), 0, ctypes.byref(h)) == _abi.ERR_INVALID_SHAPE
