@@ -13,8 +13,10 @@
  *   mmr_<operator>_bind  ->  mmr_op_run / mmr_op_run_on  ->  mmr_op_quiesce  ->  mmr_op_destroy
  *
  * A handle's runs are ordered one after another whichever streams they are
- * given (a workspace belongs to its handle). Under stream capture the caller
- * orders the graph's launches; quiesce then reports only the error word.
+ * given, cudaStreamPerThread among them (a workspace belongs to its handle), and
+ * may come from several host threads, as may quiesce; destroy follows them all.
+ * Under stream capture the caller orders the graph's launches; quiesce then
+ * reports only the error word.
  */
 #ifndef MOMIRU_OPS_H
 #define MOMIRU_OPS_H

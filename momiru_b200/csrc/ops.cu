@@ -51,6 +51,8 @@ struct mmr_op_handle {
   cudaEvent_t done = nullptr, err_ev = nullptr;
   bool ran = false;       // `done` was recorded (a run outside stream capture)
   bool launched = false;
+  std::mutex run_mu;      // one run's wait, launches and record at a time; guards the two flags and last_stream
+  std::mutex quiesce_mu;  // the pinned error word and its event
 };
 
 namespace {
@@ -1574,27 +1576,41 @@ int32_t poll_event(cudaEvent_t ev, uint64_t timeout_ns) {
 }
 
 int32_t run_on(Handle* h, cudaStream_t s) {
+  std::lock_guard<std::mutex> lock(h->run_mu);
   DeviceGuard guard(h->device);
   if (!guard.ok) return fail(MMR_ERR_CUDA, "cudaSetDevice(%d) failed", h->device);
   cudaStreamCaptureStatus cap = cudaStreamCaptureStatusNone;
   MMR_CUDA(cudaStreamIsCapturing(s, &cap));
   const bool capturing = cap != cudaStreamCaptureStatusNone;
-  // The workspaces are the handle's own: a run on another stream follows the last.
-  if (!capturing && h->ran && s != h->last_stream) MMR_CUDA(cudaStreamWaitEvent(s, h->done, 0));
-  for (const auto& step : h->steps) MMR_TRY(step.launch(s));
+  // The workspaces are the handle's own: a run follows the last. Only the legacy
+  // default stream is known by its value to be the stream of the last run: any
+  // other value may have been destroyed and given out again, and
+  // cudaStreamPerThread is another stream in every thread.
+  if (!capturing && h->ran && (s != nullptr || h->last_stream != nullptr)) MMR_CUDA(cudaStreamWaitEvent(s, h->done, 0));
+  int32_t rc = MMR_OK;
+  for (const auto& step : h->steps)
+    if ((rc = step.launch(s))) break;
   h->launched = true;
-  if (!capturing) {
+  if (!capturing) {  // also after a failed launch: those before it use the workspaces
     MMR_CUDA(cudaEventRecord(h->done, s));
     h->ran = true;
     h->last_stream = s;
   }
-  return MMR_OK;
+  return rc;
 }
 
 int32_t quiesce(Handle* h, uint64_t timeout_ns) {
-  if (!h->launched) return MMR_OK;
+  std::lock_guard<std::mutex> lock(h->quiesce_mu);
+  bool ran = false, launched = false;
+  {
+    std::lock_guard<std::mutex> run_lock(h->run_mu);
+    ran = h->ran;
+    launched = h->launched;
+  }
+  if (!launched) return MMR_OK;
   DeviceGuard guard(h->device);
-  if (h->ran) MMR_TRY(poll_event(h->done, timeout_ns));
+  if (!guard.ok) return fail(MMR_ERR_CUDA, "cudaSetDevice(%d) failed", h->device);
+  if (ran) MMR_TRY(poll_event(h->done, timeout_ns));
   for (mmr_gemm_handle* g : h->products) MMR_TRY(mmr::gemm_read_error(g, timeout_ns));
   MMR_CUDA(cudaMemcpyAsync(h->h_err, h->d_err, sizeof(int), cudaMemcpyDeviceToHost, h->stream));
   MMR_CUDA(cudaEventRecord(h->err_ev, h->stream));

@@ -57,8 +57,9 @@ def _fill(desc, device_ordinal: int, stream: int | None, **views: DeviceView | N
 
 class BoundOp:
     """A bound operator: replay enqueues it, quiesce_or_abort waits for it and
-    reports a kernel's error, close releases it. The views (and so their
-    buffers) are kept alive until then."""
+    reports a kernel's error, close releases it. Runs follow one another
+    whatever streams and host threads they come from. The views (and so their
+    buffers) are kept alive until close."""
 
     def __init__(self, bind: str, desc, views):
         self._lib = _ops_abi.load()
