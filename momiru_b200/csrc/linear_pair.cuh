@@ -80,8 +80,11 @@ struct PairParams {
 };
 
 // Rows of each of `tiles` equal tiles of `rows` rows; tiles = ceil(rows / 256),
-// so every tile but the last is full and the last has at least one row.
-__host__ __device__ inline int lp_tile_rows(int rows, int tiles) { return ((rows + tiles - 1) / tiles + 31) / 32 * 32; }
+// so every tile but the last is full and the last has at least one row. No sum
+// passes 32 bits at the largest extent admitted, 2^31 - 1024 rows.
+__host__ __device__ constexpr int lp_tile_rows(int rows, int tiles) { return ((rows - 1) / tiles + 32) / 32 * 32; }
+static_assert(lp_tile_rows(2147482624, 8388604) == 256 && lp_tile_rows(300, 2) == 160 && lp_tile_rows(1, 1) == 32,
+              "rows of a tile");
 
 // One piece of work, found from its index.
 struct LpTile {
