@@ -67,7 +67,7 @@ static_assert(lp_smem_bytes(0) <= 232448 && lp_smem_bytes(1) <= 232448, "shared 
 
 struct PairParams {
   int m = 0, n = 0;
-  int tiles_m = 0, tiles_n = 0, tiles_total = 0;  // RAG 1: tiles_n only
+  int tiles_m = 0, tiles_n = 0, tiles_total = 0;  // RAG 1: tiles_n, and the most tiles any layout has
   int tile_rows = 256;                            // rows of a tile, a multiple of 32 (RAG 1: by expert)
   int k_blocks = 0;                               // RAG 2: from the counts
   int experts = 0;
@@ -230,11 +230,11 @@ __global__ void __launch_bounds__(LP_THREADS, 1)
         if (lane >= d) incl += up;
       }
       if (e < p.experts) {
-        first[e] = base + incl - own;
+        first[e] = min(base + incl - own, p.tiles_total);
         off[e] = o;
         cnt[e] = c;
       }
-      base += __shfl_sync(0xffffffffu, incl, 31);
+      base = min(base + __shfl_sync(0xffffffffu, incl, 31), p.tiles_total);  // no layout of a sort has more tiles
     }
     if (lane == 0) {
       first[p.experts] = base;

@@ -68,27 +68,29 @@ __device__ __forceinline__ void st_async_f4(uint32_t addr, uint32_t bar, uint32_
 }
 
 // Expert and first row of unit `unit` when each expert with c tokens has
-// ceil(c / mt) units; false when there are fewer units. One warp.
+// ceil(c / mt) units; false when there are fewer units. One warp. The counts are
+// data: sums stop at LS_UNITS_END, above every unit's number, so that none wraps.
+constexpr int LS_UNITS_END = 1 << 29;
 __device__ __forceinline__ bool find_expert_unit(const int* counts, int experts, int mt, int unit, int lane, int* expert,
                                                  int* local) {
   int base = 0;
   for (int e0 = 0; e0 < experts; e0 += 32) {
     const int c = e0 + lane < experts ? max(counts[e0 + lane], 0) : 0;
-    const int units = (c + mt - 1) / mt;
-    int incl = units;
+    int incl = c > 0 ? (c - 1) / mt + 1 : 0;
 #pragma unroll
     for (int d = 1; d < 32; d <<= 1) {
       const int up = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += up;
+      if (lane >= d) incl = min(incl + up, LS_UNITS_END);
     }
     const unsigned hit = __ballot_sync(0xffffffffu, base + incl > unit);
     if (hit) {
       const int l = __ffs(hit) - 1;
+      const int before = __shfl_sync(0xffffffffu, incl, max(l - 1, 0));
       *expert = e0 + l;
-      *local = unit - base - __shfl_sync(0xffffffffu, incl - units, l);
+      *local = unit - base - (l ? before : 0);
       return true;
     }
-    base += __shfl_sync(0xffffffffu, incl, 31);
+    base = min(base + __shfl_sync(0xffffffffu, incl, 31), LS_UNITS_END);
   }
   return false;
 }
@@ -177,7 +179,7 @@ __global__ void __launch_bounds__(LS_THREADS, 3)
       const int local = unit_info[1], count = p.counts[expert];
       row0 = max(p.offsets[expert], 0) + static_cast<long long>(local) * p.mt;
       valid = static_cast<int>(max(0ll, min(static_cast<long long>(min(p.mt, count - local * p.mt)), p.rows - row0)));
-      if ((local + 1) * p.mt >= count) zero_end = min(static_cast<long long>(p.offsets[expert + 1]), p.rows);
+      if (count - local * p.mt <= p.mt) zero_end = min(static_cast<long long>(p.offsets[expert + 1]), p.rows);
     }
   }
   const int kb0 = static_cast<int>(static_cast<long long>(p.k_blocks) * rank / p.split);
