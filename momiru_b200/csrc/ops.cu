@@ -218,6 +218,9 @@ bool overlap(const Ref& x, const Ref& y) {
   }
   return true;
 }
+// Whether the bytes from one operand's first element to its last lie apart from
+// the other's: what the MatMul node asks of its output.
+bool apart(const Ref& x, const Ref& y) { return x.lo >= x.hi || y.lo >= y.hi || x.lo >= y.hi || y.lo >= x.hi; }
 bool same_view(const Ref& x, const Ref& y) {
   return x.base == y.base && x.rank == y.rank && memcmp(x.d, y.d, sizeof x.d) == 0 && memcmp(x.s, y.s, sizeof x.s) == 0;
 }
@@ -1081,7 +1084,7 @@ int32_t linear_bind(const mmr_linear_desc* d, Handle** out) {
     // bias and SiLU took 375 us in it, 256 bare.
     mmr::ActResParams q;
     const Ref& to = pre.on ? pre : o;
-    const bool to_free = pre.on || !res.on || !overlap(o, res);
+    const bool to_free = (pre.on || !res.on || !overlap(o, res)) && apart(to, lhs) && apart(to, rhs);
     const bool more = res.on || pre.on || d->activation != MMR_ACT_NONE;
     q.pre = epi_mat(pre);
     q.residual = epi_mat(res);
@@ -1154,8 +1157,9 @@ int32_t linear_grad_bind(const mmr_linear_grad_desc* d, Handle** out) {
   MMR_TRY(add_act_grad(h.get(), d->activation, dy, pre, db, &dp, nullptr, nullptr));
   if (dy.dtype == MMR_DTYPE_F32) {
     // out^T = B^T A^T where the gradient's unit stride is its row axis
-    auto product = [&](F32Mat a, F32Mat b, const Ref& o) -> int32_t {
+    auto product = [&](F32Mat a, F32Mat b, const Ref& o, const Ref& operand) -> int32_t {
       if (o.lo == o.hi) return MMR_OK;
+      const bool free = apart(o, dy) && apart(o, operand);
       F32Mat v = f32_mat(o);
       if (v.s_c != 1 && v.s_r == 1) {
         std::swap(a, b);
@@ -1172,13 +1176,13 @@ int32_t linear_grad_bind(const mmr_linear_grad_desc* d, Handle** out) {
       q.n = int(v.cols);
       if (add_f32_dot(h.get(), d->math_mode, a, b, MMR_ACT_NONE, q)) return MMR_OK;
       bool direct = false, biased = false;
-      MMR_TRY(add_f32_bare(h.get(), d->math_mode, a, b, v, true, nullptr, &q.x, &q.parts, &direct, &biased));
+      MMR_TRY(add_f32_bare(h.get(), d->math_mode, a, b, v, free, nullptr, &q.x, &q.parts, &direct, &biased));
       if (!direct) add_act_res(h.get(), MMR_ACT_NONE, q);
       return MMR_OK;
     };
     const F32Mat dpm = f32_mat(dp);
-    if (dl.on) MMR_TRY(product(dpm, f32_mat(rhs).t(), dl));
-    if (dr.on) MMR_TRY(product(f32_mat(lhs).t(), dpm, dr));
+    if (dl.on) MMR_TRY(product(dpm, f32_mat(rhs).t(), dl, rhs));
+    if (dr.on) MMR_TRY(product(f32_mat(lhs).t(), dpm, dr, lhs));
   } else {
     if (dl.on) MMR_TRY(add_plain_product(h.get(), dy.dtype, operand(dp, true), operand(rhs, true), dl));
     if (dr.on) MMR_TRY(add_plain_product(h.get(), dy.dtype, operand(lhs, false), operand(dp, false), dr));
