@@ -218,9 +218,6 @@ bool overlap(const Ref& x, const Ref& y) {
   }
   return true;
 }
-// Whether the bytes from one operand's first element to its last lie apart from
-// the other's: what the MatMul node asks of its output.
-bool apart(const Ref& x, const Ref& y) { return x.lo >= x.hi || y.lo >= y.hi || x.lo >= y.hi || y.lo >= x.hi; }
 bool same_view(const Ref& x, const Ref& y) {
   return x.base == y.base && x.rank == y.rank && memcmp(x.d, y.d, sizeof x.d) == 0 && memcmp(x.s, y.s, sizeof x.s) == 0;
 }
@@ -777,13 +774,15 @@ mmr_view f32_view(const void* p, int64_t rows, int64_t cols, int64_t ld, int dev
 // / 323 us at 2048 x 4096 x 4096. A layer's f32 sums are kept below 1e-6.
 constexpr int kF32Chunk = 64;
 
-int32_t add_f32_product(Handle* h, int math, const mmr_view& lhs, const mmr_view& rhs, const mmr_view& out,
-                        const Ref* bias, int epilogue) {
+mmr_matmul_desc f32_desc(const Handle* h, int math, const mmr_view& lhs, const mmr_view& rhs, const mmr_view& out,
+                         const Ref* bias) {
   mmr_matmul_desc d{};
   d.lhs = lhs;
   d.rhs = rhs;
   d.out = out;
+  d.epilogue = MMR_EPI_NONE;
   if (bias && bias->on) {
+    d.epilogue = MMR_EPI_BIAS;
     d.bias.address = bias->lo;
     d.bias.bytes = bias->hi - bias->lo;
     d.bias.base_offset_bytes = bias->base - bias->lo;
@@ -793,16 +792,25 @@ int32_t add_f32_product(Handle* h, int math, const mmr_view& lhs, const mmr_view
     d.bias.strides[0] = bias->s[2];
   }
   d.math_mode = math;
-  d.epilogue = epilogue;
   d.family = MMR_FAMILY_AUTO;
   d.device_ordinal = h->device;
   d.stream = h->stream;
+  return d;
+}
+
+int32_t add_f32_product(Handle* h, const mmr_matmul_desc& d) {
   mmr_gemm_handle* g = nullptr;
   MMR_TRY(mmr_gemm_bind(&d, &g));
   h->products.push_back(g);
   mmr::gemm_set_chunk(g, kF32Chunk);
-  h->plan += "matmul node (f32)\n";
-  h->steps.push_back({"matmul node (f32)", [g](cudaStream_t s) { return mmr::gemm_enqueue(g, s); }});
+  mmr_gemm_info info{};
+  MMR_TRY(mmr_gemm_query(g, &info));
+  const char* what = info.family == MMR_FAMILY_TCGEN05 ? "matmul node (f32, tcgen05)"
+                     : info.family == MMR_FAMILY_GEMV  ? "matmul node (f32, gemv)"
+                                                       : "matmul node (f32, simt)";
+  h->plan += what;
+  h->plan += "\n";
+  h->steps.push_back({what, [g](cudaStream_t s) { return mmr::gemm_enqueue(g, s); }});
   return MMR_OK;
 }
 
@@ -814,12 +822,18 @@ struct F32Mat {
 };
 F32Mat f32_mat(const Ref& r) { return {r.base, r.d[1], r.d[2], r.s[1], r.s[2]}; }
 
+// The same matrix with strides that TMA takes on axes of extent 1, whose strides
+// say nothing.
+F32Mat f32_plain(F32Mat o) {
+  if (o.rows == 1) o.s_r = ((o.cols - 1) * std::abs(o.s_c) + 4) / 4 * 4;
+  if (o.cols == 1) o.s_c = o.rows > 1 && o.s_r == 1 ? (o.rows + 3) / 4 * 4 : 1;
+  return o;
+}
+
 // As TMA wants it: one axis contiguous, the other a pitch of whole 16 bytes.
 bool f32_aligned(const F32Mat& o) {
-  auto ok = [&](int64_t unit, int64_t extent, int64_t pitch, int64_t other) {
-    return (unit == 1 || extent == 1) && (other == 1 || (pitch > 0 && pitch % 4 == 0 && pitch >= extent));
-  };
-  return o.base % 16 == 0 && (ok(o.s_c, o.cols, o.s_r, o.rows) || ok(o.s_r, o.rows, o.s_c, o.cols));
+  auto pitch = [](int64_t s, int64_t extent) { return s % 4 == 0 && s >= extent; };
+  return o.base % 16 == 0 && ((o.s_c == 1 && pitch(o.s_r, o.cols)) || (o.s_r == 1 && pitch(o.s_c, o.rows)));
 }
 
 // A batch of `parts` views along the contraction of a (axis `cols`) or b (`rows`).
@@ -871,16 +885,26 @@ bool add_f32_dot(Handle* h, int math, const F32Mat& a, const F32Mat& b, int act,
 // x = a b, bare, in f32: into `out` where that can hold it, else into a
 // workspace; *x says where, in *parts K parts that the reader adds. *direct: the
 // whole product lies in out. A bias that is all that follows the product may be
-// given; it is added in the node's epilogue, and *biased set, where *direct is.
+// given; *biased: the node's epilogue adds it.
 //
-// The MatMul node, with operands that TMA cannot read packed first, and a K that is long for its few tiles divided into a batch of parts
-// (100 x 1000 x 8000: 347 -> 43 us; both, 500 x 77 x 5000: 732 -> 36 us). The parts'
+// The MatMul node, whose own admission decides its kernel for these views: the
+// streaming ones where they take the operands, else the tensor-core ones, with
+// operands that TMA cannot read packed first, an output or a bias that would send
+// the whole product to the scalar kernel left to the pass that follows, and a K
+// that is long for its few tiles divided into a batch of parts. The streaming
+// kernels end at a K of 8192 (16 x 500 x 8193: 1823 us and 1.6e-6 on the scalar
+// kernel, 55 us and 7.8e-7 in parts). 100 x 1000 x 8000: 347 -> 43 us; packed as
+// well, 500 x 77 x 5000: 732 -> 36 us. The parts'
 // number is the one of least estimated time: 0.42 us a 16-wide k-block on the
 // CTA-pair kernel, 0.72 on the one-CTA kernel (up to 128 rows).
-int32_t add_f32_bare(Handle* h, int math, F32Mat a, F32Mat b, const F32Mat& out, bool out_free, const Ref* bias,
-                     EpiMat* x, int* parts, bool* direct, bool* biased) {
+int32_t add_f32_bare(Handle* h, int math, F32Mat a, F32Mat b, F32Mat out, bool out_free, const Ref* bias, EpiMat* x,
+                     int* parts, bool* direct, bool* biased) {
   const int64_t m = a.rows, k = a.cols, n = b.cols;
   const int dev = h->device;
+  a = f32_plain(a);
+  b = f32_plain(b);
+  out = f32_plain(out);
+  if (n == 1) out.s_c = 1;  // its rows keep their pitch
   auto use_out = [&] {
     x->p = reinterpret_cast<void*>(out.base);
     x->ld = out.s_r;
@@ -908,11 +932,20 @@ int32_t add_f32_bare(Handle* h, int math, F32Mat a, F32Mat b, const F32Mat& out,
     const int64_t hi = std::max<int64_t>(0, (o.rows - 1) * o.s_r) + std::max<int64_t>(0, (o.cols - 1) * o.s_c);
     return f32_view(o.base, o.rows, o.cols, o.s_r, o.s_c, dev, o.base + 4 * lo, o.base + 4 * (hi + 1));
   };
-  auto x_view = [&] { return f32_view(x->p, m, n, x->ld, dev); };
-  auto node = [&] {
-    *biased = *direct && bias && bias->on;
-    return add_f32_product(h, math, plain_view(a), plain_view(b), *direct ? plain_view(out) : x_view(),
-                           *biased ? bias : nullptr, *biased ? MMR_EPI_BIAS : MMR_EPI_NONE);
+  // The family that the node takes for out = a b (+ bias); -1: none.
+  auto family = [&](const F32Mat& a, const F32Mat& b, const F32Mat& out, const Ref* bias) {
+    const mmr_matmul_desc d = f32_desc(h, math, plain_view(a), plain_view(b), plain_view(out), bias);
+    mmr_gemm_info info{};
+    return mmr_gemm_validate(&d, &info) == MMR_OK ? int(info.family) : -1;
+  };
+  // Row-major stand-ins at addresses that meet nothing, for a matrix still to be packed or allocated.
+  const F32Mat packed_b = {uint64_t(1) << 60, k, n, (n + 3) / 4 * 4, 1}, own_out = {uint64_t(1) << 61, m, n, (n + 3) / 4 * 4, 1};
+  auto node = [&](int want) -> int32_t {
+    if (out_free && family(a, b, out, nullptr) == want) use_out();
+    else MMR_TRY(use_workspace(1));
+    *biased = *direct && bias && bias->on && family(a, b, out, bias) == want;
+    return add_f32_product(h, f32_desc(h, math, plain_view(a), plain_view(b),
+                                       *direct ? plain_view(out) : f32_view(x->p, m, n, x->ld, dev), *biased ? bias : nullptr));
   };
   *biased = false;
   if (k == 0) {
@@ -922,13 +955,8 @@ int32_t add_f32_bare(Handle* h, int math, F32Mat a, F32Mat b, const F32Mat& out,
     add_step(h, "zeros", [=](cudaStream_t s) { return cudaMemsetAsync(w, 0, bytes, s); });
     return MMR_OK;
   }
-  if (math == MMR_MATH_EXACT) {  // sums in the node's own order
-    if (out_free) use_out();
-    else MMR_TRY(use_workspace(1));
-    return node();
-  }
-  // The streaming kernels take few rows against a row-major b, and any a.
-  const bool stream = m <= 16 && (b.s_c == 1 || n == 1);
+  if (math == MMR_MATH_EXACT) return node(MMR_FAMILY_SIMT);  // sums in the node's own order
+  const bool stream = b.s_c == 1 && family(a, f32_aligned(b) ? b : packed_b, own_out, nullptr) == MMR_FAMILY_GEMV;
   int count = 1;
   if (!stream) {
     const int64_t tiles = m > 128 ? (m + 255) / 256 * ((n + 255) / 256) : (n + 255) / 256;
@@ -972,13 +1000,9 @@ int32_t add_f32_bare(Handle* h, int math, F32Mat a, F32Mat b, const F32Mat& out,
   if (!stream && (uneven || !f32_aligned(a))) MMR_TRY(pack(&a, true));
   if (uneven || !f32_aligned(b)) MMR_TRY(pack(&b, false));
   add_packs(h, packs, 4);
-  if (count == 1) {
-    if (out_free && (stream || (out.s_c == 1 && f32_aligned(out)))) use_out();
-    else MMR_TRY(use_workspace(1));
-    return node();
-  }
+  if (count == 1) return node(stream ? MMR_FAMILY_GEMV : MMR_FAMILY_TCGEN05);
   MMR_TRY(use_workspace(count));
-  mmr_view to = x_view();
+  mmr_view to = f32_view(x->p, m, n, x->ld, dev);
   to.rank = 3;
   to.dims[0] = count;
   to.dims[1] = m;
@@ -987,8 +1011,8 @@ int32_t add_f32_bare(Handle* h, int math, F32Mat a, F32Mat b, const F32Mat& out,
   to.strides[1] = x->ld;
   to.strides[2] = 1;
   to.bytes = 4 * uint64_t(count) * x->bs;
-  return add_f32_product(h, math, f32_parts_view(a, true, count, each, dev), f32_parts_view(b, false, count, each, dev),
-                         to, nullptr, MMR_EPI_NONE);
+  return add_f32_product(h, f32_desc(h, math, f32_parts_view(a, true, count, each, dev),
+                                     f32_parts_view(b, false, count, each, dev), to, nullptr));
 }
 
 // pre = sum of x's parts + bias; out = act(pre) + residual.
@@ -1084,7 +1108,7 @@ int32_t linear_bind(const mmr_linear_desc* d, Handle** out) {
     // bias and SiLU took 375 us in it, 256 bare.
     mmr::ActResParams q;
     const Ref& to = pre.on ? pre : o;
-    const bool to_free = (pre.on || !res.on || !overlap(o, res)) && apart(to, lhs) && apart(to, rhs);
+    const bool to_free = pre.on || !res.on || !overlap(o, res);
     const bool more = res.on || pre.on || d->activation != MMR_ACT_NONE;
     q.pre = epi_mat(pre);
     q.residual = epi_mat(res);
@@ -1157,9 +1181,8 @@ int32_t linear_grad_bind(const mmr_linear_grad_desc* d, Handle** out) {
   MMR_TRY(add_act_grad(h.get(), d->activation, dy, pre, db, &dp, nullptr, nullptr));
   if (dy.dtype == MMR_DTYPE_F32) {
     // out^T = B^T A^T where the gradient's unit stride is its row axis
-    auto product = [&](F32Mat a, F32Mat b, const Ref& o, const Ref& operand) -> int32_t {
+    auto product = [&](F32Mat a, F32Mat b, const Ref& o) -> int32_t {
       if (o.lo == o.hi) return MMR_OK;
-      const bool free = apart(o, dy) && apart(o, operand);
       F32Mat v = f32_mat(o);
       if (v.s_c != 1 && v.s_r == 1) {
         std::swap(a, b);
@@ -1176,13 +1199,13 @@ int32_t linear_grad_bind(const mmr_linear_grad_desc* d, Handle** out) {
       q.n = int(v.cols);
       if (add_f32_dot(h.get(), d->math_mode, a, b, MMR_ACT_NONE, q)) return MMR_OK;
       bool direct = false, biased = false;
-      MMR_TRY(add_f32_bare(h.get(), d->math_mode, a, b, v, free, nullptr, &q.x, &q.parts, &direct, &biased));
+      MMR_TRY(add_f32_bare(h.get(), d->math_mode, a, b, v, true, nullptr, &q.x, &q.parts, &direct, &biased));
       if (!direct) add_act_res(h.get(), MMR_ACT_NONE, q);
       return MMR_OK;
     };
     const F32Mat dpm = f32_mat(dp);
-    if (dl.on) MMR_TRY(product(dpm, f32_mat(rhs).t(), dl, rhs));
-    if (dr.on) MMR_TRY(product(f32_mat(lhs).t(), dpm, dr, lhs));
+    if (dl.on) MMR_TRY(product(dpm, f32_mat(rhs).t(), dl));
+    if (dr.on) MMR_TRY(product(f32_mat(lhs).t(), dpm, dr));
   } else {
     if (dl.on) MMR_TRY(add_plain_product(h.get(), dy.dtype, operand(dp, true), operand(rhs, true), dl));
     if (dr.on) MMR_TRY(add_plain_product(h.get(), dy.dtype, operand(lhs, false), operand(dp, false), dr));

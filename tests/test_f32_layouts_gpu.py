@@ -32,3 +32,59 @@ def test_column_blocks_of_one_buffer(m, node):
     kept = torch.ones(1024, dtype=torch.bool, device="cuda")
     kept[256:256 + n], kept[600:600 + k] = False, False
     assert torch.equal(wide[:, kept], before[:, kept])
+
+
+def planned(op):
+    """One run of `op`, which may not fall to the node's scalar kernel."""
+    assert "simt" not in op.plan, op.plan
+    replay(op)
+
+
+TF32 = mb.LinearNode(math_mode=mb.KernelMathMode.Tf32, accuracy=mb.AccuracyContract.AllowTf32)
+
+
+@pytest.mark.parametrize("m,n,k", [
+    (1, 1001, 11008), (1, 1000, 11008), (2, 130, 8193), (16, 500, 8193), (16, 77, 12000), (9, 515, 8192), (16, 1, 9000),
+    (9, 1, 900), (40, 1, 900), (200, 1, 4001), (1, 1, 9001), (17, 3, 5), (8200, 12, 40), (8195, 3, 9), (300, 1, 1)])
+def test_no_product_falls_to_the_scalar_kernel(m, n, k):
+    """Few rows with a long contraction, single columns, gradients of many rows: in both layouts of rhs."""
+    g = gen(m + n + k)
+    lhs, b, r, dy = rand(g, m, k), rand(g, n), rand(g, m, n), rand(g, m, n)
+    for tr in (False, True):
+        rhs = rand(g, *((n, k) if tr else (k, n)), scale=k ** -0.5)
+        b64 = (rhs.t() if tr else rhs).double()
+        want = lhs.double() @ b64
+        for node, bound in ((STRICT, 1e-5), (TF32, 2e-3)):
+            node = mb.LinearNode(transpose_rhs=tr, math_mode=node.math_mode, accuracy=node.accuracy)
+            out = torch.full((m, n), float("nan"), device="cuda")
+            planned(mb.BoundLinear(node, V(lhs), V(rhs), V(out)))
+            assert rel(out, want) <= bound
+            planned(mb.BoundLinear(node, V(lhs), V(rhs), V(out), bias=V(b), residual=V(r)))
+            assert rel(out, want + b.double() + r.double()) <= bound
+            d_lhs, d_rhs = torch.full_like(lhs, float("nan")), torch.full_like(rhs, float("nan"))
+            planned(mb.BoundLinearGrad(node, V(dy), V(lhs), V(rhs), d_lhs=V(d_lhs), d_rhs=V(d_rhs)))
+            assert rel(d_lhs, dy.double() @ b64.t()) <= bound
+            assert rel(d_rhs.t() if tr else d_rhs, lhs.double().t() @ dy.double()) <= bound
+
+
+@pytest.mark.parametrize("m", [1, 5, 12, 200])
+@pytest.mark.parametrize("k", [136, 8195])
+def test_strided_outputs_bias_and_reversed_rows(m, k):
+    """Every second column of a buffer, every second entry of a bias, an lhs read from its last row or column on."""
+    g = gen(m + k)
+    n = 260
+    lhs, rhs, bias = rand(g, m, k), rand(g, k, n, scale=k ** -0.5), rand(g, 2 * n)[::2]
+    want = lhs.double() @ rhs.double() + bias.double()
+    buf = torch.full((m, 2 * n), 7.0, device="cuda")
+    planned(mb.BoundLinear(STRICT, V(lhs), V(rhs), V(buf[:, ::2]), bias=V(bias)))
+    assert rel(buf[:, ::2], want) <= 1e-5 and bool((buf[:, 1::2] == 7).all())
+    out = torch.empty(m, n, device="cuda")
+    planned(mb.BoundLinear(STRICT, V(lhs), V(rhs), V(out), bias=V(bias)))
+    assert rel(out, want) <= 1e-5
+    v = V(lhs)
+    rows = mb.DeviceView(v.buffer, v.dims, (-k, 1), (m - 1) * k)
+    planned(mb.BoundLinear(STRICT, rows, V(rhs), V(out), bias=V(bias)))
+    assert rel(out, want.flip(0)) <= 1e-5
+    cols = mb.DeviceView(v.buffer, v.dims, (k, -1), k - 1)
+    planned(mb.BoundLinear(STRICT, cols, V(rhs), V(out)))
+    assert rel(out, lhs.double().flip(1) @ rhs.double()) <= 1e-5
