@@ -301,12 +301,15 @@ int32_t new_handle(int device, int sms, void* stream, Owned* out) {
   return MMR_OK;
 }
 
-int32_t workspace(Handle* h, size_t bytes, void** out) {
+// `bytes` in 128 bits: an operand broadcast over its axes (strides of 0) may be
+// larger to pack than 64 bits can say.
+int32_t workspace(Handle* h, __int128 bytes, void** out) {
+  if (bytes > (int64_t(1) << 48)) return fail(MMR_ERR_INVALID_SHAPE, "a workspace of %.3g bytes", double(bytes));
   void* p = nullptr;
-  const cudaError_t e = cudaMalloc(&p, std::max<size_t>(bytes, 256));
+  const cudaError_t e = cudaMalloc(&p, size_t(std::max<__int128>(bytes, 256)));
   if (e != cudaSuccess) {
     cudaGetLastError();
-    return fail(MMR_ERR_CUDA, "allocating a workspace of %zu bytes: %s", bytes, cudaGetErrorString(e));
+    return fail(MMR_ERR_CUDA, "allocating a workspace of %lld bytes: %s", (long long)bytes, cudaGetErrorString(e));
   }
   h->workspaces.push_back(p);
   *out = p;
@@ -407,7 +410,7 @@ int32_t admit(Handle* h, Operand* o, int major, const char* name, mmr::PackList*
   if (o->batch > 65535) return fail(MMR_ERR_UNSUPPORTED_LAYOUT, "%s: more than 65535 matrices to pack", name);
   const int64_t per = int64_t(q.rows) * q.pitch;
   q.batch = int(o->batch);
-  MMR_TRY(workspace(h, size_t(per) * o->batch * 2, &q.dst));
+  MMR_TRY(workspace(h, __int128(per) * o->batch * 2, &q.dst));
   packs->p[packs->n++] = q;
   o->base = reinterpret_cast<uint64_t>(q.dst);
   o->mn_major = mn_major;
@@ -700,14 +703,14 @@ int32_t add_act_grad(Handle* h, int act, const Ref& d_out, const Ref& pre, const
     d_pre->s[2] = 1;
     d_pre->s[1] = (n + 7) / 8 * 8;
     void* w = nullptr;
-    MMR_TRY(workspace(h, size_t(rows) * d_pre->s[1] * d_out.es, &w));
+    MMR_TRY(workspace(h, __int128(rows) * d_pre->s[1] * d_out.es, &w));
     d_pre->base = reinterpret_cast<uint64_t>(w);
     d_pre->name = "d_pre";
     p.d_pre = epi_mat(*d_pre);
   }
   if (d_bias.on) {
     void* w = nullptr;
-    MMR_TRY(workspace(h, size_t(chunks) * n * sizeof(float), &w));
+    MMR_TRY(workspace(h, __int128(chunks) * n * 4, &w));
     p.partial = static_cast<float*>(w);
   }
   const int dt = d_out.dtype;
@@ -916,7 +919,7 @@ int32_t add_f32_bare(Handle* h, int math, F32Mat a, F32Mat b, F32Mat out, bool o
   auto use_workspace = [&](int count) -> int32_t {
     const int64_t ld = (n + 3) / 4 * 4;
     void* w = nullptr;
-    MMR_TRY(workspace(h, size_t(count) * m * ld * 4, &w));
+    MMR_TRY(workspace(h, __int128(count) * m * ld * 4, &w));
     x->p = w;
     x->bs = m * ld;
     x->ld = ld;
@@ -989,7 +992,7 @@ int32_t add_f32_bare(Handle* h, int math, F32Mat a, F32Mat b, F32Mat out, bool o
     const bool k_inner = cols_inner == k_is_cols;
     q.pitch = int(((k_inner ? k_padded : int64_t(q.cols)) + 3) / 4 * 4);
     q.rows_out = int(k_inner ? int64_t(q.rows) : k_padded);
-    MMR_TRY(workspace(h, size_t(q.rows_out) * q.pitch * 4, &q.dst));
+    MMR_TRY(workspace(h, __int128(q.rows_out) * q.pitch * 4, &q.dst));
     packs.p[packs.n++] = q;
     o->base = reinterpret_cast<uint64_t>(q.dst);
     (cols_inner ? o->s_r : o->s_c) = q.pitch;
@@ -1331,7 +1334,7 @@ int32_t dispatch_bind(const mmr_dispatch_desc* d, Handle** out) {
   const int grid = int(std::max<int64_t>(need, std::min<int64_t>(2 * sms, 1 + l.rows / mmr::ES_WARPS)));
   if (l.tokens * l.top_k > mmr::ES_DIRECT) {
     void* w = nullptr;
-    MMR_TRY(workspace(h.get(), size_t(grid) * l.experts * 4, &w));
+    MMR_TRY(workspace(h.get(), __int128(grid) * l.experts * 4, &w));
     p.hist = static_cast<int*>(w);
     add_step(h.get(), "mmr_expert_hist_kernel grid %lld", [=](cudaStream_t s) {
       return mmr::launch_kernel(mmr::mmr_expert_hist_kernel, dim3(grid), dim3(mmr::ES_THREADS), p.experts * 4, s,
