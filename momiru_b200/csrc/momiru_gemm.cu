@@ -51,6 +51,35 @@ int32_t set_last_error(int32_t code, const char* message) {
   g_last_error = message;
   return code;
 }
+
+// What a bind writes to device memory has to be there before the first run,
+// which may be on any stream: cudaMemset and cudaMemcpy go to the legacy default
+// stream, which non-blocking streams do not wait for and whose own queue may be
+// long. So: on a non-blocking stream of the library's own, waited for here.
+static cudaError_t bind_stream(cudaStream_t* out) {
+  static std::mutex mu;
+  static std::vector<cudaStream_t> streams;  // by device
+  int dev = 0;
+  if (const cudaError_t e = cudaGetDevice(&dev)) return e;
+  std::lock_guard<std::mutex> lock(mu);
+  if (size_t(dev) >= streams.size()) streams.resize(dev + 1);
+  if (!streams[dev])
+    if (const cudaError_t e = cudaStreamCreateWithFlags(&streams[dev], cudaStreamNonBlocking)) return e;
+  *out = streams[dev];
+  return cudaSuccess;
+}
+cudaError_t bind_zero(void* p, size_t bytes) {
+  cudaStream_t s = nullptr;
+  cudaError_t e = bind_stream(&s);
+  if (e == cudaSuccess) e = cudaMemsetAsync(p, 0, bytes, s);
+  return e == cudaSuccess ? cudaStreamSynchronize(s) : e;
+}
+cudaError_t bind_copy(void* to, const void* from, size_t bytes) {
+  cudaStream_t s = nullptr;
+  cudaError_t e = bind_stream(&s);
+  if (e == cudaSuccess) e = cudaMemcpyAsync(to, from, bytes, cudaMemcpyHostToDevice, s);
+  return e == cudaSuccess ? cudaStreamSynchronize(s) : e;
+}
 }  // namespace mmr
 
 namespace {
@@ -1053,7 +1082,7 @@ int32_t mmr_gemm_bind(const mmr_matmul_desc* desc, mmr_gemm_handle** out) {
     return code;
   };
   if (cudaMalloc(&h->d_err, sizeof(int)) != cudaSuccess) return cleanup(fail(MMR_ERR_CUDA, "cudaMalloc(error word) failed"));
-  if (cudaMemset(h->d_err, 0, sizeof(int)) != cudaSuccess) return cleanup(fail(MMR_ERR_CUDA, "cudaMemset failed"));
+  if (mmr::bind_zero(h->d_err, sizeof(int)) != cudaSuccess) return cleanup(fail(MMR_ERR_CUDA, "zeroing the error word failed"));
   if (cudaHostAlloc(&h->h_err, sizeof(int), cudaHostAllocDefault) != cudaSuccess)
     return cleanup(fail(MMR_ERR_CUDA, "cudaHostAlloc failed"));
   *h->h_err = 0;
@@ -1108,7 +1137,7 @@ int32_t mmr_gemm_bind(const mmr_matmul_desc* desc, mmr_gemm_handle** out) {
     if (h->mode == 1) {
       const size_t words = 2 + 2 * size_t(L.tiles);
       if (cudaMalloc(&h->d_nf, words * sizeof(unsigned int)) != cudaSuccess ||
-          cudaMemset(h->d_nf, 0, words * sizeof(unsigned int)) != cudaSuccess)
+          mmr::bind_zero(h->d_nf, words * sizeof(unsigned int)) != cudaSuccess)
         return cleanup(fail(MMR_ERR_CUDA, "allocating the non-finite bookkeeping failed"));
       q.nf = h->d_nf;
       fill_simt_params(p, &h->sp);
@@ -1121,7 +1150,7 @@ int32_t mmr_gemm_bind(const mmr_matmul_desc* desc, mmr_gemm_handle** out) {
       h->ws_count_bytes = size_t(2 * L.npairs) * 2 * mmr::TC_EPI_WARPS * sizeof(unsigned int);
       if (cudaMalloc(&h->d_ws, ws_bytes) != cudaSuccess ||
           cudaMalloc(&h->d_ws_count, h->ws_count_bytes) != cudaSuccess ||
-          cudaMemset(h->d_ws_count, 0, h->ws_count_bytes) != cudaSuccess)
+          mmr::bind_zero(h->d_ws_count, h->ws_count_bytes) != cudaSuccess)
         return cleanup(fail(MMR_ERR_CUDA, "allocating the stream-K workspace failed"));
       q.ws = h->d_ws;
       q.ws_count = h->d_ws_count;
@@ -1749,7 +1778,7 @@ int32_t mmr_sharded_gemm_bind(const mmr_sharded_desc* d, mmr_gemm_handle** out) 
     }
     DeviceGuard guard(h->device);
     if (cudaMalloc(&h->d_peer_tm, sizeof(CUtensorMap) * size_t(q)) != cudaSuccess ||
-        cudaMemcpy(h->d_peer_tm, maps, sizeof(CUtensorMap) * size_t(q), cudaMemcpyHostToDevice) != cudaSuccess) {
+        mmr::bind_copy(h->d_peer_tm, maps, sizeof(CUtensorMap) * size_t(q)) != cudaSuccess) {
       mmr_gemm_destroy(h);
       return fail(MMR_ERR_CUDA, "storing the peer tensor maps failed");
     }

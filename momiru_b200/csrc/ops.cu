@@ -29,6 +29,7 @@
 namespace mmr {
 // momiru_gemm.cu
 int32_t set_last_error(int32_t code, const char* message);
+cudaError_t bind_zero(void* p, size_t bytes);
 void gemm_set_chunk(mmr_gemm_handle* h, int k);
 int32_t gemm_enqueue(mmr_gemm_handle* h, cudaStream_t s);
 int32_t gemm_read_error(mmr_gemm_handle* h, uint64_t timeout_ns);
@@ -292,7 +293,7 @@ int32_t new_handle(int device, int sms, void* stream, Owned* out) {
   h->sms = sms;
   h->stream = reinterpret_cast<cudaStream_t>(stream);
   MMR_CUDA(cudaMalloc(&h->d_err, 256));
-  MMR_CUDA(cudaMemset(h->d_err, 0, 256));
+  MMR_CUDA(mmr::bind_zero(h->d_err, 256));
   MMR_CUDA(cudaHostAlloc(&h->h_err, sizeof(int), cudaHostAllocDefault));
   *h->h_err = 0;
   MMR_CUDA(cudaEventCreateWithFlags(&h->done, cudaEventDisableTiming));
