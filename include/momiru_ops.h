@@ -35,7 +35,9 @@ enum {
   MMR_DTYPE_I32 = 3
 };
 
-/* ---- activations (the formulas of the MMR_EPI_* codes) */
+/* ---- activations: the functions of the MMR_EPI_* codes. f32 operands in
+ * MMR_MATH_EXACT evaluate them as the MatMul node does, bit for bit; the other
+ * modes and 16-bit operands in f32 arithmetic of their own */
 enum {
   MMR_ACT_NONE = 0,
   MMR_ACT_RELU = 1,

@@ -1019,12 +1019,18 @@ int32_t add_f32_bare(Handle* h, int math, F32Mat a, F32Mat b, F32Mat out, bool o
                                      f32_parts_view(b, false, count, each, dev), to, nullptr));
 }
 
-// pre = sum of x's parts + bias; out = act(pre) + residual.
-void add_act_res(Handle* h, int act, const mmr::ActResParams& q) {
+// pre = sum of x's parts + bias; out = act(pre) + residual. In EXACT mode the
+// activation is the node's, bit for bit.
+void add_act_res(Handle* h, int math, int act, const mmr::ActResParams& q) {
   const int grid = int(std::min<int64_t>((int64_t(q.m) * ((q.n + 127) / 128) + 7) / 8, 16 * h->sms));
   add_step(h, "mmr_act_res_kernel grid %lld, %lld parts", [=](cudaStream_t s) {
     using K = void (*)(const mmr::ActResParams);
-    const K k = pick_act(act, [](auto a) -> K { return mmr::mmr_act_res_kernel<decltype(a)::value>; });
+    const K k = pick_act(act, [&](auto a) -> K {
+      constexpr int kAct = decltype(a)::value;
+      if constexpr (kAct != MMR_ACT_NONE)
+        if (math == MMR_MATH_EXACT) return mmr::mmr_act_res_kernel<kAct, true>;
+      return mmr::mmr_act_res_kernel<kAct, false>;
+    });
     return mmr::launch_kernel(k, dim3(grid), dim3(256), 0, s, dim3(1, 1, 1), q);
   }, grid, q.parts);
 }
@@ -1125,7 +1131,7 @@ int32_t linear_bind(const mmr_linear_desc* d, Handle** out) {
       bool direct = false, biased = false;
       MMR_TRY(add_f32_bare(h.get(), d->math_mode, f32_mat(lhs), f32_mat(rhs), f32_mat(to), to_free,
                            more ? nullptr : &bias, &q.x, &q.parts, &direct, &biased));
-      if (!direct || more || (bias.on && !biased)) add_act_res(h.get(), d->activation, q);
+      if (!direct || more || (bias.on && !biased)) add_act_res(h.get(), d->math_mode, d->activation, q);
     }
   } else {
     mmr::EpiParams epi;
@@ -1204,7 +1210,7 @@ int32_t linear_grad_bind(const mmr_linear_grad_desc* d, Handle** out) {
       if (add_f32_dot(h.get(), d->math_mode, a, b, MMR_ACT_NONE, q)) return MMR_OK;
       bool direct = false, biased = false;
       MMR_TRY(add_f32_bare(h.get(), d->math_mode, a, b, v, true, nullptr, &q.x, &q.parts, &direct, &biased));
-      if (!direct) add_act_res(h.get(), MMR_ACT_NONE, q);
+      if (!direct) add_act_res(h.get(), d->math_mode, MMR_ACT_NONE, q);
       return MMR_OK;
     };
     const F32Mat dpm = f32_mat(dp);

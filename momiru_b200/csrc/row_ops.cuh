@@ -297,9 +297,10 @@ struct ActResParams {
 
 // The activations in f32, inlined (the matmul node's epilogue calls them out of
 // line): the formulas of linear_epi.cuh on CUDA's expf and normcdff and correctly
-// rounded divisions.
-template <int ACT>
+// rounded divisions. EXACT: the node's own, step by step (act_apply).
+template <int ACT, bool EXACT = false>
 __device__ __forceinline__ float act_f32(float x) {
+  if (EXACT) return act_apply(ACT, x);
   if (ACT == ACT_RELU) return act_relu(x);
   if (ACT == ACT_RELU6) return x != x ? x : fminf(fmaxf(x, 0.0f), 6.0f);
   if (ACT == ACT_SILU) return no_inf(x, __fdiv_rn(x, 1.0f + expf(-x)));
@@ -310,7 +311,7 @@ __device__ __forceinline__ float act_f32(float x) {
 
 // A warp takes 128 columns of a row, four columns a thread where everything is
 // 16-byte vectors.
-template <int ACT>
+template <int ACT, bool EXACT>
 __global__ void __launch_bounds__(256) mmr_act_res_kernel(const ActResParams p) {
   griddep_wait();
   griddep_release();
@@ -340,7 +341,7 @@ __global__ void __launch_bounds__(256) mmr_act_res_kernel(const ActResParams p) 
         v.w = __fadd_rn(v.w, p.bias[(c + 3) * p.bias_s]);
       }
       if (pre) *reinterpret_cast<float4*>(pre + row * p.pre.ld + c) = v;
-      v = make_float4(act_f32<ACT>(v.x), act_f32<ACT>(v.y), act_f32<ACT>(v.z), act_f32<ACT>(v.w));
+      v = make_float4(act_f32<ACT, EXACT>(v.x), act_f32<ACT, EXACT>(v.y), act_f32<ACT, EXACT>(v.z), act_f32<ACT, EXACT>(v.w));
       if (res) v = make_float4(v.x + r.x, v.y + r.y, v.z + r.z, v.w + r.w);
       *reinterpret_cast<float4*>(out + row * p.out.ld + c) = v;
     } else {
@@ -349,7 +350,7 @@ __global__ void __launch_bounds__(256) mmr_act_res_kernel(const ActResParams p) 
         for (int q = 1; q < p.parts; ++q) v += x[q * p.x.bs + row * p.x.ld + c * p.x.cs];
         if (p.bias) v = __fadd_rn(v, p.bias[c * p.bias_s]);
         if (pre) pre[row * p.pre.ld + c * p.pre.cs] = v;
-        v = act_f32<ACT>(v);
+        v = act_f32<ACT, EXACT>(v);
         if (res) v += res[row * p.residual.ld + c * p.residual.cs];
         out[row * p.out.ld + c * p.out.cs] = v;
       }

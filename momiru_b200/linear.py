@@ -7,8 +7,10 @@ epilogue, and its gradient.
 Beside the f32 MatMul node (execution.py) this takes bf16 and f16 operands
 (f32 sums, one rounding), adds the residual, and keeps `pre` for the gradient.
 Bound, replayed and quiesced as the MatMul node is; errors are its typed
-exceptions. The activations are the node's own (the reference CPU provider's
-elementwise kernels, src/momiru/tensor_light/execution/cpu.rs:2117-2222).
+exceptions. The activations are the node's (the reference CPU provider's
+elementwise kernels, src/momiru/tensor_light/execution/cpu.rs:2117-2222): bit
+for bit in KernelMathMode.Exact, the same functions in f32 arithmetic of their
+own in the other modes.
 """
 from __future__ import annotations
 
