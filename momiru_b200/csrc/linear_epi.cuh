@@ -17,8 +17,6 @@
 
 namespace mmr {
 
-
-
 template <typename T>
 __device__ __forceinline__ float to_f32(T x);
 template <>
@@ -49,13 +47,13 @@ __device__ __forceinline__ float fast_rcp(float x) {
   return y;
 }
 
-// Activations for 16-bit results, each of one exponential and one reciprocal
-// (good to about 2^-20, against the 2^-12 of an f16 rounding).
+// Activations for 16-bit results, each of one exponential and one reciprocal:
+// relative error below 2^-17 plus 2^-22 for every unit of the exponent (an
+// argument rounded in f32), against the 2^-12 of an f16 rounding.
 //   silu       x / (1 + e^-x)
 //   gelu_tanh  x (1 + tanh u) / 2 = x / (1 + e^-2u), u = sqrt(2/pi)(x + 0.044715 x^3):
 //              no 1 + tanh, which cancels for x < 0
-//   gelu_erf   x Phi(x) with erfc by Abramowitz & Stegun 7.1.26 (absolute
-//              error below 1.5e-7)
+//   gelu_erf   x Phi(x), by the tail Phi(-|x|) below
 // As in the f32 epilogue, -inf gives -0 (not inf times 0) and NaN stays NaN.
 constexpr float kLog2e = 1.4426950408890f;
 __device__ __forceinline__ float no_inf(float x, float y) { return x == -__int_as_float(0x7f800000) ? -0.0f : y; }
@@ -66,22 +64,28 @@ __device__ __forceinline__ float gelu_gate(float x) {
 }
 __device__ __forceinline__ float lact_silu(float x) { return no_inf(x, x * fast_sigmoid(x)); }
 __device__ __forceinline__ float lact_gelu_tanh(float x) { return no_inf(x, x * gelu_gate(x)); }
-// Phi(x) and e^(-x^2/2).
-__device__ __forceinline__ float normal_cdf(float x, float* gauss) {
-  const float t = fast_rcp(fmaf(0.3275911f * 0.70710678118655f, fabsf(x), 1.0f));
+// Phi(-|x|) and e^(-x^2/2). With z = |x| / sqrt 2 and t = 1 / (1 + 0.38 z),
+//   erfc(z) = t P(t) e^(-z^2),
+// P of degree 6 with the least largest relative error on 0 <= z <= 9.5, 1.0e-6
+// (found by linear programming over 6000 points): relative, so that x Phi(x)
+// keeps its bits where it runs out to the left. The coefficients are P's halves.
+__device__ __forceinline__ float normal_tail(float x, float* gauss) {
+  const float t = fast_rcp(fmaf(0.38f * 0.70710678118655f, fabsf(x), 1.0f));
   const float g = fast_exp2(-0.5f * kLog2e * x * x);
-  float p = fmaf(0.5f * 1.061405429f, t, 0.5f * -1.453152027f);
-  p = fmaf(p, t, 0.5f * 1.421413741f);
-  p = fmaf(p, t, 0.5f * -0.284496736f);
-  p = fmaf(p, t, 0.5f * 0.254829592f);
-  const float half_erfc = p * t * g;
+  float p = fmaf(-0.0625223433007686f, t, 0.1673000517084580f);
+  p = fmaf(p, t, -0.0338413079234745f);
+  p = fmaf(p, t, 0.1230267267987761f);
+  p = fmaf(p, t, 0.0906809299674027f);
+  p = fmaf(p, t, 0.1082044550110211f);
+  p = fmaf(p, t, 0.1071509821877172f);
   *gauss = g;
-  return x < 0.0f ? half_erfc : 1.0f - half_erfc;
+  return p * t * g;
 }
+// x Phi(x) = max(x, 0) - |x| Phi(-|x|); of an infinity the first term alone.
 __device__ __forceinline__ float lact_gelu_erf(float x) {
   float g;
-  const float c = normal_cdf(x, &g);
-  return no_inf(x, x * c);
+  const float tail = normal_tail(x, &g), rest = fmaxf(x, -0.0f);
+  return fabsf(x) == __int_as_float(0x7f800000) ? rest : fmaf(-fabsf(x), tail, rest);
 }
 
 template <int N>

@@ -126,9 +126,9 @@ __device__ __forceinline__ float lact_grad(int act, float x) {
   x = x > 1e4f ? 1e4f : (x < -1e4f ? -1e4f : x);
   if (act == ACT_GELU_ERF) {
     if (FAST) {
-      float g;
-      const float c = normal_cdf(x, &g);
-      return fmaf(0.39894228040143f * x, g, c);
+      float g;  // Phi(x) + x phi(x), which is 1 less its value at -|x| for x > 0
+      const float w = normal_tail(x, &g), left = fmaf(-0.39894228040143f * fabsf(x), g, w);
+      return x < 0.0f ? left : 1.0f - left;
     }
     return fmaf(0.39894228040143f * x, expf(-0.5f * x * x), normcdff(x));
   }
