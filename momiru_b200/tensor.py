@@ -190,7 +190,8 @@ class DeviceView:
 
     def copy_from_host(self, arr: np.ndarray) -> None:
         import torch
-        self.torch_view().copy_(torch.from_numpy(np.ascontiguousarray(arr, dtype=np.float32)))
+        host = np.int32 if self.dtype == DType.I32 else np.float32  # f32 holds no integer past 2^24
+        self.torch_view().copy_(torch.from_numpy(np.ascontiguousarray(arr, dtype=host)))
 
     # ------------------------------------------------------------------ ABI
     def to_abi(self) -> _abi.MmrView:
