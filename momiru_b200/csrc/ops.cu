@@ -108,7 +108,8 @@ struct DeviceGuard {
   } while (0)
 
 // ---------------------------------------------------------------- tensors --
-bool present(const mmr_tensor& t) { return t.view.rank > 0; }
+// Absent: rank 0 and no address. A scalar, or a negative rank, is present and refused.
+bool present(const mmr_tensor& t) { return t.view.rank != 0 || t.view.address != 0; }
 
 int elem_size(int dtype) { return dtype == MMR_DTYPE_BF16 || dtype == MMR_DTYPE_F16 ? 2 : 4; }
 
