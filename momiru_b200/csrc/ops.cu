@@ -984,7 +984,7 @@ int32_t add_f32_bare(Handle* h, int math, F32Mat a, F32Mat b, F32Mat out, bool o
   const int64_t each = uneven ? ((k + count - 1) / count + 15) / 16 * 16 : k / count, k_padded = uneven ? each * count : k;
   mmr::PackList packs;
   auto pack = [&](F32Mat* o, bool k_is_cols) -> int32_t {
-    const bool cols_inner = std::abs(o->s_c) <= std::abs(o->s_r);
+    const bool cols_inner = stream || std::abs(o->s_c) <= std::abs(o->s_r);  // streaming: a row-major b
     mmr::PackParams q;
     q.src = reinterpret_cast<const void*>(o->base);
     q.rows = int(cols_inner ? o->rows : o->cols);

@@ -88,3 +88,21 @@ def test_strided_outputs_bias_and_reversed_rows(m, k):
     cols = mb.DeviceView(v.buffer, v.dims, (k, -1), k - 1)
     planned(mb.BoundLinear(STRICT, cols, V(rhs), V(out)))
     assert rel(out, lhs.double().flip(1) @ rhs.double()) <= 1e-5
+
+
+@pytest.mark.parametrize("m", [1, 12, 16, 40])
+def test_repeated_rows_and_columns(m):
+    """Operands broadcast along one of their axes (a stride of 0)."""
+    g = gen(m)
+    n, k = 528, 4163
+    lhs, row, col = rand(g, m, k, scale=k ** -0.5), rand(g, n), rand(g, k)
+    out = torch.empty(m, n, device="cuda")
+    repeated = mb.DeviceView(V(row).buffer, (k, n), (0, 1))
+    planned(mb.BoundLinear(STRICT, V(lhs), repeated, V(out)))
+    # the sums over lhs cancel: the error is that of the absolute sums
+    want, size = lhs.double().sum(1, keepdim=True) * row.double(), lhs.double().abs().sum(1, keepdim=True) * row.double().abs()
+    assert float((out.double() - want).norm() / size.norm()) <= 1e-5
+    repeated = mb.DeviceView(V(col).buffer, (k, n), (1, 0))
+    planned(mb.BoundLinear(STRICT, V(lhs), repeated, V(out)))
+    want, size = (lhs.double() @ col.double())[:, None].expand(m, n), (lhs.double().abs() @ col.double().abs())[:, None].expand(m, n)
+    assert float((out.double() - want).norm() / size.norm()) <= 1e-5
