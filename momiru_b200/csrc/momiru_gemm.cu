@@ -637,9 +637,13 @@ cudaError_t launch_gemv_mt(const mmr_gemm_handle* h, cudaStream_t s) {
                             dim3(1, mmr::GV_KSPLIT, 1), h->tmB, h->gvp);
 }
 
+// The limit belongs to the function, which handles of every K share: always the
+// largest slice's.
 template <int MT>
-cudaError_t prepare_gemv_mt(int smem) {
-  cudaError_t e = cudaFuncSetAttribute(mmr::mmr_gemv_cluster_kernel<MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+cudaError_t prepare_gemv_mt() {
+  constexpr int most = mmr::gemv_smem_bytes(MT, mmr::GV_MAX_KSLICE);
+  static_assert(most <= 227 * 1024, "shared memory");
+  cudaError_t e = cudaFuncSetAttribute(mmr::mmr_gemv_cluster_kernel<MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
   if (e != cudaSuccess) return e;
   return cudaFuncSetAttribute(mmr::mmr_gemv_cluster_kernel<MT>, cudaFuncAttributeNonPortableClusterSizeAllowed, 0);
 }
@@ -659,13 +663,13 @@ cudaError_t launch_gemv(const mmr_gemm_handle* h, cudaStream_t s) {
     default: return launch_gemv_mt<16>(h, s);
   }
 }
-cudaError_t prepare_gemv(int mt, int smem) {
+cudaError_t prepare_gemv(int mt) {
   switch (mt) {
-    case 1: return prepare_gemv_mt<1>(smem);
-    case 2: return prepare_gemv_mt<2>(smem);
-    case 4: return prepare_gemv_mt<4>(smem);
-    case 8: return prepare_gemv_mt<8>(smem);
-    default: return prepare_gemv_mt<16>(smem);
+    case 1: return prepare_gemv_mt<1>();
+    case 2: return prepare_gemv_mt<2>();
+    case 4: return prepare_gemv_mt<4>();
+    case 8: return prepare_gemv_mt<8>();
+    default: return prepare_gemv_mt<16>();
   }
 }
 
@@ -1224,7 +1228,7 @@ int32_t mmr_gemm_bind(const mmr_matmul_desc* desc, mmr_gemm_handle** out) {
                               false, true))
       return cleanup(e);
     h->gv_mt = L.gv_mt;
-    cudaError_t ce = prepare_gemv(h->gv_mt, h->smem);
+    cudaError_t ce = prepare_gemv(h->gv_mt);
     if (ce != cudaSuccess) return cleanup(fail(MMR_ERR_CUDA, "cudaFuncSetAttribute(gemv): %s", cudaGetErrorString(ce)));
     h->info.bytes = algorithmic_bytes(p, true, true);
     h->info.cluster = mmr::GV_KSPLIT;
