@@ -87,7 +87,7 @@ static __global__ void __launch_bounds__(ES_THREADS) mmr_expert_hist_kernel(cons
 
 // Shared memory: total[E], before[E] (then the run's next row per expert),
 // start[E + 1], and per-warp counts [ES_WARPS][E].
-inline int dispatch_smem_bytes(int experts) { return 4 * (3 * experts + 1 + ES_WARPS * experts); }
+constexpr int dispatch_smem_bytes(int experts) { return 4 * (3 * experts + 1 + ES_WARPS * experts); }
 
 template <int VB>
 __global__ void __launch_bounds__(ES_THREADS) mmr_dispatch_kernel(const DispatchParams p) {

@@ -1350,11 +1350,9 @@ int32_t dispatch_bind(const mmr_dispatch_desc* d, Handle** out) {
     }, grid);
   }
   const int smem = mmr::dispatch_smem_bytes(p.experts);
+  static_assert(mmr::dispatch_smem_bytes(mmr::ES_MAX_EXPERTS) <= 48 * 1024, "more than a launch has without asking");
   auto kernel = vb == 16 ? mmr::mmr_dispatch_kernel<16> : vb == 8 ? mmr::mmr_dispatch_kernel<8>
                 : vb == 4 ? mmr::mmr_dispatch_kernel<4> : mmr::mmr_dispatch_kernel<2>;
-  if (smem > 48 * 1024)  // the function's limit, shared by handles of every size
-    MMR_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(kernel), cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                  mmr::dispatch_smem_bytes(mmr::ES_MAX_EXPERTS)));
   add_step(h.get(), "mmr_dispatch_kernel grid %lld, %lld-byte vectors", [=](cudaStream_t s) {
     return mmr::launch_kernel(kernel, dim3(grid), dim3(mmr::ES_THREADS), smem, s, dim3(1, 1, 1), p);
   }, grid, vb);
