@@ -79,8 +79,9 @@ typedef struct mmr_linear_desc {
  * d_rhs = lhs^T d_pre;  d_bias = column sums of d_pre (f32 sums). The
  * residual's gradient is d_out itself. d_lhs, d_rhs (in the layouts of lhs and
  * rhs) and d_bias are each optional, one at least present; `pre` is needed
- * where there is an activation. d_pre is held in the operands' type between
- * its two products. */
+ * where there is an activation. d_pre is held in the operands' type between it
+ * and the two products: rounded once more, and with that type's range (an f16
+ * d_pre above 65504 is infinite). */
 typedef struct mmr_linear_grad_desc {
   mmr_tensor d_out, lhs, rhs, pre, d_lhs, d_rhs, d_bias;
   int32_t transpose_lhs, transpose_rhs;

@@ -32,8 +32,8 @@
 //
 // Bound: the tensor pipe. A tile of 4096 k takes 33.3 thousand cycles against
 // 32.8 of MMAs; the clock under that load is the power cap's. 4096 x 11008 x
-// 4096: 1.53 PFLOP/s in a short run (1.63 GHz), 1.29 after a second of it (1.27
-// GHz; the library's product 1.30 on the same box).
+// 4096: 1.52 PFLOP/s in a short run, 1.31 after a second of it (the library's
+// product 1.55 and 1.34 on the same box).
 //
 // Warps: 0-7 epilogue (TMEM lane quarter = 32 columns, every second box of 32
 // rows), 8 TMA producer, 9 MMA

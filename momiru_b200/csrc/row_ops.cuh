@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(256) mmr_act_res_kernel(const ActResParams p) 
 // pre = a b^T + bias; out = act(pre) + residual, b contiguous along k and a of at
 // most eight rows: a warp takes a row of b, read once, against all rows of a
 // (which stay in L1), and lane i finishes row i. Bound by b's bytes: 1 x 16384 x
-// 4096 41.9 us, 6.4 TB/s. The MatMul node's streaming kernels want b row-major;
+// 4096 42 to 45 us by the box, 6.0 to 6.4 TB/s. The MatMul node's streaming kernels want b row-major;
 // its tensor-core kernel took 184 us at 1 x 4096 x 4096.
 struct DotParams {
   const float *a = nullptr, *b = nullptr;

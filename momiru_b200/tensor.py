@@ -84,7 +84,7 @@ class DeviceBuffer:
 class DeviceView:
     buffer: DeviceBuffer
     dims: tuple
-    strides: tuple          # element strides (>= 0)
+    strides: tuple          # element strides (signed)
     offset: int = 0         # element offset of [0, .., 0]
     dtype: DType = DType.F32
 
